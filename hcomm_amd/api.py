@@ -37,6 +37,9 @@ __all__ = [
     "DoubleRingReduceScatterPlan", "dbring_rs_emit", "dbring_rs_check",
     "DoubleRingHierReduceScatterPlan", "dbring_hier_rs_emit", "dbring_hier_rs_check",
     "HcommGfxAllReduceLocalReduceNoAlloc", "NOALLOC_SCRATCH_BYTES", "NOALLOC_MAX_RANKS",
+    "MxView", "mx_views", "HcommGfxMxQuantizeOnThread", "HcommGfxMxReduceKOnThread", "HcommGfxMxProductKOnThread",
+    "MX_BLOCK", "ReduceNormDesc", "ReduceNormGradDesc", "HcommGfxReduceNormOnThread", "HcommGfxReduceNormGradOnThread",
+    "reduce_norm_grad_workspace_bytes", "NORM_MAX_COLS",
     "OpBasePlan", "OpListPlan", "opbase_emit", "opbase_check", "opbase_max_count", "BUF_USER_IN", "BUF_USER_OUT",
 ]
 
@@ -88,7 +91,7 @@ class Lowering:
 
 
 class Kernel:
-    COPY, REDUCE2, CHAIN, TREE, BYTEWISE = range(5)
+    COPY, REDUCE2, CHAIN, TREE, BYTEWISE, MX_QUANTIZE, MX_REDUCE, MX_PRODUCT, NORM, NORM_GRAD, NORM_SUMS = range(11)
 
 
 class LaunchRecord(C.Structure):
@@ -938,3 +941,61 @@ class HierPlan(Plan):
         info = PlanInfo()
         check(_plan_info(self._p, C.byref(info)), "HcommGfxHierPlanGetInfo")
         self.info = info
+
+
+# ---- operators around a fold ---------------------------------------------------------------------------------------
+
+MX_BLOCK = 32
+NORM_MAX_COLS = 16384
+
+
+class MxView(C.Structure):
+    """HcommGfxMxView: where a matrix in microscaled 4-bit floating point lies (strides in bytes)."""
+    _fields_ = [("packed", _vp), ("scales", _vp), ("packedStride", _u64), ("scaleStride", _u64)]
+
+
+def mx_views(items):
+    """An array of MxView from (packed pointer, packed stride, scales pointer, scale stride) tuples, one for each rank."""
+    return (MxView * len(items))(*[MxView(p, s, ps, ss) for p, ps, s, ss in items])
+
+
+# out, again, srcs, a and b take an MxView, an array of them or None
+HcommGfxMxQuantizeOnThread = _sig("HcommGfxMxQuantizeOnThread", _i32, _u64, C.POINTER(MxView), _vp, _u64, _u64, _u64, C.c_int)
+HcommGfxMxReduceKOnThread = _sig("HcommGfxMxReduceKOnThread", _i32, _u64, _vp, _u64, C.c_int, C.POINTER(MxView),
+                                 C.POINTER(MxView), _u32, _vp, _u64, _u64, _u64)
+HcommGfxMxProductKOnThread = _sig("HcommGfxMxProductKOnThread", _i32, _u64, _vp, _u64, C.c_int, C.POINTER(MxView),
+                                  C.POINTER(MxView), _u32, _u64, _u64, _u64)
+
+
+class ReduceNormDesc(C.Structure):
+    """HcommGfxReduceNormDesc; srcs is a list of pointers and sets k."""
+    _fields_ = [("rows", _u64), ("cols", _u64), ("dataType", C.c_int), ("paramType", C.c_int), ("k", _u32),
+                ("residualScale", C.c_float), ("eps", C.c_float), ("reserved", _u32), ("rowsPerGate", _u64),
+                ("srcs", C.POINTER(_vp)), ("srcStride", _u64), ("residual", _vp), ("residualStride", _u64),
+                ("postWeight", _vp), ("preWeight", _vp), ("gate", _vp), ("gateStride", _u64),
+                ("sum", _vp), ("sumStride", _u64), ("y", _vp), ("yStride", _u64), ("z", _vp), ("zStride", _u64)]
+
+    def __init__(self, srcs=(), **fields):
+        super().__init__(k=len(srcs), srcs=(_vp * max(len(srcs), 1))(*srcs), **fields)
+
+
+class ReduceNormGradDesc(C.Structure):
+    """HcommGfxReduceNormGradDesc."""
+    _fields_ = [("rows", _u64), ("cols", _u64), ("dataType", C.c_int), ("paramType", C.c_int),
+                ("residualScale", C.c_float), ("eps", C.c_float), ("rowsPerGate", _u64),
+                ("sum", _vp), ("sumStride", _u64), ("y", _vp), ("yStride", _u64), ("dy", _vp), ("dyStride", _u64),
+                ("dz", _vp), ("dzStride", _u64), ("postWeight", _vp), ("preWeight", _vp), ("gate", _vp),
+                ("gateStride", _u64), ("dSum", _vp), ("dSumStride", _u64), ("dResidual", _vp),
+                ("dResidualStride", _u64), ("dPostWeight", _vp), ("dPreWeight", _vp), ("dGate", _vp),
+                ("dGateStride", _u64), ("workspace", _vp), ("workspaceBytes", _u64)]
+
+
+HcommGfxReduceNormOnThread = _sig("HcommGfxReduceNormOnThread", _i32, _u64, C.POINTER(ReduceNormDesc))
+HcommGfxReduceNormGradOnThread = _sig("HcommGfxReduceNormGradOnThread", _i32, _u64, C.POINTER(ReduceNormGradDesc))
+_norm_grad_workspace = _sig("HcommGfxReduceNormGradWorkspaceBytes", _i32, C.POINTER(ReduceNormGradDesc), C.POINTER(_u64))
+
+
+def reduce_norm_grad_workspace_bytes(desc):
+    n = _u64(0)
+    check(_norm_grad_workspace(C.byref(desc), C.byref(n)), "HcommGfxReduceNormGradWorkspaceBytes")
+    return n.value

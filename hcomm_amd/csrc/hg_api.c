@@ -288,18 +288,24 @@ int32_t HcommGfxThreadSynchronize(ThreadHandle thread)
 
 /* ---- launch log and submission ---------------------------------------------------------------------- */
 
-static void log_launch(HgThread* t, const HgLaunch* l, int backwards)
+static HcommGfxLaunchRecord* log_next(HgThread* t)
 {
-    if (!t->log_enabled || t->log_n >= HG_LOG_MAX) return;
+    if (!t->log_enabled || t->log_n >= HG_LOG_MAX) return NULL;
     if (t->log_n == t->log_cap) {
-        if (t->log_fixed) return;
+        if (t->log_fixed) return NULL;
         uint32_t cap = t->log_cap ? t->log_cap * 2 : 64;
         HcommGfxLaunchRecord* p = (HcommGfxLaunchRecord*)realloc(t->log, cap * sizeof(*p));
-        if (!p) return;
+        if (!p) return NULL;
         t->log = p;
         t->log_cap = cap;
     }
-    HcommGfxLaunchRecord* r = &t->log[t->log_n++];
+    return &t->log[t->log_n++];
+}
+
+static void log_launch(HgThread* t, const HgLaunch* l, int backwards)
+{
+    HcommGfxLaunchRecord* r = log_next(t);
+    if (!r) return;
     r->kind = l->kind;
     r->dtype = l->dtype;
     r->op = l->op;
@@ -406,6 +412,17 @@ int hg_submit(HgThread* t, const HgLaunch* l)
                                   l->lds_bytes);
         default: return HCCL_E_INTERNAL;
     }
+}
+
+int hg_submit_other(HgThread* t, const HcommGfxLaunchRecord* rec, int (*launch)(void* stream, const void* args), const void* args)
+{
+    HcommGfxLaunchRecord* r = log_next(t);
+    if (r) *r = *rec;
+    if (t->recorder) return HCCL_SUCCESS;
+    const int rc = hg_thread_settle(t);
+    if (rc != HCCL_SUCCESS) return rc;
+    t->own_work = 1;
+    return launch(t->stream, args);
 }
 
 int32_t HcommGfxLaunchLogRead(ThreadHandle thread, HcommGfxLaunchRecord* out, uint32_t cap, uint32_t* n)

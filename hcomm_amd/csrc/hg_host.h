@@ -109,6 +109,8 @@ void hg_finish_fold(HgLaunch* l);
 
 /* Execute (or, on a recorder thread, log) one prepared launch. */
 int hg_submit(HgThread* t, const HgLaunch* l);
+/* The same for a launch that is not made of segments: `rec` is what the log receives, `launch` gets the thread's stream. */
+int hg_submit_other(HgThread* t, const HcommGfxLaunchRecord* rec, int (*launch)(void* stream, const void* args), const void* args);
 /* Append one prepared launch to the thread's log without executing it. */
 void hg_log_only(HgThread* t, const HgLaunch* l);
 

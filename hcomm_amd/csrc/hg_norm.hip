@@ -1,0 +1,410 @@
+// hg_norm.hip - what follows the fold of a tensor-parallel block, and its gradient.
+//
+// One pass over memory: the wavefronts that share a row keep it in registers (eight elements a lane and group, 64 lanes a
+// wavefront), so k partials and the residual are read once, the sums over the row cross the lanes twice and everything
+// in between never leaves the registers.  Bound by memory from a few hundred rows on; a single row is bound by the latency of
+// its load, two reductions and store.
+#include "hg_ops_device.hpp"
+
+namespace {
+
+// ---- sums over a row ------------------------------------------------------------------------------------------------
+
+template <int CTRL> __device__ __forceinline__ float plus_dpp(float v)
+{
+    return v + bits_f32((uint32_t)__builtin_amdgcn_mov_dpp((int)f32_bits(v), CTRL, 0xf, 0xf, true));
+}
+
+// the sum over the wavefront, in every lane: inside the rows of 16 lanes by lane exchanges, across them by scalar reads
+__device__ __forceinline__ float wave_sum(float v)
+{
+    v = plus_dpp<0xB1>(v);  // 1 0 3 2
+    v = plus_dpp<0x4E>(v);  // 2 3 0 1
+    v = plus_dpp<0x141>(v); // mirrored in 8
+    v = plus_dpp<0x140>(v); // mirrored in 16
+    const float a = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), 0)), b = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), 16));
+    const float c = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), 32)), d = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), 48));
+    return (a + b) + (c + d);
+}
+
+// N sums over the wavefronts of a row, the same in all of them.  `box` holds N floats for each wavefront of the workgroup
+// and is not written again before every wavefront has passed another barrier.
+template <uint32_t N> __device__ __forceinline__ void row_sum(float (&v)[N], float* box, uint32_t waves)
+{
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+    if (waves == 1u) return;
+    const uint32_t wave = threadIdx.x >> 6, first = wave / waves * waves; // of this row
+    if ((threadIdx.x & 63u) == 0u) {
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) box[wave * N + i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) v[i] = 0.0f;
+    for (uint32_t w = 0; w < waves; ++w) {
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) v[i] += box[(first + w) * N + i];
+    }
+}
+
+__device__ __forceinline__ float inverse_rms(float squares, uint64_t cols, float eps) { return 1.0f / sqrtf(squares / (float)cols + eps); }
+
+#define MAX_WAVES 16u
+
+// ---- forward --------------------------------------------------------------------------------------------------------
+
+// DT: type of the matrices, PT: of the parameters, V: groups of eight elements a lane holds
+template <int DT, int PT, uint32_t V> __global__ __launch_bounds__(1024) void k_norm(const HgNorm a)
+{
+    __shared__ float box[2][MAX_WAVES];
+    constexpr uint32_t ES = ElemSize<DT>::v, PS = ElemSize<PT>::v, AHEAD = 4;
+    const uint32_t span = a.waves * 64u, local = threadIdx.x / span, t = threadIdx.x - local * span;
+    const uint64_t row = (uint64_t)blockIdx.x * a.rows_per_wg + local;
+    const uint64_t cols = row < a.d.rows ? a.d.cols : 0u; // a row that is not there has no columns
+    const uint32_t gate_row = a.d.gate && cols ? (uint32_t)row / (uint32_t)a.d.rowsPerGate : 0u; // the host keeps both below 2^31
+    float f[V][8];
+    for (uint32_t j0 = 0; j0 < a.d.k; j0 += AHEAD) {
+        Raw8<DT> x[AHEAD][V];
+#pragma unroll
+        for (uint32_t j = 0; j < AHEAD; ++j)
+            if (j0 + j < a.d.k) {
+#pragma unroll
+                for (uint32_t v = 0; v < V; ++v)
+                    x[j][v] = load8<DT>((const uint8_t*)a.src[j0 + j] + row * a.d.srcStride * ES, (v * span + t) * 8u, cols);
+            }
+#pragma unroll
+        for (uint32_t j = 0; j < AHEAD; ++j)
+            if (j0 + j < a.d.k) {
+#pragma unroll
+                for (uint32_t v = 0; v < V; ++v) {
+                    float g[8];
+                    widen8<DT>(x[j][v], g);
+#pragma unroll
+                    for (uint32_t e = 0; e < 8u; ++e) f[v][e] = j0 + j == 0u ? g[e] : f[v][e] + g[e];
+                }
+            }
+    }
+    Raw8<DT> res[V];
+    Raw8<PT> post[V], pre[V], gate[V];
+#pragma unroll
+    for (uint32_t v = 0; v < V; ++v) {
+        const uint32_t at = (v * span + t) * 8u;
+        if (a.d.residual) res[v] = load8<DT>((const uint8_t*)a.d.residual + row * a.d.residualStride * ES, at, cols);
+        if (a.d.postWeight) post[v] = load8<PT>(a.d.postWeight, at, cols);
+        if (a.d.preWeight) pre[v] = load8<PT>(a.d.preWeight, at, cols);
+        if (a.d.gate) gate[v] = load8<PT>((const uint8_t*)a.d.gate + (uint64_t)gate_row * a.d.gateStride * PS, at, cols);
+    }
+    if (a.d.sum) {
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v)
+            store8<DT>((uint8_t*)a.d.sum + row * a.d.sumStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(f[v]));
+    }
+    if (a.d.postWeight) {
+        float s[1] = {0.0f};
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v)
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) s[0] = fmaf(f[v][e], f[v][e], s[0]);
+        row_sum(s, box[0], a.waves);
+        const float r = inverse_rms(s[0], a.d.cols, a.d.eps);
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v) {
+            float w[8];
+            widen8<PT>(post[v], w);
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) f[v][e] = f[v][e] * r * w[e];
+        }
+    }
+    float s[1] = {0.0f};
+#pragma unroll
+    for (uint32_t v = 0; v < V; ++v) {
+        if (a.d.gate) {
+            float w[8];
+            widen8<PT>(gate[v], w);
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) f[v][e] *= w[e];
+        }
+        if (a.d.residual) {
+            float x[8];
+            widen8<DT>(res[v], x);
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) f[v][e] = fmaf(a.d.residualScale, x[e], f[v][e]);
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) s[0] = fmaf(f[v][e], f[v][e], s[0]);
+        store8<DT>((uint8_t*)a.d.y + row * a.d.yStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(f[v]));
+    }
+    if (a.d.preWeight) {
+        row_sum(s, box[1], a.waves);
+        const float r = inverse_rms(s[0], a.d.cols, a.d.eps);
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v) {
+            float w[8];
+            widen8<PT>(pre[v], w);
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) f[v][e] = f[v][e] * r * w[e];
+            store8<DT>((uint8_t*)a.d.z + row * a.d.zStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(f[v]));
+        }
+    }
+}
+
+// ---- gradient ---------------------------------------------------------------------------------------------------------
+
+template <int DT, int PT, uint32_t V, uint32_t MOST> __global__ __launch_bounds__(MOST) void k_norm_grad(const HgNormGrad a)
+{
+    __shared__ float box_a[MAX_WAVES * 3], box_b[MAX_WAVES];
+    constexpr uint32_t ES = ElemSize<DT>::v, PS = ElemSize<PT>::v;
+    const uint32_t span = a.waves * 64u, t = threadIdx.x;
+    const uint64_t cols = a.d.cols;
+    const bool has_post = a.d.postWeight != nullptr, has_pre = a.d.preWeight != nullptr, has_gate = a.d.gate != nullptr;
+    uint64_t row, end;
+    if (a.by_gate) {
+        const uint32_t per = (uint32_t)a.chunks_per_gate;
+        const uint64_t g = blockIdx.x / per, part = blockIdx.x % per;
+        const uint64_t g_end = min((g + 1u) * a.d.rowsPerGate, a.d.rows);
+        row = g * a.d.rowsPerGate + part * a.chunk_rows;
+        end = min(row + a.chunk_rows, g_end);
+    } else {
+        row = (uint64_t)blockIdx.x * a.chunk_rows;
+        end = min(row + a.chunk_rows, a.d.rows);
+    }
+    Raw8<PT> post[V], pre[V], gate[V];
+    float d_post[V][8], d_pre[V][8], d_gate[V][8];
+#pragma unroll
+    for (uint32_t v = 0; v < V; ++v) {
+        if (has_post) post[v] = load8<PT>(a.d.postWeight, (v * span + t) * 8u, cols);
+        if (has_pre) pre[v] = load8<PT>(a.d.preWeight, (v * span + t) * 8u, cols);
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) d_post[v][e] = d_pre[v][e] = d_gate[v][e] = 0.0f;
+    }
+    const float each = 1.0f / (float)cols;
+    uint64_t gate_row = has_gate && row < end ? (uint32_t)row / (uint32_t)a.d.rowsPerGate : 0u, gate_end = 0u; // row at which the next gate row begins
+    if (has_gate) {
+        gate_end = (gate_row + 1u) * a.d.rowsPerGate;
+        if (row < end) {
+#pragma unroll
+            for (uint32_t v = 0; v < V; ++v) gate[v] = load8<PT>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols);
+        }
+    }
+    for (; row < end; ++row) {
+        Raw8<DT> xs[V], xy[V], xd[V], xz[V];
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v) {
+            const uint32_t at = (v * span + t) * 8u;
+            xs[v] = load8<DT>((const uint8_t*)a.d.sum + row * a.d.sumStride * ES, at, cols);
+            xd[v] = load8<DT>((const uint8_t*)a.d.dy + row * a.d.dyStride * ES, at, cols);
+            if (has_pre) {
+                xy[v] = load8<DT>((const uint8_t*)a.d.y + row * a.d.yStride * ES, at, cols);
+                xz[v] = load8<DT>((const uint8_t*)a.d.dz + row * a.d.dzStride * ES, at, cols);
+            }
+        }
+        float q[3] = {0.0f, 0.0f, 0.0f}; // sum^2, y^2, dz preWeight y
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v) {
+            float s[8];
+            widen8<DT>(xs[v], s);
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) q[0] = fmaf(s[e], s[e], q[0]);
+            if (has_pre) {
+                float y[8], z[8], w[8];
+                widen8<DT>(xy[v], y);
+                widen8<DT>(xz[v], z);
+                widen8<PT>(pre[v], w);
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; ++e) q[1] = fmaf(y[e], y[e], q[1]), q[2] = fmaf(z[e] * w[e], y[e], q[2]);
+            }
+        }
+        row_sum(q, box_a, a.waves);
+        const float r1 = inverse_rms(q[0], cols, a.d.eps), r2 = has_pre ? inverse_rms(q[1], cols, a.d.eps) : 0.0f;
+        const float c2 = r2 * (q[2] * each); // mean of dz preWeight y / rms(y): r2 alone never underflows, its powers do
+        float g1[V][8]; // g D postWeight, or g D
+        float p[1] = {0.0f};
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v) {
+            float s[8], d[8];
+            widen8<DT>(xs[v], s);
+            widen8<DT>(xd[v], d);
+            if (has_pre) {
+                float y[8], z[8], w[8];
+                widen8<DT>(xy[v], y);
+                widen8<DT>(xz[v], z);
+                widen8<PT>(pre[v], w);
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; ++e) {
+                    const float n = y[e] * r2;
+                    d_pre[v][e] = fmaf(z[e], n, d_pre[v][e]);
+                    d[e] = fmaf(r2, fmaf(z[e], w[e], -c2 * n), d[e]);
+                }
+            }
+            if (a.d.dResidual) {
+                float x[8];
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; ++e) x[e] = a.d.residualScale * d[e];
+                store8<DT>((uint8_t*)a.d.dResidual + row * a.d.dResidualStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(x));
+            }
+            float w1[8], g[8];
+            if (has_post) widen8<PT>(post[v], w1);
+            if (has_gate) widen8<PT>(gate[v], g);
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) {
+                const float n = has_post ? s[e] * r1 : s[e];
+                if (has_gate) {
+                    d_gate[v][e] = fmaf(d[e], has_post ? n * w1[e] : n, d_gate[v][e]);
+                    d[e] *= g[e];
+                }
+                if (has_post) {
+                    d_post[v][e] = fmaf(d[e], n, d_post[v][e]);
+                    d[e] *= w1[e];
+                    p[0] = fmaf(d[e], s[e], p[0]);
+                }
+                g1[v][e] = d[e];
+            }
+        }
+        if (has_post) {
+            row_sum(p, box_b, a.waves);
+            const float c1 = r1 * (p[0] * each);
+#pragma unroll
+            for (uint32_t v = 0; v < V; ++v) {
+                float s[8];
+                widen8<DT>(xs[v], s);
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; ++e) g1[v][e] = r1 * fmaf(-c1, s[e] * r1, g1[v][e]);
+            }
+        } else if (a.waves > 1u) {
+            __syncthreads(); // box_a is free for the next row
+        }
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v)
+            store8<DT>((uint8_t*)a.d.dSum + row * a.d.dSumStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(g1[v]));
+        if (has_gate && !a.by_gate && (row + 1u == gate_end || row + 1u == end)) { // whole gate rows in one run: theirs are done
+            const uint64_t g = gate_row++;
+            gate_end += a.d.rowsPerGate;
+#pragma unroll
+            for (uint32_t v = 0; v < V; ++v) {
+                if (a.d.dGate) store8<PT>((uint8_t*)a.d.dGate + g * a.d.dGateStride * PS, (v * span + t) * 8u, cols, narrow8<PT>(d_gate[v]));
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; ++e) d_gate[v][e] = 0.0f;
+                if (row + 1u < end) gate[v] = load8<PT>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols);
+            }
+        }
+    }
+    float* mine = (float*)a.d.workspace + (uint64_t)blockIdx.x * a.sums * cols;
+#pragma unroll
+    for (uint32_t v = 0; v < V; ++v) {
+        const uint32_t at = (v * span + t) * 8u;
+        if (a.at_post >= 0) store8<DT_F32>(mine + (uint64_t)a.at_post * cols, at, cols, narrow8<DT_F32>(d_post[v]));
+        if (a.at_pre >= 0) store8<DT_F32>(mine + (uint64_t)a.at_pre * cols, at, cols, narrow8<DT_F32>(d_pre[v]));
+        if (a.at_gate >= 0) store8<DT_F32>(mine + (uint64_t)a.at_gate * cols, at, cols, narrow8<DT_F32>(d_gate[v]));
+    }
+}
+
+// The runs' sums joined, in the order of the runs: a workgroup takes 64 columns of one result, its 16 wavefronts every
+// sixteenth run each.
+template <int PT> __global__ __launch_bounds__(1024) void k_norm_sums(const HgNormGrad a)
+{
+    __shared__ float part[16][64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint64_t col = (uint64_t)blockIdx.x * 64u + lane;
+    const uint32_t results = (a.at_post >= 0) + (a.at_pre >= 0);
+    uint64_t first = 0u, n = a.chunks;
+    uint32_t which;
+    uint8_t* out;
+    if (blockIdx.y < results) {
+        const bool post = blockIdx.y == 0u && a.at_post >= 0;
+        which = (uint32_t)(post ? a.at_post : a.at_pre);
+        out = (uint8_t*)(post ? a.d.dPostWeight : a.d.dPreWeight);
+    } else {
+        const uint64_t g = blockIdx.y - results;
+        which = (uint32_t)a.at_gate;
+        first = g * a.chunks_per_gate;
+        n = a.chunks_per_gate;
+        out = (uint8_t*)a.d.dGate + g * a.d.dGateStride * ElemSize<PT>::v;
+    }
+    float s = 0.0f;
+    if (col < a.d.cols) {
+        const float* p = (const float*)a.d.workspace + (first * a.sums + which) * a.d.cols + col;
+#pragma unroll 8
+        for (uint64_t i = wave; i < n; i += 16u) s += p[i * a.sums * a.d.cols];
+    }
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0u && col < a.d.cols) {
+        for (uint32_t w = 1; w < 16u; ++w) s += part[w][lane];
+        if (PT == DT_F32) ((float*)out)[col] = s;
+        else if (PT == DT_BF16) ((__bf16*)out)[col] = (__bf16)s;
+        else ((_Float16*)out)[col] = (_Float16)s;
+    }
+}
+
+template <int DT, int PT> int launch_norm(hipStream_t st, const HgNorm* a)
+{
+    const dim3 g(a->wgs), b(a->waves * 64u * a->rows_per_wg);
+    if (a->vecs == 1u) hipLaunchKernelGGL((k_norm<DT, PT, 1>), g, b, 0, st, *a);
+    else hipLaunchKernelGGL((k_norm<DT, PT, 2>), g, b, 0, st, *a);
+    return rc(hipGetLastError());
+}
+
+template <int DT, int PT> int launch_norm_grad(hipStream_t st, const HgNormGrad* a)
+{
+    const dim3 g((uint32_t)a->chunks), b(a->waves * 64u);
+    if (a->vecs == 1u) {
+        if (a->waves <= 4u) hipLaunchKernelGGL((k_norm_grad<DT, PT, 1, 256>), g, b, 0, st, *a);
+        else hipLaunchKernelGGL((k_norm_grad<DT, PT, 1, 1024>), g, b, 0, st, *a);
+    } else {
+        if (a->waves <= 4u) hipLaunchKernelGGL((k_norm_grad<DT, PT, 2, 256>), g, b, 0, st, *a);
+        else hipLaunchKernelGGL((k_norm_grad<DT, PT, 2, 1024>), g, b, 0, st, *a);
+    }
+    return rc(hipGetLastError());
+}
+
+} // namespace
+
+extern "C" {
+
+int hg_launch_norm(void* stream, const void* args)
+{
+    const HgNorm* a = (const HgNorm*)args;
+    OnDeviceOf device((hipStream_t)stream);
+    if (device.err != hipSuccess) return HCCL_E_RUNTIME;
+    const hipStream_t st = (hipStream_t)stream;
+    const bool wide = a->d.paramType == HCOMM_DATA_TYPE_FP32;
+    switch (a->d.dataType) {
+        case HCOMM_DATA_TYPE_FP16: return wide ? launch_norm<DT_F16, DT_F32>(st, a) : launch_norm<DT_F16, DT_F16>(st, a);
+        case HCOMM_DATA_TYPE_BFP16: return wide ? launch_norm<DT_BF16, DT_F32>(st, a) : launch_norm<DT_BF16, DT_BF16>(st, a);
+        case HCOMM_DATA_TYPE_FP32: return launch_norm<DT_F32, DT_F32>(st, a);
+        default: return HCCL_E_PARA;
+    }
+}
+
+int hg_launch_norm_grad(void* stream, const void* args)
+{
+    const HgNormGrad* a = (const HgNormGrad*)args;
+    OnDeviceOf device((hipStream_t)stream);
+    if (device.err != hipSuccess) return HCCL_E_RUNTIME;
+    const hipStream_t st = (hipStream_t)stream;
+    const bool wide = a->d.paramType == HCOMM_DATA_TYPE_FP32;
+    switch (a->d.dataType) {
+        case HCOMM_DATA_TYPE_FP16: return wide ? launch_norm_grad<DT_F16, DT_F32>(st, a) : launch_norm_grad<DT_F16, DT_F16>(st, a);
+        case HCOMM_DATA_TYPE_BFP16: return wide ? launch_norm_grad<DT_BF16, DT_F32>(st, a) : launch_norm_grad<DT_BF16, DT_BF16>(st, a);
+        case HCOMM_DATA_TYPE_FP32: return launch_norm_grad<DT_F32, DT_F32>(st, a);
+        default: return HCCL_E_PARA;
+    }
+}
+
+int hg_launch_norm_sums(void* stream, const void* args)
+{
+    const HgNormGrad* a = (const HgNormGrad*)args;
+    OnDeviceOf device((hipStream_t)stream);
+    if (device.err != hipSuccess) return HCCL_E_RUNTIME;
+    const dim3 g((uint32_t)((a->d.cols + 63u) / 64u), (uint32_t)((a->at_post >= 0) + (a->at_pre >= 0) + (a->at_gate >= 0 ? a->gates : 0u))), b(1024);
+    switch (a->d.paramType) {
+        case HCOMM_DATA_TYPE_FP16: hipLaunchKernelGGL((k_norm_sums<DT_F16>), g, b, 0, (hipStream_t)stream, *a); break;
+        case HCOMM_DATA_TYPE_BFP16: hipLaunchKernelGGL((k_norm_sums<DT_BF16>), g, b, 0, (hipStream_t)stream, *a); break;
+        case HCOMM_DATA_TYPE_FP32: hipLaunchKernelGGL((k_norm_sums<DT_F32>), g, b, 0, (hipStream_t)stream, *a); break;
+        default: return HCCL_E_PARA;
+    }
+    return rc(hipGetLastError());
+}
+
+} // extern "C"

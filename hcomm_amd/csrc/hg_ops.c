@@ -1,0 +1,420 @@
+/*
+ * hg_ops.c - the operators around a fold: argument checks, launch geometry, submission.  The kernels trust what is
+ * checked here: strides that hold a row, ranges whose ends do not wrap, counts that fit the grid.
+ */
+#include <string.h>
+
+#include "hg_host.h"
+#include "hg_ops.h"
+
+#define HG_LIMIT_WGS 0x7fffffffull
+#define HG_LIMIT_ROWS 0x7fffffffull
+
+static uint64_t elem_size(int dtype)
+{
+    return dtype == HCOMM_DATA_TYPE_FP32 ? 4u : (dtype == HCOMM_DATA_TYPE_FP16 || dtype == HCOMM_DATA_TYPE_BFP16) ? 2u : 0u;
+}
+
+/* ---- memory ranges ------------------------------------------------------------------------------------------ */
+
+typedef struct {
+    uintptr_t at;
+    uint64_t bytes, row, stride; /* from its first byte to behind its last; of a row; from row to row */
+} Range;
+
+/* rows x row_bytes at `p`, `stride` bytes apart; 0 where a row does not fit its stride or the end wraps */
+static int range_of(Range* r, const void* p, uint64_t rows, uint64_t row_bytes, uint64_t stride)
+{
+    uint64_t n;
+    r->at = (uintptr_t)p;
+    r->stride = stride;
+    r->bytes = 0;
+    r->row = row_bytes;
+    if (rows == 0 || row_bytes == 0) return 1;
+    if (rows > 1 && stride < row_bytes) return 0;
+    if (rows == 1) r->stride = stride = row_bytes;
+    if (__builtin_mul_overflow(rows - 1u, stride, &n) || __builtin_add_overflow(n, row_bytes, &n)) return 0;
+    r->bytes = n;
+    return !__builtin_add_overflow((uint64_t)r->at, n, &n);
+}
+
+static int dense_range(Range* r, const void* p, uint64_t rows, uint64_t cols, uint64_t stride, uint64_t es)
+{
+    uint64_t row, step;
+    if ((uintptr_t)p % es != 0) return 0;
+    if (__builtin_mul_overflow(cols, es, &row) || __builtin_mul_overflow(stride, es, &step)) return 0;
+    if (rows == 1) step = row; /* a single row has no next one */
+    return range_of(r, p, rows, row, step);
+}
+
+static int meets(const Range* a, const Range* b)
+{
+    if (!a->bytes || !b->bytes || a->at >= b->at + b->bytes || b->at >= a->at + a->bytes) return 0;
+    if (a->stride != b->stride) return 1;
+    /* two sets of columns of one larger matrix lie between one another without meeting */
+    const uint64_t d = a->at <= b->at ? (b->at - a->at) % a->stride : (a->stride - (a->at - b->at) % a->stride) % a->stride;
+    return d < a->row || d + b->row > a->stride;
+}
+static int same(const Range* a, const Range* b) { return a->at == b->at && a->bytes == b->bytes && a->stride == b->stride; }
+
+/* an output may not meet any of these ranges, apart from the one that it may be itself */
+static int clear_of(const Range* out, const Range* others, uint32_t n, const Range* may_be)
+{
+    for (uint32_t i = 0; i < n; ++i)
+        if (&others[i] != out && meets(out, &others[i]) && !(&others[i] == may_be && same(out, may_be))) return 0;
+    return 1;
+}
+
+/* ---- threads ------------------------------------------------------------------------------------------------- */
+
+static int ready(const HgThread* t)
+{
+    if (hg_caller_is_batching()) return HCCL_E_NOT_SUPPORT;
+    return hg_thread_free_for_caller(t);
+}
+
+static HcommGfxLaunchRecord record(uint32_t kind, int dtype, uint32_t op, uint32_t nseg, uint64_t bytes, uint64_t blocks, uint32_t rows)
+{
+    HcommGfxLaunchRecord r;
+    memset(&r, 0, sizeof(r));
+    r.kind = kind;
+    r.dtype = (uint32_t)dtype;
+    r.op = op;
+    r.nseg = nseg;
+    r.bytes = bytes;
+    r.blocks = blocks;
+    r.rows = rows;
+    return r;
+}
+
+/* ---- microscaled 4-bit floating point --------------------------------------------------------------------------- */
+
+#define HG_MX_MAX_COLS (1ull << 34)
+
+static uint64_t mx_blocks(uint64_t cols) { return cols / HCOMM_GFX_MX_BLOCK + (cols % HCOMM_GFX_MX_BLOCK != 0); }
+
+static int mx_view(HgMxView* v, Range* packed, Range* scales, const HcommGfxMxView* in, uint64_t rows, uint64_t cols)
+{
+    const uint64_t blocks = mx_blocks(cols);
+    v->packed = (uint8_t*)in->packed;
+    v->scales = (uint8_t*)in->scales;
+    v->packed_stride = in->packedStride;
+    v->scale_stride = in->scaleStride;
+    if ((uintptr_t)in->packed % HCOMM_GFX_MX_BLOCK_BYTES != 0) return 0;
+    if (rows > 1 && in->packedStride % HCOMM_GFX_MX_BLOCK_BYTES != 0) return 0;
+    return range_of(packed, in->packed, rows, blocks * HCOMM_GFX_MX_BLOCK_BYTES, in->packedStride) &&
+           range_of(scales, in->scales, rows, blocks, in->scaleStride);
+}
+
+static int mx_grid(HgMxGrid* g, uint64_t rows, uint64_t cols)
+{
+    if (cols > HG_MX_MAX_COLS) return HCCL_E_NOT_SUPPORT;
+    const uint64_t groups = mx_blocks(cols) * 4u;
+    g->rows = rows;
+    g->cols = cols;
+    g->groups = (uint32_t)groups;
+    g->tiles = (uint32_t)((groups + HG_MX_TILE - 1u) / HG_MX_TILE);
+    g->rows_per_wg = groups < HG_MX_TILE ? HG_MX_TILE / (uint32_t)groups : 1u;
+    const uint64_t wgs = g->rows_per_wg > 1u ? rows / g->rows_per_wg + (rows % g->rows_per_wg != 0) : rows;
+    if (wgs > HG_LIMIT_WGS / g->tiles) return HCCL_E_NOT_SUPPORT;
+    g->wgs = (uint32_t)wgs * g->tiles;
+    return HCCL_SUCCESS;
+}
+
+int32_t HcommGfxMxQuantizeOnThread(
+    ThreadHandle thread, const HcommGfxMxView* out, const void* src, uint64_t srcStride, uint64_t rows, uint64_t cols,
+    HcommDataType srcType)
+{
+    if (!out || !out->packed || !out->scales || !src) return HCCL_E_PTR;
+    HgThread* t = hg_thread_from_handle(thread);
+    if (!t) return HCCL_E_PTR;
+    const uint64_t es = elem_size((int)srcType);
+    if (!es) return HCCL_E_PARA;
+    HgMxQuantize a;
+    memset(&a, 0, sizeof(a));
+    int rc = cols > HG_MX_MAX_COLS ? HCCL_E_NOT_SUPPORT : HCCL_SUCCESS;
+    if (rc == HCCL_SUCCESS) {
+        Range r[3];
+        if (!dense_range(&r[0], src, rows, cols, srcStride, es) || !mx_view(&a.out, &r[1], &r[2], out, rows, cols)) return HCCL_E_PARA;
+        if (!clear_of(&r[1], r, 3, NULL) || !clear_of(&r[2], r, 3, NULL)) return HCCL_E_PARA;
+        if (rows && cols) rc = mx_grid(&a.grid, rows, cols);
+    }
+    if (rc == HCCL_SUCCESS) rc = ready(t);
+    if (rc != HCCL_SUCCESS || rows == 0 || cols == 0) return rc;
+    a.src = src;
+    a.src_stride = rows > 1 ? srcStride : cols;
+    a.dtype = (int)srcType;
+    const HcommGfxLaunchRecord rec =
+        record(HCOMM_GFX_KERNEL_MX_QUANTIZE, a.dtype, 255, 1, rows * mx_blocks(cols) * (HCOMM_GFX_MX_BLOCK_BYTES + 1u), a.grid.wgs, 0);
+    return hg_submit_other(t, &rec, hg_launch_mx_quantize, &a);
+}
+
+int32_t HcommGfxMxReduceKOnThread(
+    ThreadHandle thread, void* dst, uint64_t dstStride, HcommDataType dstType, const HcommGfxMxView* again,
+    const HcommGfxMxView* srcs, uint32_t k, const void* addend, uint64_t addendStride, uint64_t rows, uint64_t cols)
+{
+    if (!dst && !again) return HCCL_E_PTR;
+    if (again && (!again->packed || !again->scales)) return HCCL_E_PTR;
+    if (!srcs) return HCCL_E_PTR;
+    if (k == 0 || k > HCOMM_GFX_MAX_RANKS) return HCCL_E_PARA;
+    for (uint32_t j = 0; j < k; ++j)
+        if (!srcs[j].packed || !srcs[j].scales) return HCCL_E_PTR;
+    HgThread* t = hg_thread_from_handle(thread);
+    if (!t) return HCCL_E_PTR;
+    const uint64_t es = elem_size((int)dstType);
+    if (!es) return HCCL_E_PARA;
+    HgMxReduce a;
+    memset(&a, 0, sizeof(a));
+    int rc = cols > HG_MX_MAX_COLS ? HCCL_E_NOT_SUPPORT : HCCL_SUCCESS;
+    if (rc == HCCL_SUCCESS) {
+        Range r[4 + 2 * HCOMM_GFX_MAX_RANKS]; /* dst, addend, again's two, the inputs' */
+        memset(r, 0, sizeof(r));
+        if (dst && !dense_range(&r[0], dst, rows, cols, dstStride, es)) return HCCL_E_PARA;
+        if (addend && !dense_range(&r[1], addend, rows, cols, addendStride, es)) return HCCL_E_PARA;
+        if (again && !mx_view(&a.again, &r[2], &r[3], again, rows, cols)) return HCCL_E_PARA;
+        for (uint32_t j = 0; j < k; ++j)
+            if (!mx_view(&a.src[j], &r[4 + 2 * j], &r[5 + 2 * j], &srcs[j], rows, cols)) return HCCL_E_PARA;
+        if (!clear_of(&r[0], r, 4 + 2 * k, &r[1]) || !clear_of(&r[2], r, 4 + 2 * k, NULL) || !clear_of(&r[3], r, 4 + 2 * k, NULL))
+            return HCCL_E_PARA;
+        if (rows && cols) rc = mx_grid(&a.grid, rows, cols);
+    }
+    if (rc == HCCL_SUCCESS) rc = ready(t);
+    if (rc != HCCL_SUCCESS || rows == 0 || cols == 0) return rc;
+    a.dst = dst;
+    a.dst_stride = rows > 1 ? dstStride : cols;
+    a.addend = addend;
+    a.addend_stride = rows > 1 ? addendStride : cols;
+    a.k = k;
+    a.dtype = (int)dstType;
+    const uint64_t bytes = (dst ? rows * cols * es : 0) + (again ? rows * mx_blocks(cols) * (HCOMM_GFX_MX_BLOCK_BYTES + 1u) : 0);
+    const HcommGfxLaunchRecord rec = record(HCOMM_GFX_KERNEL_MX_REDUCE, a.dtype, HCOMM_REDUCE_SUM, k, bytes, a.grid.wgs, 0);
+    return hg_submit_other(t, &rec, hg_launch_mx_reduce, &a);
+}
+
+/* ---- product --------------------------------------------------------------------------------------------------------- */
+
+static void product_form(HgMxProduct* a)
+{
+    const uint32_t edge = a->m <= 16u ? 16u : 32u;
+    a->form = edge == 16u ? HG_PRODUCT_DIRECT_16 : HG_PRODUCT_DIRECT_32;
+    a->wgs = (a->m + edge - 1u) / edge * ((a->n + edge - 1u) / edge);
+}
+
+int32_t HcommGfxMxProductKOnThread(
+    ThreadHandle thread, void* dst, uint64_t dstStride, HcommDataType dstType, const HcommGfxMxView* a,
+    const HcommGfxMxView* b, uint32_t k, uint64_t m, uint64_t n, uint64_t cols)
+{
+    if (!dst || !a || !b) return HCCL_E_PTR;
+    if (k == 0 || k > HCOMM_GFX_MAX_RANKS) return HCCL_E_PARA;
+    for (uint32_t j = 0; j < k; ++j)
+        if (!a[j].packed || !a[j].scales || !b[j].packed || !b[j].scales) return HCCL_E_PTR;
+    HgThread* t = hg_thread_from_handle(thread);
+    if (!t) return HCCL_E_PTR;
+    const uint64_t es = elem_size((int)dstType);
+    if (!es || cols == 0) return HCCL_E_PARA;
+    HgMxProduct p;
+    memset(&p, 0, sizeof(p));
+    /* 16 results an edge at least: the number of workgroups stays below 2^31 */
+    int rc = m > HG_LIMIT_ROWS - 512u || n > HG_LIMIT_ROWS - 512u || mx_blocks(cols) * HCOMM_GFX_MX_BLOCK_BYTES >= (1ull << 23) ? HCCL_E_NOT_SUPPORT : HCCL_SUCCESS;
+    if (rc == HCCL_SUCCESS && (m + 15u) / 16u * ((n + 15u) / 16u) > HG_LIMIT_WGS) rc = HCCL_E_NOT_SUPPORT;
+    if (rc == HCCL_SUCCESS) {
+        Range r[1 + 4 * HCOMM_GFX_MAX_RANKS];
+        memset(r, 0, sizeof(r));
+        if (!dense_range(&r[0], dst, m, n, dstStride, es)) return HCCL_E_PARA;
+        for (uint32_t j = 0; j < k; ++j) {
+            if (!mx_view(&p.a[j], &r[1 + 4 * j], &r[2 + 4 * j], &a[j], m, cols)) return HCCL_E_PARA;
+            if (!mx_view(&p.b[j], &r[3 + 4 * j], &r[4 + 4 * j], &b[j], n, cols)) return HCCL_E_PARA;
+            if ((m > 1 && a[j].packedStride >= (1ull << 23)) || (n > 1 && b[j].packedStride >= (1ull << 23))) rc = HCCL_E_NOT_SUPPORT;
+        }
+        if (!clear_of(&r[0], r, 1 + 4 * k, NULL)) return HCCL_E_PARA;
+    }
+    if (rc == HCCL_SUCCESS) rc = ready(t);
+    if (rc != HCCL_SUCCESS || m == 0 || n == 0) return rc;
+    p.dst = dst;
+    p.dst_stride = m > 1 ? dstStride : n;
+    p.m = (uint32_t)m;
+    p.n = (uint32_t)n;
+    p.cols = (uint32_t)cols;
+    p.k = k;
+    p.dtype = (int)dstType;
+    product_form(&p);
+    const HcommGfxLaunchRecord rec = record(HCOMM_GFX_KERNEL_MX_PRODUCT, p.dtype, HCOMM_REDUCE_SUM, k, m * n * es, p.wgs, p.form);
+    return hg_submit_other(t, &rec, hg_launch_mx_product, &p);
+}
+
+/* ---- norms behind a fold ------------------------------------------------------------------------------------------------ */
+
+/* wavefronts to a row and groups of eight elements to a lane */
+static void row_shape(uint64_t cols, uint32_t* waves, uint32_t* vecs)
+{
+    const uint64_t per_wave = 64u * 8u;
+    uint32_t w = 1, v = 1;
+    if (cols > per_wave * 16u) v = 2;
+    while (w < 16u && per_wave * v * w < cols) w *= 2u;
+    *waves = w;
+    *vecs = v;
+}
+
+static int norm_types(HcommDataType data, HcommDataType param)
+{
+    return elem_size((int)data) != 0 && (param == data || param == HCOMM_DATA_TYPE_FP32);
+}
+
+/* eps >= 0 and neither number NaN or infinite */
+static int norm_numbers(float scale, float eps) { return eps >= 0.0f && eps - eps == 0.0f && scale - scale == 0.0f; }
+
+static uint64_t gate_rows(uint64_t rows, uint64_t per) { return rows / per + (rows % per != 0); }
+
+int32_t HcommGfxReduceNormOnThread(ThreadHandle thread, const HcommGfxReduceNormDesc* desc)
+{
+    if (!desc || !desc->srcs || !desc->y) return HCCL_E_PTR;
+    if (!desc->preWeight != !desc->z) return HCCL_E_PTR;
+    if (desc->k == 0 || desc->k > HCOMM_GFX_MAX_RANKS) return HCCL_E_PARA;
+    for (uint32_t j = 0; j < desc->k; ++j)
+        if (!desc->srcs[j]) return HCCL_E_PTR;
+    HgThread* t = hg_thread_from_handle(thread);
+    if (!t) return HCCL_E_PTR;
+    if (!norm_types(desc->dataType, desc->paramType) || !norm_numbers(desc->residualScale, desc->eps)) return HCCL_E_PARA;
+    if (desc->gate && desc->rowsPerGate == 0) return HCCL_E_PARA;
+    HgNorm a;
+    memset(&a, 0, sizeof(a));
+    a.d = *desc;
+    const uint64_t rows = desc->rows, cols = desc->cols, es = elem_size((int)desc->dataType), ps = elem_size((int)desc->paramType);
+    int rc = cols > HCOMM_GFX_NORM_MAX_COLS || rows > HG_LIMIT_ROWS ? HCCL_E_NOT_SUPPORT : HCCL_SUCCESS;
+    if (rc == HCCL_SUCCESS) {
+        enum { SUM, Y, Z, RES, POST, PRE, GATE, SRC };
+        Range r[SRC + HCOMM_GFX_MAX_RANKS];
+        memset(r, 0, sizeof(r));
+        if (desc->sum && !dense_range(&r[SUM], desc->sum, rows, cols, desc->sumStride, es)) return HCCL_E_PARA;
+        if (!dense_range(&r[Y], desc->y, rows, cols, desc->yStride, es)) return HCCL_E_PARA;
+        if (desc->z && !dense_range(&r[Z], desc->z, rows, cols, desc->zStride, es)) return HCCL_E_PARA;
+        if (desc->residual && !dense_range(&r[RES], desc->residual, rows, cols, desc->residualStride, es)) return HCCL_E_PARA;
+        if (desc->postWeight && !dense_range(&r[POST], desc->postWeight, 1, cols, cols, ps)) return HCCL_E_PARA;
+        if (desc->preWeight && !dense_range(&r[PRE], desc->preWeight, 1, cols, cols, ps)) return HCCL_E_PARA;
+        if (desc->gate && !dense_range(&r[GATE], desc->gate, gate_rows(rows, desc->rowsPerGate), cols, desc->gateStride, ps)) return HCCL_E_PARA;
+        for (uint32_t j = 0; j < desc->k; ++j)
+            if (!dense_range(&r[SRC + j], desc->srcs[j], rows, cols, desc->srcStride, es)) return HCCL_E_PARA;
+        const uint32_t n = SRC + desc->k;
+        if (!clear_of(&r[SUM], r, n, &r[SRC]) || !clear_of(&r[Y], r, n, &r[RES]) || !clear_of(&r[Z], r, n, NULL)) return HCCL_E_PARA;
+    }
+    if (rc == HCCL_SUCCESS) rc = ready(t);
+    if (rc != HCCL_SUCCESS || rows == 0 || cols == 0) return rc;
+    for (uint32_t j = 0; j < desc->k; ++j) a.src[j] = desc->srcs[j];
+    a.d.srcs = NULL;
+    if (!a.d.gate || a.d.rowsPerGate > rows) a.d.rowsPerGate = rows;
+    row_shape(cols, &a.waves, &a.vecs);
+    a.rows_per_wg = a.waves < 4u ? 4u / a.waves : 1u;
+    a.wgs = (uint32_t)((rows + a.rows_per_wg - 1u) / a.rows_per_wg);
+    const uint64_t bytes = rows * cols * es * (1u + (desc->sum != NULL) + (desc->z != NULL));
+    const HcommGfxLaunchRecord rec = record(HCOMM_GFX_KERNEL_NORM, (int)desc->dataType, HCOMM_REDUCE_SUM, desc->k, bytes, a.wgs, a.waves * 64u);
+    return hg_submit_other(t, &rec, hg_launch_norm, &a);
+}
+
+/* Runs of rows for about this many wavefronts: enough to keep every CU loading, few enough that the runs' sums stay a small part of the traffic. */
+#define HG_NORM_GRAD_WAVES 2048u
+
+/* the geometry, from the sizes and from which parameters' gradients are wanted alone */
+static void norm_grad_shape(HgNormGrad* a)
+{
+    HcommGfxReduceNormGradDesc* d = &a->d;
+    const uint64_t rows = d->rows;
+    row_shape(d->cols, &a->waves, &a->vecs);
+    const uint64_t most = HG_NORM_GRAD_WAVES / a->waves;
+    if (!d->gate || d->rowsPerGate > rows) d->rowsPerGate = rows ? rows : 1u;
+    a->gates = d->gate ? gate_rows(rows, d->rowsPerGate) : 0u;
+    const int gate_wanted = d->gate && d->dGate;
+    a->by_gate = gate_wanted && a->gates < most;
+    a->chunks = a->chunk_rows = a->chunks_per_gate = 0;
+    if (rows && a->by_gate) {
+        uint64_t per = most / a->gates;
+        if (per > d->rowsPerGate) per = d->rowsPerGate;
+        a->chunk_rows = (d->rowsPerGate + per - 1u) / per;
+        a->chunks_per_gate = (d->rowsPerGate + a->chunk_rows - 1u) / a->chunk_rows;
+        a->chunks = a->chunks_per_gate * a->gates;
+    } else if (rows) {
+        /* with a gradient of the gate to write, whole gate rows */
+        const uint64_t unit = gate_wanted ? d->rowsPerGate : 1u, units = gate_rows(rows, unit);
+        a->chunk_rows = (units + most - 1u) / most * unit;
+        a->chunks = gate_rows(rows, a->chunk_rows);
+    }
+    a->sums = 0;
+    a->at_post = d->dPostWeight ? (int)a->sums++ : -1;
+    a->at_pre = d->dPreWeight ? (int)a->sums++ : -1;
+    a->at_gate = a->by_gate ? (int)a->sums++ : -1;
+}
+
+static uint64_t norm_grad_workspace(const HgNormGrad* a) { return a->chunks * a->sums * a->d.cols * sizeof(float); }
+
+int32_t HcommGfxReduceNormGradWorkspaceBytes(const HcommGfxReduceNormGradDesc* desc, uint64_t* bytes)
+{
+    if (!desc || !bytes) return HCCL_E_PTR;
+    if (desc->gate && desc->rowsPerGate == 0) return HCCL_E_PARA;
+    if (desc->cols > HCOMM_GFX_NORM_MAX_COLS || desc->rows > HG_LIMIT_ROWS) return HCCL_E_NOT_SUPPORT;
+    HgNormGrad a;
+    memset(&a, 0, sizeof(a));
+    a.d = *desc;
+    if (desc->cols) norm_grad_shape(&a);
+    *bytes = norm_grad_workspace(&a);
+    return HCCL_SUCCESS;
+}
+
+int32_t HcommGfxReduceNormGradOnThread(ThreadHandle thread, const HcommGfxReduceNormGradDesc* desc)
+{
+    if (!desc || !desc->sum || !desc->dy || !desc->dSum) return HCCL_E_PTR;
+    if (!desc->preWeight != !desc->dz || (desc->preWeight && !desc->y)) return HCCL_E_PTR;
+    HgThread* t = hg_thread_from_handle(thread);
+    if (!t) return HCCL_E_PTR;
+    if (!norm_types(desc->dataType, desc->paramType) || !norm_numbers(desc->residualScale, desc->eps)) return HCCL_E_PARA;
+    if (desc->gate && desc->rowsPerGate == 0) return HCCL_E_PARA;
+    if ((desc->dPostWeight && !desc->postWeight) || (desc->dPreWeight && !desc->preWeight) || (desc->dGate && !desc->gate)) return HCCL_E_PARA;
+    HgNormGrad a;
+    memset(&a, 0, sizeof(a));
+    a.d = *desc;
+    const uint64_t rows = desc->rows, cols = desc->cols, es = elem_size((int)desc->dataType), ps = elem_size((int)desc->paramType);
+    int rc = cols > HCOMM_GFX_NORM_MAX_COLS || rows > HG_LIMIT_ROWS ? HCCL_E_NOT_SUPPORT : HCCL_SUCCESS;
+    if (rc == HCCL_SUCCESS) {
+        if (cols) norm_grad_shape(&a);
+        const uint64_t need = norm_grad_workspace(&a), gates = desc->gate ? gate_rows(rows, desc->rowsPerGate) : 0u;
+        if (need && !desc->workspace) return HCCL_E_PTR;
+        if (need && (desc->workspaceBytes < need || (uintptr_t)desc->workspace % 16u != 0)) return HCCL_E_PARA;
+        enum { DSUM, DRES, DPOST, DPRE, DGATE, WORK, OUTPUTS, SUM = OUTPUTS, Y, DY, DZ, POST, PRE, GATE, ALL };
+        Range r[ALL];
+        memset(r, 0, sizeof(r));
+        int ok = dense_range(&r[DSUM], desc->dSum, rows, cols, desc->dSumStride, es) && dense_range(&r[SUM], desc->sum, rows, cols, desc->sumStride, es) &&
+                 dense_range(&r[DY], desc->dy, rows, cols, desc->dyStride, es);
+        if (ok && desc->dResidual) ok = dense_range(&r[DRES], desc->dResidual, rows, cols, desc->dResidualStride, es);
+        if (ok && desc->preWeight)
+            ok = dense_range(&r[Y], desc->y, rows, cols, desc->yStride, es) && dense_range(&r[DZ], desc->dz, rows, cols, desc->dzStride, es) &&
+                 dense_range(&r[PRE], desc->preWeight, 1, cols, cols, ps);
+        if (ok && desc->postWeight) ok = dense_range(&r[POST], desc->postWeight, 1, cols, cols, ps);
+        if (ok && desc->gate) ok = dense_range(&r[GATE], desc->gate, gates, cols, desc->gateStride, ps);
+        if (ok && desc->dPostWeight) ok = dense_range(&r[DPOST], desc->dPostWeight, 1, cols, cols, ps);
+        if (ok && desc->dPreWeight) ok = dense_range(&r[DPRE], desc->dPreWeight, 1, cols, cols, ps);
+        if (ok && desc->dGate) ok = dense_range(&r[DGATE], desc->dGate, gates, cols, desc->dGateStride, ps);
+        if (ok && need) ok = range_of(&r[WORK], desc->workspace, 1, need, need);
+        if (!ok) return HCCL_E_PARA;
+        for (uint32_t o = 0; o < OUTPUTS; ++o) {
+            /* the gradient of a matrix may overwrite the matrix, and either of the two dy - but not both */
+            const Range* may = NULL;
+            if (o == DSUM) may = same(&r[DSUM], &r[SUM]) ? &r[SUM] : &r[DY];
+            if (o == DRES) may = same(&r[DRES], &r[Y]) ? &r[Y] : &r[DY];
+            if (!clear_of(&r[o], r, ALL, may)) return HCCL_E_PARA;
+        }
+    }
+    if (rc == HCCL_SUCCESS) rc = ready(t);
+    if (rc != HCCL_SUCCESS || cols == 0) return rc;
+    if (a.chunks) {
+        const HcommGfxLaunchRecord rec = record(
+            HCOMM_GFX_KERNEL_NORM_GRAD, (int)desc->dataType, 255, 1, rows * cols * es * (1u + (desc->dResidual != NULL)), a.chunks, a.waves * 64u);
+        rc = hg_submit_other(t, &rec, hg_launch_norm_grad, &a);
+    }
+    if (rc == HCCL_SUCCESS && a.sums) {
+        const uint64_t results = (a.at_post >= 0) + (a.at_pre >= 0) + (a.at_gate >= 0 ? a.gates : 0u);
+        if (results) {
+            const HcommGfxLaunchRecord rec = record(HCOMM_GFX_KERNEL_NORM_SUMS, (int)desc->paramType, HCOMM_REDUCE_SUM, (uint32_t)a.chunks,
+                                                    results * cols * ps, results * ((cols + 63u) / 64u), 0);
+            rc = hg_submit_other(t, &rec, hg_launch_norm_sums, &a);
+        }
+    }
+    return rc;
+}

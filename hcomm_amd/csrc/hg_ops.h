@@ -1,0 +1,107 @@
+/*
+ * hg_ops.h - the operators around a fold: what the host code (hg_ops.c) hands to their launchers (hg_mx.hip,
+ * hg_mx_product.hip, hg_norm.hip).  Plain C.  All geometry is decided on the host and checked there.
+ */
+#ifndef HG_OPS_H
+#define HG_OPS_H
+
+#include "hg_internal.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* ---- microscaled 4-bit floating point --------------------------------------------------------------------- */
+
+typedef struct {
+    uint8_t* packed;
+    uint8_t* scales;
+    uint64_t packed_stride, scale_stride; /* bytes */
+} HgMxView;
+
+/*
+ * Quantise and fold walk a matrix in groups of eight elements (a quarter of a block, one dword of elements), four
+ * neighbouring lanes to a block.  A workgroup takes `rows_per_wg` whole rows where a row has fewer groups than
+ * HG_MX_TILE, else one of the `tiles` pieces of HG_MX_TILE groups of a row.
+ */
+#define HG_MX_TILE 1024u /* groups of a workgroup: 256 lanes, four each */
+
+typedef struct {
+    uint64_t rows, cols;
+    uint32_t groups;      /* of a row: 4 * ceil(cols / 32) */
+    uint32_t tiles;       /* workgroups to a row */
+    uint32_t rows_per_wg;
+    uint32_t wgs;
+} HgMxGrid;
+
+typedef struct {
+    HgMxGrid grid;
+    HgMxView out;
+    const void* src;
+    uint64_t src_stride; /* elements */
+    int dtype;
+} HgMxQuantize;
+
+typedef struct {
+    HgMxGrid grid;
+    HgMxView src[HCOMM_GFX_MAX_RANKS];
+    HgMxView again; /* packed == NULL: not wanted */
+    void* dst;      /* NULL: not wanted */
+    const void* addend;
+    uint64_t dst_stride, addend_stride; /* elements */
+    uint32_t k;
+    int dtype;
+} HgMxReduce;
+
+enum { HG_PRODUCT_DIRECT_16 = 0, HG_PRODUCT_DIRECT_32 = 1 }; /* results of a workgroup: 16 x 16, 32 x 32 */
+
+typedef struct {
+    HgMxView a[HCOMM_GFX_MAX_RANKS];
+    HgMxView b[HCOMM_GFX_MAX_RANKS];
+    void* dst;
+    uint64_t dst_stride; /* elements */
+    uint32_t m, n, cols, k;
+    uint32_t form; /* HG_PRODUCT_* */
+    uint32_t wgs;
+    int dtype;
+} HgMxProduct;
+
+int hg_launch_mx_quantize(void* stream, const void* args); /* HgMxQuantize */
+int hg_launch_mx_reduce(void* stream, const void* args);   /* HgMxReduce */
+int hg_launch_mx_product(void* stream, const void* args);  /* HgMxProduct */
+
+/* ---- norms behind a fold ------------------------------------------------------------------------------------ */
+
+typedef struct {
+    HcommGfxReduceNormDesc d; /* .srcs is not followed on the device: */
+    const void* src[HCOMM_GFX_MAX_RANKS];
+    uint32_t waves;       /* wavefronts that share a row */
+    uint32_t vecs;        /* groups of eight elements a lane holds */
+    uint32_t rows_per_wg;
+    uint32_t wgs;
+} HgNorm;
+
+/*
+ * The gradient walks the rows in `chunks` runs of `chunk_rows` rows, one workgroup a run, and joins the runs' sums in a
+ * second launch.  by_gate: a run never crosses from one row of the gate to the next (`chunks_per_gate` runs to each), so
+ * that the gate's gradient is joined from runs too; otherwise every run holds whole gate rows and writes their
+ * gradients itself.
+ */
+typedef struct {
+    HcommGfxReduceNormGradDesc d;
+    uint64_t gates;           /* rows of the gate */
+    uint64_t chunks, chunk_rows, chunks_per_gate;
+    uint32_t by_gate;
+    uint32_t waves, vecs;
+    uint32_t sums;            /* rows of cols fp32 a run writes to the workspace: post, pre, gate as wanted */
+    int at_post, at_pre, at_gate; /* which of them, -1: not there */
+} HgNormGrad;
+
+int hg_launch_norm(void* stream, const void* args);      /* HgNorm */
+int hg_launch_norm_grad(void* stream, const void* args); /* HgNormGrad */
+int hg_launch_norm_sums(void* stream, const void* args); /* HgNormGrad */
+
+#ifdef __cplusplus
+}
+#endif
+#endif

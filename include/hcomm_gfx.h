@@ -6,7 +6,7 @@
  * name and numeric value, so a caller compiled against the reference headers can bind these symbols
  * unchanged.  Citations are paths relative to the reference tree.
  *
- * Four groups of entry points:
+ * Five groups of entry points:
  *   1. drop-in primitives      - same names, argument meaning and return codes as the reference;
  *   2. HcommGfx* extensions    - k-way fused reduce, stream sync, launch log (no reference counterpart);
  *   3. HcommGfxPlan*           - build once / run many replay of the templates' schedules (ring, recursive
@@ -20,7 +20,10 @@
  *                                HcommGfxOrderPreservedFused*: what the
  *                                reference's executors do around the templates (chunk loops through the CCL
  *                                buffers, two communicator levels, user memory read and written directly), each
- *                                as PlanCreate / Emit / Check.
+ *                                as PlanCreate / Emit / Check;
+ *   5. operators around a fold - HcommGfxMx*: messages in microscaled 4-bit floating point, quantised, folded and
+ *                                multiplied; HcommGfxReduceNorm*: the norms, gate and residual that follow a
+ *                                tensor-parallel fold, with their gradient (no reference counterpart).
  */
 #ifndef HCOMM_GFX_H
 #define HCOMM_GFX_H
@@ -355,7 +358,14 @@ typedef enum {
     HCOMM_GFX_KERNEL_REDUCE2 = 1,  /* batched dst = dst (op) src */
     HCOMM_GFX_KERNEL_CHAIN = 2,    /* k inputs folded in sequence, optional partial stores, fan-out stores */
     HCOMM_GFX_KERNEL_TREE = 3,     /* k = 2^j inputs folded as a binary tree with partial stores, fan-out */
-    HCOMM_GFX_KERNEL_BYTEWISE = 4  /* copy / two-input reduce for pointers off 16-byte boundaries (unaligned 16-byte items) */
+    HCOMM_GFX_KERNEL_BYTEWISE = 4, /* copy / two-input reduce for pointers off 16-byte boundaries (unaligned 16-byte items) */
+    /* the operators of group 5: `nseg` is the number of ranks folded, `rows` the form of the kernel (0 where it has one) */
+    HCOMM_GFX_KERNEL_MX_QUANTIZE = 5,
+    HCOMM_GFX_KERNEL_MX_REDUCE = 6,
+    HCOMM_GFX_KERNEL_MX_PRODUCT = 7,
+    HCOMM_GFX_KERNEL_NORM = 8,
+    HCOMM_GFX_KERNEL_NORM_GRAD = 9,
+    HCOMM_GFX_KERNEL_NORM_SUMS = 10 /* the parameters' gradients joined from the workspace */
 } HcommGfxKernelKind;
 
 /* Copy up to `cap` records of the thread's launch log into `out`; *n receives the total logged. */
@@ -1018,6 +1028,160 @@ uint64_t HcommGfxSetAlternateBytes(uint64_t bytes);
  * 0 = plans keep one launch per step.  Returns the previous value; the initial one is HCOMM_GFX_PIECE_BYTES from
  * the environment, 128 MiB without it.  Results never depend on it. */
 uint64_t HcommGfxSetPieceBytes(uint64_t bytes);
+
+/* ---------------------------------------------------------------------------------------------
+ * 5. Operators around a fold (no reference counterpart)
+ *
+ * Every call is asynchronous on the thread's stream, allocates nothing, keeps nothing after it returns and may be
+ * captured into a graph.  Checks come in this order: pointers (HCCL_E_PTR, an invalid thread last), then sizes, types,
+ * alignment and overlaps (HCCL_E_PARA), a limit of this library (HCCL_E_NOT_SUPPORT), a call between
+ * HcommBatchModeStart and HcommBatchModeEnd (HCCL_E_NOT_SUPPORT), a thread that holds recorded operations of another
+ * host thread's batch (HCCL_E_UNAVAIL).  After a refusal nothing was queued.
+ * Dense matrices are row-major, `Stride` is the distance of two rows in ELEMENTS and at least the row's length; any
+ * element-aligned address and any stride are taken.  Nothing outside the rows x cols elements is read or written.
+ * Dense types: FP16, BFP16, FP32.  Outputs overlap no input and no other output unless a call says so.
+ * The work runs on the device of the thread's stream, whatever the caller's current device.
+ * ------------------------------------------------------------------------------------------- */
+
+#define HCOMM_GFX_MX_BLOCK 32u       /* elements of a row that share a scale */
+#define HCOMM_GFX_MX_BLOCK_BYTES 16u /* their bytes without the scale */
+
+/*
+ * A rows x cols matrix in microscaled 4-bit floating point (the OCP microscaling format MXFP4: E2M1 elements, E8M0
+ * scales).  A row is ceil(cols / 32) blocks; block b is 16 bytes at packed + row * packedStride + 16 b, element 2 i of
+ * it in the low four bits of byte i and element 2 i + 1 in the high four, and one byte s at scales + row * scaleStride
+ * + b.  An element stands for 2^(s - 127) x {0, 0.5, 1, 1.5, 2, 3, 4, 6} with its top bit as sign; s = 255: NaN.  Elements of
+ * the last block past cols are written as 0 and never count.  Strides are in BYTES: packedStride a multiple of 16,
+ * packed on a 16-byte boundary, scales anywhere.
+ */
+typedef struct {
+    void* packed; /* only read where the matrix is an input */
+    void* scales;
+    uint64_t packedStride;
+    uint64_t scaleStride;
+} HcommGfxMxView;
+
+/*
+ * out = src in the format above.  A block's scale is 2^(E - 2), E the exponent of its largest magnitude (never below
+ * 2^-127); elements go to the nearest value, at the middle to the even code, above 6 x scale to 6 x scale; signs are
+ * kept, zeros' too.  A block that holds an infinity or a NaN becomes s = 255 with elements 0.  cols up to 2^34.
+ * rows == 0 or cols == 0 succeed without doing anything.  (Its gradient is the identity.)
+ */
+int32_t HcommGfxMxQuantizeOnThread(
+    ThreadHandle thread, const HcommGfxMxView* out, const void* src, uint64_t srcStride, uint64_t rows, uint64_t cols,
+    HcommDataType srcType);
+
+/*
+ * The fold of k ranks' quantised contributions: v = addend + srcs[0] + .. + srcs[k-1], every element of it, then
+ * dst = v rounded once to dstType and / or again = v quantised as above (from v, not from dst).  1 <= k <= HCOMM_GFX_MAX_RANKS.
+ * Every contribution is taken as its fp32 value (2^128 and above: infinite) and the sum is that of fp64, so it is exact,
+ * and does not depend on the ranks' order, where its terms span no more than 53 bits.  addend (dstType, or NULL: the own
+ * contribution in full precision) may be dst itself with the same stride.  One of dst and again may be NULL.
+ * k = 1 with neither addend nor again turns a message back into dense values.
+ */
+int32_t HcommGfxMxReduceKOnThread(
+    ThreadHandle thread, void* dst, uint64_t dstStride, HcommDataType dstType, const HcommGfxMxView* again,
+    const HcommGfxMxView* srcs, uint32_t k, const void* addend, uint64_t addendStride, uint64_t rows, uint64_t cols);
+
+/*
+ * dst[i, j] = sum over ranks r < k and c < cols of a[r][i, c] * b[r][j, c]: the product of a row-parallel layer whose
+ * inner length the ranks share, and the reduction of their partial results, in one pass (k = 1: a plain product).
+ * a[r] is m x cols (activations), b[r] n x cols (weights); sums in fp32, rounded once to dstType.
+ * cols == 0 is HCCL_E_PARA, m == 0 or n == 0 succeed without doing anything.  packedStride below 2^23.
+ */
+int32_t HcommGfxMxProductKOnThread(
+    ThreadHandle thread, void* dst, uint64_t dstStride, HcommDataType dstType, const HcommGfxMxView* a,
+    const HcommGfxMxView* b, uint32_t k, uint64_t m, uint64_t n, uint64_t cols);
+
+#define HCOMM_GFX_NORM_MAX_COLS 16384u
+
+/*
+ * What follows the fold of a tensor-parallel block's k partial outputs, in one pass over them:
+ *     s = srcs[0] + .. + srcs[k-1]          (fp32, left to right)
+ *     h = s / rms(s) * postWeight           (postWeight NULL: h = s)
+ *     y = residualScale * residual + g * h  (residual NULL: no first term; gate NULL: g = 1)
+ *     z = y / rms(y) * preWeight            (z and preWeight both given or both NULL)
+ * rms(v) = sqrt(mean of v^2 over the row + eps).  Row r takes row r / rowsPerGate of the gate: one learned gate for
+ * all rows (rowsPerGate >= rows), one for each sample, or one for each row (rowsPerGate = 1).  sum receives s (NULL:
+ * not kept; the gradient needs it).  Statistics and everything between are fp32; sum, y and z are rounded once, z from the y that is
+ * not yet rounded.  The weights and the gate are of paramType, all else of dataType.
+ * y may be residual itself and sum may be srcs[0], with the same stride each.
+ */
+typedef struct {
+    uint64_t rows, cols; /* cols <= HCOMM_GFX_NORM_MAX_COLS */
+    HcommDataType dataType;
+    HcommDataType paramType; /* dataType or FP32 */
+    uint32_t k;              /* 1 <= k <= HCOMM_GFX_MAX_RANKS */
+    float residualScale;
+    float eps; /* >= 0 */
+    uint32_t reserved;
+    uint64_t rowsPerGate;
+    const void* const* srcs;
+    uint64_t srcStride; /* of every srcs[j] */
+    const void* residual;
+    uint64_t residualStride;
+    const void* postWeight;
+    const void* preWeight;
+    const void* gate;
+    uint64_t gateStride;
+    void* sum;
+    uint64_t sumStride;
+    void* y;
+    uint64_t yStride;
+    void* z;
+    uint64_t zStride;
+} HcommGfxReduceNormDesc;
+
+int32_t HcommGfxReduceNormOnThread(ThreadHandle thread, const HcommGfxReduceNormDesc* desc);
+
+/*
+ * The gradient of the above at the stored sum and y, given dy and (where there is a z) dz:
+ *     D         = dy + the gradient of z with respect to y, applied to dz
+ *     dResidual = residualScale * D                       (NULL: not wanted)
+ *     dGate     = D * h, summed over the rows that share a row of the gate
+ *     dSum      = the gradient of h with respect to s, applied to g * D: every partial's gradient is this one
+ *     dPostWeight = g * D * s / rms(s), dPreWeight = dz * y / rms(y), summed over the rows
+ * A parameter's gradient may be NULL where it is not wanted and has to be NULL where the parameter is; it has
+ * paramType, and is 0 for rows == 0.  Sums over rows are fp32 in a fixed order: the same call gives the same bits.  preWeight and dz are both given
+ * or both NULL.  dSum may be sum or dy, dResidual may be y or dy, with the same stride each.
+ * workspace: HcommGfxReduceNormGradWorkspaceBytes(desc) bytes on a 16-byte boundary that no call in flight on another
+ * stream uses (NULL where that is 0); the contents do not matter before and after.
+ */
+typedef struct {
+    uint64_t rows, cols;
+    HcommDataType dataType;
+    HcommDataType paramType;
+    float residualScale;
+    float eps;
+    uint64_t rowsPerGate;
+    const void* sum;
+    uint64_t sumStride;
+    const void* y; /* only read where preWeight is given; may be NULL otherwise */
+    uint64_t yStride;
+    const void* dy;
+    uint64_t dyStride;
+    const void* dz;
+    uint64_t dzStride;
+    const void* postWeight;
+    const void* preWeight;
+    const void* gate;
+    uint64_t gateStride;
+    void* dSum;
+    uint64_t dSumStride;
+    void* dResidual;
+    uint64_t dResidualStride;
+    void* dPostWeight;
+    void* dPreWeight;
+    void* dGate;
+    uint64_t dGateStride;
+    void* workspace;
+    uint64_t workspaceBytes;
+} HcommGfxReduceNormGradDesc;
+
+int32_t HcommGfxReduceNormGradOnThread(ThreadHandle thread, const HcommGfxReduceNormGradDesc* desc);
+
+/* Bytes of workspace the call needs: depends on rows, cols, rowsPerGate and on which parameter gradients are asked for. */
+int32_t HcommGfxReduceNormGradWorkspaceBytes(const HcommGfxReduceNormGradDesc* desc, uint64_t* bytes);
 
 /* Library version string, e.g. "hcomm_gfx 0.1 gfx950". */
 const char* HcommGfxVersion(void);
