@@ -90,6 +90,7 @@ static HcommGfxLaunchRecord record(uint32_t kind, int dtype, uint32_t op, uint32
 /* ---- microscaled 4-bit floating point --------------------------------------------------------------------------- */
 
 #define HG_MX_MAX_COLS (1ull << 34)
+#define HG_MX_PRODUCT_STRIDE (1ull << 23)
 
 static uint64_t mx_blocks(uint64_t cols) { return cols / HCOMM_GFX_MX_BLOCK + (cols % HCOMM_GFX_MX_BLOCK != 0); }
 
@@ -195,8 +196,12 @@ int32_t HcommGfxMxReduceKOnThread(
 
 static void product_form(HgMxProduct* a)
 {
-    const uint32_t edge = a->m <= 16u ? 16u : 32u;
+    uint32_t edge = a->m <= 16u ? 16u : 32u;
     a->form = edge == 16u ? HG_PRODUCT_DIRECT_16 : HG_PRODUCT_DIRECT_32;
+    if (a->m > 256u && a->n > 256u) {
+        a->form = HG_PRODUCT_TILE;
+        edge = 256u;
+    }
     a->wgs = (a->m + edge - 1u) / edge * ((a->n + edge - 1u) / edge);
 }
 
@@ -215,7 +220,7 @@ int32_t HcommGfxMxProductKOnThread(
     HgMxProduct p;
     memset(&p, 0, sizeof(p));
     /* 16 results an edge at least: the number of workgroups stays below 2^31 */
-    int rc = m > HG_LIMIT_ROWS - 512u || n > HG_LIMIT_ROWS - 512u || mx_blocks(cols) * HCOMM_GFX_MX_BLOCK_BYTES >= (1ull << 23) ? HCCL_E_NOT_SUPPORT : HCCL_SUCCESS;
+    int rc = m > HG_LIMIT_ROWS - 512u || n > HG_LIMIT_ROWS - 512u || mx_blocks(cols) * HCOMM_GFX_MX_BLOCK_BYTES >= HG_MX_PRODUCT_STRIDE ? HCCL_E_NOT_SUPPORT : HCCL_SUCCESS;
     if (rc == HCCL_SUCCESS && (m + 15u) / 16u * ((n + 15u) / 16u) > HG_LIMIT_WGS) rc = HCCL_E_NOT_SUPPORT;
     if (rc == HCCL_SUCCESS) {
         Range r[1 + 4 * HCOMM_GFX_MAX_RANKS];
@@ -224,7 +229,9 @@ int32_t HcommGfxMxProductKOnThread(
         for (uint32_t j = 0; j < k; ++j) {
             if (!mx_view(&p.a[j], &r[1 + 4 * j], &r[2 + 4 * j], &a[j], m, cols)) return HCCL_E_PARA;
             if (!mx_view(&p.b[j], &r[3 + 4 * j], &r[4 + 4 * j], &b[j], n, cols)) return HCCL_E_PARA;
-            if ((m > 1 && a[j].packedStride >= (1ull << 23)) || (n > 1 && b[j].packedStride >= (1ull << 23))) rc = HCCL_E_NOT_SUPPORT;
+            /* 256 rows of a tile are told apart by 32-bit offsets */
+            if (m > 1 && (a[j].packedStride >= HG_MX_PRODUCT_STRIDE || a[j].scaleStride >= HG_MX_PRODUCT_STRIDE)) rc = HCCL_E_NOT_SUPPORT;
+            if (n > 1 && (b[j].packedStride >= HG_MX_PRODUCT_STRIDE || b[j].scaleStride >= HG_MX_PRODUCT_STRIDE)) rc = HCCL_E_NOT_SUPPORT;
         }
         if (!clear_of(&r[0], r, 1 + 4 * k, NULL)) return HCCL_E_PARA;
     }

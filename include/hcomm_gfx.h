@@ -1087,7 +1087,7 @@ int32_t HcommGfxMxReduceKOnThread(
  * dst[i, j] = sum over ranks r < k and c < cols of a[r][i, c] * b[r][j, c]: the product of a row-parallel layer whose
  * inner length the ranks share, and the reduction of their partial results, in one pass (k = 1: a plain product).
  * a[r] is m x cols (activations), b[r] n x cols (weights); sums in fp32, rounded once to dstType.
- * cols == 0 is HCCL_E_PARA, m == 0 or n == 0 succeed without doing anything.  packedStride below 2^23.
+ * cols == 0 is HCCL_E_PARA, m == 0 or n == 0 succeed without doing anything.  Strides of a and b below 2^23.
  */
 int32_t HcommGfxMxProductKOnThread(
     ThreadHandle thread, void* dst, uint64_t dstStride, HcommDataType dstType, const HcommGfxMxView* a,
