@@ -151,13 +151,18 @@ template <int DT, int FA, int FB> __global__ __launch_bounds__(256) void k_mx_pr
 //
 // A workgroup of four wavefronts owns 256 x 256 results, each wavefront 128 x 128 of them in accumulators (16 matrix
 // instructions of 32 x 32 x 64 for every 64 columns).  A stage of 256 columns of both operands (64 KiB) is copied to LDS
-// without passing through registers while the stage before it is multiplied; one barrier a stage tells that all four have
-// their copies there and are done with the stage before.  Rows lie in LDS as eight blocks, block b of row r at place b ^ (r % 8),
-// so that both the copies (eight whole rows an instruction) and the reads (one block of 32 rows) meet every bank evenly.
-// Scales go to registers: eight bytes of a row a stage, of which the two lanes of a row take every other byte.
+// without passing through registers while the stage before it is multiplied.  Rows lie in LDS as eight blocks, block b of
+// row r at place b ^ (r % 8), so that both the copies (eight whole rows an instruction) and the reads (one block of 32
+// rows) meet every bank evenly.  Scales are fetched by one lane a row, eight bytes a stage, and go through LDS too: fetched by
+// the lanes that need them, each would touch 32 lines for a quarter of the lanes' worth of new bytes.
+// The wavefronts meet once a stage, before its last quarter is multiplied: by then everything of the stage is in
+// registers, its buffer takes the stage after the next, and the fragments of the next one arrive behind that quarter.
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint64_t u64_at1 __attribute__((aligned(1)));
+typedef __attribute__((address_space(3))) uint8_t lds_byte;
+typedef __attribute__((address_space(3))) u32x4 lds_vec;
+typedef __attribute__((address_space(3))) uint64_t lds_u64;
 
 #define STAGE_BLOCKS 8u
 #define TILE_ROWS 256u
@@ -168,44 +173,50 @@ template <int T> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc, MX_FP4, MX_FP4, T, (int)sa, T, (int)sb);
 }
 
-typedef __attribute__((address_space(3))) uint8_t lds_byte;
-typedef __attribute__((address_space(3))) u32x4 lds_vec;
-
-// one operand's rows of the tile, as distances in bytes: those that this lane copies a block of, those of its four
-// fragments' scales; rows past the end are the last one once more, their results are not stored
+// One operand's rows of the tile.  Copies go through a buffer descriptor that ends with the matrix' last block: rows
+// past it are not read, whatever lies in their place has no result that is stored.  Scales are read by address, those
+// of rows past the end from the last row once more.
 struct Side {
-    uint32_t copy[8], scale[4];
+    uint32_t rows_at[8]; // this wavefront's eight copies of a stage, as distances of their first rows (scalars)
+    uint32_t lane_at;    // and from there this lane's row
+    uint32_t scale_at;   // distance of the scale row that this lane fetches
+    uint32_t bytes;      // of the tile's rows of the matrix
 };
 
-__device__ __forceinline__ Side place_side(const HgMxView& v, uint32_t row0, uint32_t rows, uint32_t wave, uint32_t lane, uint32_t frag0)
+__device__ __forceinline__ Side place_side(const HgMxView& v, uint32_t row0, uint32_t rows, uint32_t blocks, uint32_t wave, uint32_t lane)
 {
     Side s;
-    const uint32_t last = rows - 1u - row0;
+    const uint32_t last = min(rows - row0, TILE_ROWS) - 1u, stride = (uint32_t)v.packed_stride;
 #pragma unroll
-    for (uint32_t i = 0; i < 8u; ++i) s.copy[i] = min((wave * 8u + i) * 8u + (lane >> 3), last) * (uint32_t)v.packed_stride;
-#pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i) s.scale[i] = min(frag0 + i * 32u + (lane & 31u), last) * (uint32_t)v.scale_stride;
+    for (uint32_t i = 0; i < 8u; ++i) s.rows_at[i] = (wave * 8u + i) * 8u * stride;
+    s.lane_at = (lane >> 3) * stride;
+    s.scale_at = min(threadIdx.x, last) * (uint32_t)v.scale_stride;
+    s.bytes = last * stride + blocks * HCOMM_GFX_MX_BLOCK_BYTES;
     return s;
 }
 
-// The stage that begins at block `first` on its way to LDS, its scales to registers.  Past the rows' last block that
-// block is copied once more and its scale is 0: with 2^-127 on both sides the products are far below what fp32 holds.
-__device__ __forceinline__ void stage_side(lds_byte* to, uint64_t (&scale)[4], const Side& s, const HgMxView& v, uint32_t row0, uint32_t wave, uint32_t lane, uint32_t first, uint32_t blocks)
+// The stage that begins at block `first` on its way to LDS.  Past the rows' last block that block is copied once more;
+// its scale is 0 (fetch_scales), and with 2^-127 on both sides the products are far below what fp32 holds.
+__device__ __forceinline__ void copy_stage(lds_byte* to, const Side& s, const HgMxView& v, uint32_t row0, uint32_t wave, uint32_t lane, uint32_t first, uint32_t blocks)
 {
-    const uint8_t* base = v.packed + (uint64_t)row0 * v.packed_stride;
-    const uint32_t block = min(first + ((lane & 7u) ^ (lane >> 3)), blocks - 1u) * HCOMM_GFX_MX_BLOCK_BYTES;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(v.packed + (uint64_t)row0 * v.packed_stride, 0, (int)s.bytes, HG_BUFFER_WORD3);
+    const uint32_t at = s.lane_at + min(first + ((lane & 7u) ^ (lane >> 3)), blocks - 1u) * HCOMM_GFX_MX_BLOCK_BYTES;
 #pragma unroll
     for (uint32_t i = 0; i < 8u; ++i)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(base + (s.copy[i] + block)),
-                                         (__attribute__((address_space(3))) uint32_t*)(to + (wave * 8u + i) * 1024u), 16, 0, 0);
-    const uint32_t from = min(first, blocks - STAGE_BLOCKS); // the host takes this form from STAGE_BLOCKS blocks on
-    const uint8_t* scales = v.scales + (uint64_t)row0 * v.scale_stride + from;
-#pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i) scale[i] = *(const __attribute__((address_space(1))) u64_at1*)(scales + s.scale[i]) >> (8u * (first - from));
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + (wave * 8u + i) * 1024u), 16, (int)(at + s.rows_at[i]), 0, 0, 0);
 }
 
-// elements of the last block past cols do not count: one operand's become 0, a row to a lane
-__device__ __forceinline__ void cut_stage(lds_byte* la, uint32_t block, uint32_t n)
+// the eight scales of this lane's row; the host takes this form from STAGE_BLOCKS blocks on
+__device__ __forceinline__ uint64_t fetch_scales(const Side& s, const HgMxView& v, uint32_t row0, uint32_t first, uint32_t blocks)
+{
+    const uint8_t* base = v.scales + (uint64_t)row0 * v.scale_stride + min(first, blocks - STAGE_BLOCKS);
+    return *(const __attribute__((address_space(1))) u64_at1*)(base + s.scale_at);
+}
+
+// Elements of the last block past cols do not count: one operand's become 0, in the rows that this wavefront has copied.
+// n: the elements of it that count, 32 in stages that end with a whole block (a branch around this would end the basic
+// block in which the compiler places the matrix instructions).
+__device__ __forceinline__ void cut_rows(lds_byte* la, uint32_t block, uint32_t n)
 {
     lds_vec* p = (lds_vec*)(la + threadIdx.x * 128u + ((block ^ (threadIdx.x & 7u)) << 4));
     u32x4 v = *p;
@@ -215,51 +226,64 @@ __device__ __forceinline__ void cut_stage(lds_byte* la, uint32_t block, uint32_t
         v[q] &= keep >= 8u ? 0xffffffffu : (1u << (4u * keep)) - 1u;
     }
     *p = v;
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
 }
 
-__device__ __forceinline__ void multiply_stage(f32x16 (&acc)[4][4], lds_byte* la, lds_byte* lb, uint32_t wm, uint32_t wn, uint32_t lane, const uint64_t (&sa)[4], const uint64_t (&sb)[4])
+// what a wavefront multiplies: four fragments of 32 rows and 64 columns of each operand
+struct Fragments {
+    u32x4 a[4], b[4];
+};
+
+__device__ __forceinline__ void read_fragments(Fragments& f, lds_byte* la, lds_byte* lb, uint32_t at, uint32_t t)
 {
-    const uint32_t r = lane & 31u, g = lane >> 5;
-    uint32_t xa[2][4], xb[2][4]; // this lane's bytes: of instruction t byte 2 (t % 2) of word t / 2
+    // at: row lane % 32 at place (lane / 32) ^ (row % 8); two blocks on with every t
 #pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i) {
-        xa[0][i] = (uint32_t)sa[i] >> (8u * g), xa[1][i] = (uint32_t)(sa[i] >> 32) >> (8u * g);
-        xb[0][i] = (uint32_t)sb[i] >> (8u * g), xb[1][i] = (uint32_t)(sb[i] >> 32) >> (8u * g);
-    }
+    for (uint32_t i = 0; i < 4u; ++i) f.a[i] = *(lds_vec*)(la + (at ^ (t << 5)) + i * 4096u);
 #pragma unroll
-    for (uint32_t t = 0; t < 4u; ++t) {
-        const uint32_t at = r * 128u + (((2u * t + g) ^ (r & 7u)) << 4);
-        u32x4 a[4], b[4];
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
-            a[i] = *(lds_vec*)(la + (wm * 128u + i * 32u) * 128u + at);
-            b[i] = *(lds_vec*)(lb + (wn * 128u + i * 32u) * 128u + at);
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i)
-#pragma unroll
-            for (uint32_t j = 0; j < 4u; ++j) {
-                if (t % 2u == 0u) acc[i][j] = mfma32<0>(a[i], b[j], acc[i][j], xa[t / 2u][i], xb[t / 2u][j]);
-                else acc[i][j] = mfma32<2>(a[i], b[j], acc[i][j], xa[t / 2u][i], xb[t / 2u][j]);
-            }
-    }
+    for (uint32_t i = 0; i < 4u; ++i) f.b[i] = *(lds_vec*)(lb + (at ^ (t << 5)) + i * 4096u);
 }
 
-// all of this wavefront's copies have arrived; then all wavefronts'
-__device__ __forceinline__ void copies_there()
+// a stage's scales of those fragments' rows, shifted so that instruction t takes byte 2 (t % 2) of word t / 2
+struct Scales {
+    uint64_t a[4], b[4];
+};
+
+__device__ __forceinline__ void read_scales(Scales& s, lds_u64* sa, lds_u64* sb, uint32_t lane)
 {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) s.a[i] = sa[i * 32u + (lane & 31u)], s.b[i] = sb[i * 32u + (lane & 31u)];
 }
 
-template <int DT> __global__ __launch_bounds__(256) void k_mx_product_tile(const HgMxProduct a)
+// T: the instruction of the stage; I0 .. I1: which fragments of a
+template <uint32_t T, uint32_t I0, uint32_t I1> __device__ __forceinline__ void multiply(f32x16 (&acc)[4][4], const Fragments& f, const Scales& s, uint32_t shift)
+{
+    uint32_t xa[4], xb[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) xa[i] = (uint32_t)(s.a[i] >> (32u * (T / 2u))) >> shift, xb[i] = (uint32_t)(s.b[i] >> (32u * (T / 2u))) >> shift;
+#pragma unroll
+    for (uint32_t i = I0; i < I1; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; ++j) acc[i][j] = mfma32<2u * (T % 2u)>(f.b[j], f.a[i], acc[i][j], xb[j], xa[i]);
+}
+
+// The compiler's order of what it may move: N times a matrix instruction followed by one read of LDS, by one access to
+// memory.  A wavefront issues in order and is alone on its SIMD, so whatever is not placed behind a matrix instruction that
+// is still running leaves the matrix unit idle.
+template <int N> __device__ __forceinline__ void behind_each(bool reads, bool loads)
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (reads) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (loads) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+    }
+}
+
+// TAIL: rows end inside a block
+template <int DT, bool TAIL> __global__ __launch_bounds__(256) void k_mx_product_tile(const HgMxProduct a)
 {
     // four arrays, not one: the compiler then sees that the copies into one pair do not touch the pair that is read
     __shared__ __align__(1024) uint8_t a0[32768], b0[32768], a1[32768], b1[32768];
+    __shared__ uint64_t scales[2][2][TILE_ROWS];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1u;
     const uint32_t tiles_m = (a.m + TILE_ROWS - 1u) / TILE_ROWS, tiles_n = (a.n + TILE_ROWS - 1u) / TILE_ROWS;
     // each XCD walks tiles next to one another, four rows of tiles at a time: its L2 keeps what they share
@@ -275,56 +299,129 @@ template <int DT> __global__ __launch_bounds__(256) void k_mx_product_tile(const
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
     // the ranks' matrices have the same strides (the host sees to it)
-    const Side ra = place_side(a.a[0], m0, a.m, wave, lane, wm * 128u), rb = place_side(a.b[0], n0, a.n, wave, lane, wn * 128u);
-    uint64_t sa[2][4], sb[2][4];
-    uint32_t rank = 0, stage = 0; // of the copies
+    const Side ra = place_side(a.a[0], m0, a.m, blocks, wave, lane), rb = place_side(a.b[0], n0, a.n, blocks, wave, lane);
+    const uint32_t at = (lane & 31u) * 128u + (((lane >> 5) ^ (lane & 7u)) << 4), shift = 8u * (lane >> 5);
     const uint32_t total = a.k * stages, tail = a.cols % HCOMM_GFX_MX_BLOCK;
-    uint32_t left = stages; // of the products: stages to the rank's end
-#define STAGE(TO_A, TO_B, S)                                                                                     \
-    {                                                                                                            \
-        stage_side((lds_byte*)(TO_A), sa[S], ra, a.a[rank], m0, wave, lane, stage * STAGE_BLOCKS, blocks);       \
-        stage_side((lds_byte*)(TO_B), sb[S], rb, a.b[rank], n0, wave, lane, stage * STAGE_BLOCKS, blocks);       \
-        if (++stage == stages) stage = 0u, ++rank;                                                               \
+    uint32_t rank = 0, stage = 0;       // of the copies and fetches
+    uint32_t left = stages, done = 0;   // of the stages that have arrived: how many to the rank's end, how many in all
+    uint64_t fetched_a, fetched_b;
+    Fragments f0, f1;
+    Scales s;
+    // where the next stage is: the rank's matrices, read ahead of their use
+    HgMxView va = a.a[0], vb = a.b[0];
+    // copies and fetches of the next stage; behind the last one that stage once more, which will not count
+#define ASK(TO_A, TO_B)                                                                                               \
+    {                                                                                                                 \
+        copy_stage((lds_byte*)(TO_A), ra, va, m0, wave, lane, stage * STAGE_BLOCKS, blocks);                          \
+        copy_stage((lds_byte*)(TO_B), rb, vb, n0, wave, lane, stage * STAGE_BLOCKS, blocks);                          \
+        fetched_a = fetch_scales(ra, va, m0, stage * STAGE_BLOCKS, blocks);                                           \
+        fetched_b = fetch_scales(rb, vb, n0, stage * STAGE_BLOCKS, blocks);                                           \
+        const bool ends = stage + 1u == stages, last = ends && rank + 1u == a.k;                                      \
+        stage = last ? stage : ends ? 0u : stage + 1u;                                                                \
+        rank = ends && !last ? rank + 1u : rank;                                                                      \
+        va = a.a[rank], vb = a.b[rank];                                                                               \
     }
-#define MULTIPLY(LA, LB, S)                                                                                      \
-    {                                                                                                            \
-        if (--left == 0u) {                                                                                      \
-            left = stages;                                                                                       \
-            if (tail) cut_stage((lds_byte*)(LA), (blocks - 1u) % STAGE_BLOCKS, tail);                            \
-        }                                                                                                        \
-        multiply_stage(acc, (lds_byte*)(LA), (lds_byte*)(LB), wm, wn, lane, sa[S], sb[S]);                       \
+    // what was asked for last has arrived: its scales (and the cut) on their way to LDS ...
+#define ARRIVE(LA, S)                                                                                                 \
+    {                                                                                                                 \
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                                                              \
+        left = left == 0u ? stages - 1u : left - 1u;                                                                  \
+        /* scales past the rows' last block are shifted out: the fetch went back by as many */                        \
+        const uint32_t out = left == 0u ? (stages * STAGE_BLOCKS - blocks) * 8u : 0u;                                 \
+        const uint64_t counts = done++ < total ? ~0ull : 0ull;                                                        \
+        scales[S][0][threadIdx.x] = (fetched_a >> out) & counts;                                                      \
+        scales[S][1][threadIdx.x] = (fetched_b >> out) & counts;                                                      \
+        if (TAIL) cut_rows((lds_byte*)(LA), (blocks - 1u) % STAGE_BLOCKS, left == 0u ? tail : HCOMM_GFX_MX_BLOCK);    \
     }
-    // stages in pairs, so that which buffer a stage lies in is known to the compiler; an odd one goes first
-    if (total & 1u) {
-        STAGE(a1, b1, 1)
-        copies_there();
-        if (total > 1u) STAGE(a0, b0, 0)
-        MULTIPLY(a1, b1, 1)
-    } else {
-        STAGE(a0, b0, 0)
+    // ... and all wavefronts have come this far
+#define MEET()                                                                                                        \
+    {                                                                                                                 \
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                                                            \
+        __builtin_amdgcn_s_barrier();                                                                                 \
+        asm volatile("" ::: "memory");                                                                                \
     }
+#define FRAGMENTS(F, LA, LB, T) read_fragments(F, (lds_byte*)(LA) + wm * 16384u, (lds_byte*)(LB) + wn * 16384u, at, T);
+#define SCALES(S) read_scales(s, (lds_u64*)scales[S][0] + wm * 128u, (lds_u64*)scales[S][1] + wn * 128u, lane);
+#define STAGE(LA, LB, NEXT_A, NEXT_B, NEXT)                                                                           \
+    {                                                                                                                 \
+        FRAGMENTS(f1, LA, LB, 1)                                                                                      \
+        multiply<0, 0, 4>(acc, f0, s, shift);                                                                         \
+        behind_each<8>(true, false);                                                                                  \
+        __builtin_amdgcn_sched_barrier(0);                                                                            \
+        FRAGMENTS(f0, LA, LB, 2)                                                                                      \
+        multiply<1, 0, 4>(acc, f1, s, shift);                                                                         \
+        behind_each<8>(true, false);                                                                                  \
+        __builtin_amdgcn_sched_barrier(0);                                                                            \
+        FRAGMENTS(f1, LA, LB, 3)                                                                                      \
+        multiply<2, 0, 2>(acc, f0, s, shift);                                                                         \
+        behind_each<8>(true, false);                                                                                  \
+        __builtin_amdgcn_sched_barrier(0);                                                                            \
+        ARRIVE(NEXT_A, NEXT)                                                                                          \
+        multiply<2, 2, 4>(acc, f0, s, shift);                                                                         \
+        __builtin_amdgcn_sched_barrier(0);                                                                            \
+        MEET()                                                                                                        \
+        Scales now = s;                                                                                               \
+        FRAGMENTS(f0, NEXT_A, NEXT_B, 0)                                                                              \
+        SCALES(NEXT)                                                                                                  \
+        ASK(LA, LB)                                                                                                   \
+        multiply<3, 0, 4>(acc, f1, now, shift);                                                                       \
+        behind_each<16>(true, true);                                                                                  \
+        __builtin_amdgcn_sched_barrier(0);                                                                            \
+    }
+    ASK(a0, b0)
+    ARRIVE(a0, 0)
+    MEET()
+    ASK(a1, b1)
+    FRAGMENTS(f0, a0, b0, 0)
+    SCALES(0)
+    // stages in pairs, so that which buffers a stage lies in is known to the compiler
 #pragma unroll 1
-    for (uint32_t pairs = total >> 1; pairs != 0u; --pairs) {
-        copies_there();
-        STAGE(a1, b1, 1)
-        MULTIPLY(a0, b0, 0)
-        copies_there();
-        if (pairs > 1u) STAGE(a0, b0, 0)
-        MULTIPLY(a1, b1, 1)
+    for (uint32_t pairs = (total + 1u) >> 1; pairs != 0u; --pairs) {
+        STAGE(a0, b0, a1, b1, 1)
+        STAGE(a1, b1, a0, b0, 0)
     }
-#undef MULTIPLY
-#undef STAGE
+    // All copies have arrived, in this wavefront and in the others: the LDS is free for the results.  Four neighbours of
+    // a row lie in a lane; by way of LDS they become runs of a row that a store instruction writes in one piece.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    constexpr uint32_t ES = ElemSize<DT>::v, PASS = ES == 4u ? 2u : 4u, CHUNKS = 128u * ES / 16u; // fragments of rows at a time; chunks of 16 bytes of a row
+    lds_byte* mine = (lds_byte*)(wave == 0u ? a0 : wave == 1u ? b0 : wave == 2u ? a1 : b1);
 #pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i)
+    for (uint32_t i0 = 0; i0 < 4u; i0 += PASS) {
 #pragma unroll
-        for (uint32_t j = 0; j < 4u; ++j) {
-            const uint32_t col = n0 + wn * 128u + j * 32u + (lane & 31u);
+        for (uint32_t i = 0; i < PASS; ++i)
 #pragma unroll
-            for (uint32_t e = 0; e < 16u; ++e) {
-                const uint32_t row = m0 + wm * 128u + i * 32u + 8u * (e / 4u) + 4u * (lane >> 5) + e % 4u;
-                if (row < a.m && col < a.n) put<DT>(a.dst, row * a.dst_stride + col, acc[i][j][e]);
+            for (uint32_t j = 0; j < 4u; ++j)
+#pragma unroll
+                for (uint32_t q = 0; q < 4u; ++q) {
+                    const f32x16& v = acc[i0 + i][j];
+                    const uint32_t row = i * 32u + (lane & 31u), col = j * 32u + 8u * q + 4u * (lane >> 5); // of four results
+                    lds_byte* p = mine + row * 128u * ES + (((col * ES / 16u) ^ (row & (CHUNKS - 1u))) << 4) + col * ES % 16u;
+                    if (ES == 4u) *(lds_vec*)p = u32x4{f32_bits(v[4 * q]), f32_bits(v[4 * q + 1]), f32_bits(v[4 * q + 2]), f32_bits(v[4 * q + 3])};
+                    else {
+                        const float f[8] = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], 0.0f, 0.0f, 0.0f, 0.0f};
+                        const Raw8<DT> r = narrow8<DT>(f);
+                        *(lds_u64*)p = (uint64_t)r.w[1] << 32 | r.w[0];
+                    }
+                }
+        __builtin_amdgcn_wave_barrier();
+        // eight results a lane and step: 16 lanes to a row
+#pragma unroll
+        for (uint32_t t = 0; t < PASS * 8u; ++t) {
+            const uint32_t row = t * 4u + (lane >> 4), col = (lane & 15u) * 8u;
+            Raw8<DT> r;
+#pragma unroll
+            for (uint32_t h = 0; h < Raw8<DT>::words / 4u; ++h) {
+                const u32x4 v = *(lds_vec*)(mine + row * 128u * ES + (((col * ES / 16u + h) ^ (row & (CHUNKS - 1u))) << 4));
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) r.w[4u * h + e] = v[e];
             }
+            const uint32_t m = m0 + wm * 128u + i0 * 32u + row, n = n0 + wn * 128u + col;
+            if (m < a.m) store8<DT>((uint8_t*)a.dst + m * a.dst_stride * ES, n, a.n, r);
         }
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 
 template <int DT> int launch(hipStream_t st, const HgMxProduct* a)
@@ -333,7 +430,10 @@ template <int DT> int launch(hipStream_t st, const HgMxProduct* a)
     switch (a->form) {
         case HG_PRODUCT_DIRECT_16: hipLaunchKernelGGL((k_mx_product_direct<DT, 1, 1>), g, b, 0, st, *a); break;
         case HG_PRODUCT_DIRECT_32: hipLaunchKernelGGL((k_mx_product_direct<DT, 2, 2>), g, b, 0, st, *a); break;
-        case HG_PRODUCT_TILE: hipLaunchKernelGGL((k_mx_product_tile<DT>), g, b, 0, st, *a); break;
+        case HG_PRODUCT_TILE:
+            if (a->cols % HCOMM_GFX_MX_BLOCK) hipLaunchKernelGGL((k_mx_product_tile<DT, true>), g, b, 0, st, *a);
+            else hipLaunchKernelGGL((k_mx_product_tile<DT, false>), g, b, 0, st, *a);
+            break;
         default: return HCCL_E_INTERNAL;
     }
     return rc(hipGetLastError());
