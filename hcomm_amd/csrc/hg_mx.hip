@@ -8,30 +8,48 @@
 namespace {
 
 // ---- where a lane's group lies ------------------------------------------------------------------------------
+//
+// ONE: every workgroup lies in one row, so that the row and where the workgroup begins in it are scalars and a lane adds
+// a small distance of its own; otherwise a workgroup takes several short rows and the row is the lane's.
 
-struct Place {
+template <bool ONE> struct Place {
     uint64_t row;
-    uint32_t group; // of the row
+    uint32_t tile;  // first group of the workgroup in its row (ONE) or 0
+    uint32_t group; // of the row, from `tile` on
     bool there;
 };
 
-__device__ __forceinline__ Place place_of(const HgMxGrid& g, uint32_t q)
+template <bool ONE, uint32_t U> __device__ __forceinline__ Place<ONE> place_of(const HgMxGrid& g, uint32_t u)
 {
-    const uint32_t wg = blockIdx.x;
-    Place p;
-    if (g.rows_per_wg <= 1u) {
-        const uint32_t row = wg / g.tiles, tile = wg - row * g.tiles;
+    const uint32_t wg = blockIdx.x, q = u * 256u + threadIdx.x;
+    Place<ONE> p;
+    if (ONE) {
+        const uint32_t row = g.rows == 1u ? 0u : wg / g.tiles;
         p.row = row;
-        p.group = tile * HG_MX_TILE + q;
-        p.there = p.group < g.groups;
+        p.tile = (wg - row * g.tiles) * (256u * U);
+        p.group = q;
+        p.there = q < g.groups - p.tile;
     } else {
-        // q / groups by a multiplication: with q < 2^10 and 2 <= groups < 2^10 the factor rounded up to 2^-20 is exact
+        // q / groups by a multiplication: with q < 2^10 and 4 <= groups < 2^10 the factor rounded up to 2^-20 is exact
         const uint32_t r = (q * (((1u << 20) + g.groups - 1u) / g.groups)) >> 20;
         p.row = (uint64_t)wg * g.rows_per_wg + r;
+        p.tile = 0u;
         p.group = q - r * g.groups;
         p.there = r < g.rows_per_wg && p.row < g.rows;
     }
     return p;
+}
+
+// eight elements of a dense matrix at a place, and where they go back
+template <int DT, bool ONE> __device__ __forceinline__ Raw8<DT> load_at(const void* m, uint64_t stride, const Place<ONE>& p, uint64_t cols)
+{
+    const uint64_t at = (uint64_t)p.tile * 8u;
+    return load8<DT>((const uint8_t*)m + (p.row * stride + at) * ElemSize<DT>::v, p.group * 8u, p.there ? cols - at : 0u);
+}
+template <int DT, bool ONE> __device__ __forceinline__ void store_at(void* m, uint64_t stride, const Place<ONE>& p, uint64_t cols, const Raw8<DT>& v)
+{
+    const uint64_t at = (uint64_t)p.tile * 8u;
+    store8<DT>((uint8_t*)m + (p.row * stride + at) * ElemSize<DT>::v, p.group * 8u, p.there ? cols - at : 0u, v);
 }
 
 // the largest of a value over the four lanes of a block
@@ -65,25 +83,21 @@ __device__ __forceinline__ uint32_t encode8(const float (&f)[8], uint32_t s)
     return s == 255u ? 0u : w;
 }
 
-__device__ __forceinline__ void put_group(const HgMxView& out, const Place& p, uint32_t w, uint32_t s)
+template <bool ONE> __device__ __forceinline__ void put_group(const HgMxView& out, const Place<ONE>& p, uint32_t w, uint32_t s)
 {
-    *(__attribute__((address_space(1))) uint32_t*)(out.packed + p.row * out.packed_stride + (uint64_t)p.group * 4u) = w;
-    if ((p.group & 3u) == 0u) out.scales[p.row * out.scale_stride + (p.group >> 2)] = (uint8_t)s;
+    uint8_t* packed = out.packed + (p.row * out.packed_stride + (uint64_t)p.tile * 4u);
+    uint8_t* scales = out.scales + (p.row * out.scale_stride + (p.tile >> 2));
+    *(__attribute__((address_space(1))) uint32_t*)(packed + p.group * 4u) = w;
+    if ((p.group & 3u) == 0u) ((__attribute__((address_space(1))) uint8_t*)scales)[p.group >> 2] = (uint8_t)s;
 }
 
 // ---- quantise ---------------------------------------------------------------------------------------------------
 
-template <int DT> __global__ __launch_bounds__(256) void k_mx_quantize(const HgMxQuantize a)
+template <int DT, bool ONE, uint32_t U> __global__ __launch_bounds__(256) void k_mx_quantize(const HgMxQuantize a)
 {
-    constexpr uint32_t U = HG_MX_TILE / 256u;
-    Place p[U];
     Raw8<DT> x[U];
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) {
-        p[u] = place_of(a.grid, u * 256u + threadIdx.x);
-        const uint8_t* row = (const uint8_t*)a.src + p[u].row * a.src_stride * ElemSize<DT>::v;
-        x[u] = load8<DT>(row, (uint64_t)p[u].group * 8u, p[u].there ? a.grid.cols : 0u);
-    }
+    for (uint32_t u = 0; u < U; ++u) x[u] = load_at<DT>(a.src, a.src_stride, place_of<ONE, U>(a.grid, u), a.grid.cols);
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
         float f[8];
@@ -95,7 +109,8 @@ template <int DT> __global__ __launch_bounds__(256) void k_mx_quantize(const HgM
             m = b > m ? b : m;
         }
         const uint32_t s = scale_of(quad_max(m));
-        if (p[u].there) put_group(a.out, p[u], encode8(f, s), s);
+        const Place<ONE> p = place_of<ONE, U>(a.grid, u);
+        if (p.there) put_group(a.out, p, encode8(f, s), s);
     }
 }
 
@@ -126,101 +141,145 @@ __device__ __forceinline__ void decode8(uint32_t w, float sc, float (&f)[8])
     f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y, f[4] = c.x, f[5] = c.y, f[6] = d.x, f[7] = d.y;
 }
 
-template <int DT> __global__ __launch_bounds__(256) void k_mx_reduce(const HgMxReduce a)
+// The arguments as the kernel takes them: the runtime copies them at every launch, so a fold of few ranks carries few views.
+template <uint32_t N> struct FoldArgs {
+    HgMxGrid grid;
+    HgMxView src[N];
+    HgMxView again;
+    void* dst;
+    const void* addend;
+    uint64_t dst_stride, addend_stride;
+    uint32_t k;
+};
+
+// the fp64 sum of the ranks' values from `to` on, or of the ranks' values alone where nothing is there yet
+template <uint32_t B> __device__ __forceinline__ void fold_wide(double (&to)[8], bool empty, const uint32_t (&w)[B], const uint32_t (&s)[B], uint32_t n)
 {
-    constexpr uint32_t U = HG_MX_TILE / 256u;
-    const bool join = a.k > FOLD_BATCH || a.addend != nullptr; // more than one exact sum to add up
+    for (uint32_t j = 0; j < n; ++j) {
+        uint32_t wj = w[0], sj = s[0];
+#pragma unroll
+        for (uint32_t i = 1; i < B; ++i) wj = i == j ? w[i] : wj, sj = i == j ? s[i] : sj;
+        float x[8];
+        decode8(wj, scale_f32(sj), x);
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) to[e] = empty && j == 0u ? (double)x[e] : to[e] + (double)x[e];
+    }
+}
+
+// JOIN: there is an addend or there are more than eight ranks, so that fp64 has to join exact sums
+template <int DT, bool ONE, uint32_t U, uint32_t N, bool JOIN> __global__ __launch_bounds__(256) void k_mx_reduce(const FoldArgs<N> a)
+{
+    constexpr uint32_t B = N < FOLD_BATCH ? N : FOLD_BATCH;
+#pragma unroll 1
     for (uint32_t u = 0; u < U; ++u) {
-        const Place p = place_of(a.grid, u * 256u + threadIdx.x);
-        const uint64_t at = (uint64_t)p.group * 8u;
-        double v[8];
-        float f[8];
-        bool wide = join;
-        if (a.addend) {
-            float x[8];
-            const uint8_t* row = (const uint8_t*)a.addend + p.row * a.addend_stride * ElemSize<DT>::v;
-            widen8<DT>(load8<DT>(row, at, p.there ? a.grid.cols : 0u), x);
+        const Place<ONE> p = place_of<ONE, U>(a.grid, u);
+        double v[8];             // JOIN: the sum
+        float odd[8], near[8];   // the sum as what narrower types round it from, and rounded to fp32
+        Raw8<DT> own;
+        if (JOIN && a.addend) own = load_at<DT>(a.addend, a.addend_stride, p, a.grid.cols);
+        for (uint32_t j0 = 0; j0 < (JOIN ? a.k : 1u); j0 += B) {
+            uint32_t w[B], s[B];
+            const uint32_t n = N == 1u ? 1u : min(a.k - j0, B);
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e) v[e] = (double)x[e];
-        }
-        for (uint32_t j0 = 0; j0 < a.k; j0 += FOLD_BATCH) {
-            uint32_t w[FOLD_BATCH], s[FOLD_BATCH];
-#pragma unroll
-            for (uint32_t j = 0; j < FOLD_BATCH; ++j) {
+            for (uint32_t j = 0; j < B; ++j) {
                 w[j] = 0u, s[j] = 127u;
-                if (j0 + j < a.k && p.there) {
+                if (j < n && p.there) {
                     const HgMxView& r = a.src[j0 + j];
-                    w[j] = *(const __attribute__((address_space(1))) uint32_t*)(r.packed + p.row * r.packed_stride + (uint64_t)p.group * 4u);
-                    s[j] = ((const __attribute__((address_space(1))) uint8_t*)r.scales)[p.row * r.scale_stride + (p.group >> 2)];
+                    const uint8_t* packed = r.packed + (p.row * r.packed_stride + (uint64_t)p.tile * 4u);
+                    const uint8_t* scales = r.scales + (p.row * r.scale_stride + (p.tile >> 2));
+                    w[j] = *(const __attribute__((address_space(1))) uint32_t*)(packed + p.group * 4u);
+                    s[j] = ((const __attribute__((address_space(1))) uint8_t*)scales)[p.group >> 2];
                 }
+            }
+            const bool empty = !JOIN || (j0 == 0u && !a.addend);
+            if (JOIN && j0 == 0u && a.addend) {
+                float x[8];
+                widen8<DT>(own, x);
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; ++e) v[e] = (double)x[e];
             }
             uint32_t lo = 255u, hi = 0u; // scales that have a nonzero element under them
 #pragma unroll
-            for (uint32_t j = 0; j < FOLD_BATCH; ++j) {
+            for (uint32_t j = 0; j < B; ++j) {
                 const bool any = (w[j] & 0x77777777u) != 0u || s[j] == 255u;
                 lo = any && s[j] < lo ? s[j] : lo;
                 hi = any && s[j] > hi ? s[j] : hi;
             }
-            const bool apart = hi > lo + 17u || hi > 240u;
-            const bool first = j0 == 0u && !a.addend;
-            if (!apart) {
+            if (N == 1u || !(hi > lo + 17u || hi > 240u)) {
+                float f[8];
                 decode8(w[0], scale_f32(s[0]), f);
 #pragma unroll
-                for (uint32_t j = 1; j < FOLD_BATCH; ++j)
-                    if (j0 + j < a.k) {
+                for (uint32_t j = 1; j < B; ++j)
+                    if (j < n) {
                         float x[8];
                         decode8(w[j], scale_f32(s[j]), x);
 #pragma unroll
                         for (uint32_t e = 0; e < 8u; ++e) f[e] += x[e];
                     }
-                if (wide) {
 #pragma unroll
-                    for (uint32_t e = 0; e < 8u; ++e) v[e] = first ? (double)f[e] : v[e] + (double)f[e];
+                for (uint32_t e = 0; e < 8u; ++e) {
+                    if (JOIN) v[e] = empty ? (double)f[e] : v[e] + (double)f[e];
+                    else odd[e] = near[e] = f[e];
                 }
+            } else if (JOIN) {
+                fold_wide(v, empty, w, s, n);
             } else {
-                wide = true;
-                for (uint32_t j = 0; j < FOLD_BATCH && j0 + j < a.k; ++j) {
-                    uint32_t wj = w[0], sj = s[0];
+                double x[8];
+                fold_wide(x, true, w, s, n);
 #pragma unroll
-                    for (uint32_t i = 1; i < FOLD_BATCH; ++i) wj = i == j ? w[i] : wj, sj = i == j ? s[i] : sj;
-                    float x[8];
-                    decode8(wj, scale_f32(sj), x);
-#pragma unroll
-                    for (uint32_t e = 0; e < 8u; ++e) v[e] = first && j == 0u ? (double)x[e] : v[e] + (double)x[e];
-                }
+                for (uint32_t e = 0; e < 8u; ++e) odd[e] = to_odd(x[e]), near[e] = (float)x[e];
             }
         }
-        if (wide) {
+        if (JOIN) {
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e) f[e] = to_odd(v[e]);
+            for (uint32_t e = 0; e < 8u; ++e) odd[e] = to_odd(v[e]), near[e] = (float)v[e];
         }
+        if (a.dst) store_at<DT>(a.dst, a.dst_stride, p, a.grid.cols, DT == DT_F32 ? narrow8<DT>(near) : narrow8<DT>(odd));
         if (a.again.packed) {
+            const int64_t left = (int64_t)(a.grid.cols - ((uint64_t)p.tile + p.group) * 8u); // elements to the row's end
             uint32_t m = 0;
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e) {
-                if (at + e >= a.grid.cols) f[e] = 0.0f; // elements past the row's end do not count, whatever the inputs hold there
-                const uint32_t b = f32_bits(f[e]) & 0x7fffffffu;
+                if (left <= (int64_t)e) odd[e] = 0.0f; // elements past it do not count, whatever the inputs hold there
+                const uint32_t b = f32_bits(odd[e]) & 0x7fffffffu;
                 m = b > m ? b : m;
             }
             const uint32_t s = scale_of(quad_max(m));
-            if (p.there) put_group(a.again, p, encode8(f, s), s);
-        }
-        if (a.dst && p.there) {
-            if (DT == DT_F32 && wide) {
-#pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e) f[e] = (float)v[e];
-            }
-            store8<DT>((uint8_t*)a.dst + p.row * a.dst_stride * ElemSize<DT>::v, at, a.grid.cols, narrow8<DT>(f));
+            if (p.there) put_group(a.again, p, encode8(odd, s), s);
         }
     }
 }
 
-template <class A, class F> int launch(void* stream, const A* a, F kernel)
+template <class K, class A> int launch(hipStream_t st, uint32_t wgs, K kernel, const A& a)
 {
-    OnDeviceOf device((hipStream_t)stream);
-    if (device.err != hipSuccess) return HCCL_E_RUNTIME;
-    hipLaunchKernelGGL(kernel, dim3(a->grid.wgs), dim3(256), 0, (hipStream_t)stream, *a);
+    hipLaunchKernelGGL(kernel, dim3(wgs), dim3(256), 0, st, a);
     return rc(hipGetLastError());
+}
+
+template <int DT> int quantize(hipStream_t st, const HgMxQuantize& a)
+{
+    if (a.grid.rows_per_wg > 1u) return launch(st, a.grid.wgs, k_mx_quantize<DT, false, HG_MX_UNROLL>, a);
+    if (a.grid.tile == 256u) return launch(st, a.grid.wgs, k_mx_quantize<DT, true, 1>, a);
+    return launch(st, a.grid.wgs, k_mx_quantize<DT, true, HG_MX_UNROLL>, a);
+}
+
+template <int DT, uint32_t N, bool JOIN> int reduce_n(hipStream_t st, const HgMxReduce& a)
+{
+    FoldArgs<N> f;
+    f.grid = a.grid;
+    for (uint32_t j = 0; j < N; ++j) f.src[j] = a.src[j];
+    f.again = a.again;
+    f.dst = a.dst, f.addend = a.addend, f.dst_stride = a.dst_stride, f.addend_stride = a.addend_stride, f.k = a.k;
+    if (a.grid.rows_per_wg > 1u) return launch(st, a.grid.wgs, k_mx_reduce<DT, false, HG_MX_UNROLL, N, JOIN>, f);
+    if (a.grid.tile == 256u) return launch(st, a.grid.wgs, k_mx_reduce<DT, true, 1, N, JOIN>, f);
+    return launch(st, a.grid.wgs, k_mx_reduce<DT, true, HG_MX_UNROLL, N, JOIN>, f);
+}
+
+template <int DT> int reduce(hipStream_t st, const HgMxReduce& a)
+{
+    if (a.k > FOLD_BATCH) return reduce_n<DT, HCOMM_GFX_MAX_RANKS, true>(st, a);
+    if (a.addend) return reduce_n<DT, FOLD_BATCH, true>(st, a);
+    return a.k == 1u ? reduce_n<DT, 1, false>(st, a) : reduce_n<DT, FOLD_BATCH, false>(st, a);
 }
 
 } // namespace
@@ -230,10 +289,12 @@ extern "C" {
 int hg_launch_mx_quantize(void* stream, const void* args)
 {
     const HgMxQuantize* a = (const HgMxQuantize*)args;
+    OnDeviceOf device((hipStream_t)stream);
+    if (device.err != hipSuccess) return HCCL_E_RUNTIME;
     switch (a->dtype) {
-        case DT_F16: return launch(stream, a, k_mx_quantize<DT_F16>);
-        case DT_BF16: return launch(stream, a, k_mx_quantize<DT_BF16>);
-        case DT_F32: return launch(stream, a, k_mx_quantize<DT_F32>);
+        case DT_F16: return quantize<DT_F16>((hipStream_t)stream, *a);
+        case DT_BF16: return quantize<DT_BF16>((hipStream_t)stream, *a);
+        case DT_F32: return quantize<DT_F32>((hipStream_t)stream, *a);
         default: return HCCL_E_PARA;
     }
 }
@@ -241,10 +302,12 @@ int hg_launch_mx_quantize(void* stream, const void* args)
 int hg_launch_mx_reduce(void* stream, const void* args)
 {
     const HgMxReduce* a = (const HgMxReduce*)args;
+    OnDeviceOf device((hipStream_t)stream);
+    if (device.err != hipSuccess) return HCCL_E_RUNTIME;
     switch (a->dtype) {
-        case DT_F16: return launch(stream, a, k_mx_reduce<DT_F16>);
-        case DT_BF16: return launch(stream, a, k_mx_reduce<DT_BF16>);
-        case DT_F32: return launch(stream, a, k_mx_reduce<DT_F32>);
+        case DT_F16: return reduce<DT_F16>((hipStream_t)stream, *a);
+        case DT_BF16: return reduce<DT_BF16>((hipStream_t)stream, *a);
+        case DT_F32: return reduce<DT_F32>((hipStream_t)stream, *a);
         default: return HCCL_E_PARA;
     }
 }

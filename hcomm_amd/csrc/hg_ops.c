@@ -107,19 +107,31 @@ static int mx_view(HgMxView* v, Range* packed, Range* scales, const HcommGfxMxVi
            range_of(scales, in->scales, rows, blocks, in->scaleStride);
 }
 
+/* Launches of fewer workgroups than this (of HG_MX_UNROLL groups a lane) are spread over four times as many */
+#define HG_MX_FEW_WGS 1024u
+
 static int mx_grid(HgMxGrid* g, uint64_t rows, uint64_t cols)
 {
+    const uint32_t most = HG_MX_UNROLL * 256u;
     if (cols > HG_MX_MAX_COLS) return HCCL_E_NOT_SUPPORT;
     const uint64_t groups = mx_blocks(cols) * 4u;
     g->rows = rows;
     g->cols = cols;
     g->groups = (uint32_t)groups;
-    g->tiles = (uint32_t)((groups + HG_MX_TILE - 1u) / HG_MX_TILE);
-    g->rows_per_wg = groups < HG_MX_TILE ? HG_MX_TILE / (uint32_t)groups : 1u;
+    g->rows_per_wg = groups < most && rows > 1 ? most / (uint32_t)groups : 1u;
+    g->tile = most;
+    if (g->rows_per_wg == 1u && (groups + most - 1u) / most <= HG_MX_FEW_WGS / (rows < HG_MX_FEW_WGS ? rows : HG_MX_FEW_WGS)) g->tile = 256u;
+    g->tiles = g->rows_per_wg > 1u ? 1u : (uint32_t)((groups + g->tile - 1u) / g->tile);
     const uint64_t wgs = g->rows_per_wg > 1u ? rows / g->rows_per_wg + (rows % g->rows_per_wg != 0) : rows;
     if (wgs > HG_LIMIT_WGS / g->tiles) return HCCL_E_NOT_SUPPORT;
     g->wgs = (uint32_t)wgs * g->tiles;
     return HCCL_SUCCESS;
+}
+
+/* whether the rows follow one another without a gap, in whole blocks: then the matrix is one long row */
+static int mx_is_run(const HgMxView* v, uint64_t cols)
+{
+    return cols % HCOMM_GFX_MX_BLOCK == 0 && v->scale_stride == cols / HCOMM_GFX_MX_BLOCK && v->packed_stride == cols / 2u;
 }
 
 int32_t HcommGfxMxQuantizeOnThread(
@@ -138,7 +150,9 @@ int32_t HcommGfxMxQuantizeOnThread(
         Range r[3];
         if (!dense_range(&r[0], src, rows, cols, srcStride, es) || !mx_view(&a.out, &r[1], &r[2], out, rows, cols)) return HCCL_E_PARA;
         if (!clear_of(&r[1], r, 3, NULL) || !clear_of(&r[2], r, 3, NULL)) return HCCL_E_PARA;
-        if (rows && cols) rc = mx_grid(&a.grid, rows, cols);
+        uint64_t all;
+        const int run = rows > 1 && srcStride == cols && mx_is_run(&a.out, cols) && !__builtin_mul_overflow(rows, cols, &all) && all <= HG_MX_MAX_COLS;
+        if (rows && cols) rc = run ? mx_grid(&a.grid, 1, all) : mx_grid(&a.grid, rows, cols);
     }
     if (rc == HCCL_SUCCESS) rc = ready(t);
     if (rc != HCCL_SUCCESS || rows == 0 || cols == 0) return rc;
@@ -177,7 +191,11 @@ int32_t HcommGfxMxReduceKOnThread(
             if (!mx_view(&a.src[j], &r[4 + 2 * j], &r[5 + 2 * j], &srcs[j], rows, cols)) return HCCL_E_PARA;
         if (!clear_of(&r[0], r, 4 + 2 * k, &r[1]) || !clear_of(&r[2], r, 4 + 2 * k, NULL) || !clear_of(&r[3], r, 4 + 2 * k, NULL))
             return HCCL_E_PARA;
-        if (rows && cols) rc = mx_grid(&a.grid, rows, cols);
+        uint64_t all;
+        int run = rows > 1 && (!dst || dstStride == cols) && (!addend || addendStride == cols) && (!again || mx_is_run(&a.again, cols)) &&
+                  !__builtin_mul_overflow(rows, cols, &all) && all <= HG_MX_MAX_COLS;
+        for (uint32_t j = 0; j < k && run; ++j) run = mx_is_run(&a.src[j], cols);
+        if (rows && cols) rc = run ? mx_grid(&a.grid, 1, all) : mx_grid(&a.grid, rows, cols);
     }
     if (rc == HCCL_SUCCESS) rc = ready(t);
     if (rc != HCCL_SUCCESS || rows == 0 || cols == 0) return rc;
