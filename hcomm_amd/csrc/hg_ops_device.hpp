@@ -18,8 +18,9 @@ typedef u32x4 __attribute__((aligned(4))) u32x4_at4;
 template <int DT> struct GroupVec { typedef u32x4_at2 type; };
 template <> struct GroupVec<DT_F32> { typedef u32x4_at4 type; };
 
-// elements [at, at + 8) of a row that holds `cols`; those past its end are 0
-template <int DT> __device__ __forceinline__ Raw8<DT> load8(const void* row, uint64_t at, uint64_t cols)
+// elements [at, at + 8) of a row that holds `cols`; those past its end are 0.  NT: a cache hint for what is read (written)
+// once and by no launch that follows soon.
+template <int DT, bool NT = false> __device__ __forceinline__ Raw8<DT> load8(const void* row, uint64_t at, uint64_t cols)
 {
     constexpr uint32_t ES = ElemSize<DT>::v;
     typedef const __attribute__((address_space(1))) typename GroupVec<DT>::type cv;
@@ -28,7 +29,7 @@ template <int DT> __device__ __forceinline__ Raw8<DT> load8(const void* row, uin
     if (at + 8u <= cols) {
 #pragma unroll
         for (uint32_t i = 0; i < Raw8<DT>::words / 4u; ++i) {
-            const u32x4 v = ((cv*)p)[i];
+            const u32x4 v = NT ? __builtin_nontemporal_load((cv*)p + i) : ((cv*)p)[i];
             r.w[4 * i] = v.x, r.w[4 * i + 1] = v.y, r.w[4 * i + 2] = v.z, r.w[4 * i + 3] = v.w;
         }
     } else {
@@ -77,15 +78,18 @@ template <int DT> __device__ __forceinline__ Raw8<DT> narrow8(const float (&f)[8
     return r;
 }
 
-template <int DT> __device__ __forceinline__ void store8(void* row, uint64_t at, uint64_t cols, const Raw8<DT>& r)
+template <int DT, bool NT = false> __device__ __forceinline__ void store8(void* row, uint64_t at, uint64_t cols, const Raw8<DT>& r)
 {
     constexpr uint32_t ES = ElemSize<DT>::v;
     typedef __attribute__((address_space(1))) typename GroupVec<DT>::type wv;
     uint8_t* p = (uint8_t*)row + at * ES;
     if (at + 8u <= cols) {
 #pragma unroll
-        for (uint32_t i = 0; i < Raw8<DT>::words / 4u; ++i)
-            ((wv*)p)[i] = u32x4{r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]};
+        for (uint32_t i = 0; i < Raw8<DT>::words / 4u; ++i) {
+            const typename GroupVec<DT>::type v = u32x4{r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]};
+            if (NT) __builtin_nontemporal_store(v, (wv*)p + i);
+            else ((wv*)p)[i] = v;
+        }
     } else if (at < cols) {
         const uint32_t n = (uint32_t)(cols - at);
 #pragma unroll
