@@ -45,12 +45,12 @@ template <bool ONE, uint32_t U> __device__ __forceinline__ Place<ONE> place_of(c
 template <int DT, bool NT, bool ONE> __device__ __forceinline__ Raw8<DT> load_at(const void* m, uint64_t stride, const Place<ONE>& p, uint64_t cols)
 {
     const uint64_t at = (uint64_t)p.tile * 8u;
-    return load8<DT, NT>((const uint8_t*)m + (p.row * stride + at) * ElemSize<DT>::v, p.group * 8u, p.there ? cols - at : 0u);
+    return load8<DT, true, NT>((const uint8_t*)m + (p.row * stride + at) * ElemSize<DT>::v, p.group * 8u, p.there ? cols - at : 0u);
 }
 template <int DT, bool ONE> __device__ __forceinline__ void store_at(void* m, uint64_t stride, const Place<ONE>& p, uint64_t cols, const Raw8<DT>& v)
 {
     const uint64_t at = (uint64_t)p.tile * 8u;
-    store8<DT, true>((uint8_t*)m + (p.row * stride + at) * ElemSize<DT>::v, p.group * 8u, p.there ? cols - at : 0u, v);
+    store8<DT, true, true>((uint8_t*)m + (p.row * stride + at) * ElemSize<DT>::v, p.group * 8u, p.there ? cols - at : 0u, v);
 }
 
 // the largest of a value over the four lanes of a block
@@ -272,8 +272,7 @@ template <int DT, uint32_t N, bool JOIN> int reduce_n(hipStream_t st, const HgMx
     f.again = a.again;
     f.dst = a.dst, f.addend = a.addend, f.dst_stride = a.dst_stride, f.addend_stride = a.addend_stride, f.k = a.k;
     if (a.grid.rows_per_wg > 1u) return launch(st, a.grid.wgs, k_mx_reduce<DT, false, HG_MX_UNROLL, N, JOIN>, f);
-    if (a.grid.tile == 256u) return launch(st, a.grid.wgs, k_mx_reduce<DT, true, 1, N, JOIN>, f);
-    return launch(st, a.grid.wgs, k_mx_reduce<DT, true, HG_MX_UNROLL, N, JOIN>, f);
+    return launch(st, a.grid.wgs, k_mx_reduce<DT, true, 1, N, JOIN>, f);
 }
 
 template <int DT> int reduce(hipStream_t st, const HgMxReduce& a)

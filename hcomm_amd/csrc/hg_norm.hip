@@ -15,37 +15,40 @@ template <int CTRL> __device__ __forceinline__ float plus_dpp(float v)
     return v + bits_f32((uint32_t)__builtin_amdgcn_mov_dpp((int)f32_bits(v), CTRL, 0xf, 0xf, true));
 }
 
-// the sum over the wavefront, in every lane: inside the rows of 16 lanes by lane exchanges, across them by scalar reads
+// the sum over 16 neighbouring lanes, in all of them
+__device__ __forceinline__ float sum16(float v)
+{
+    v = plus_dpp<0xB1>(v);     // 1 0 3 2
+    v = plus_dpp<0x4E>(v);     // 2 3 0 1
+    v = plus_dpp<0x141>(v);    // mirrored in 8
+    return plus_dpp<0x140>(v); // mirrored in 16
+}
+
+// the sum over the wavefront, in every lane: across its rows of 16 lanes by scalar reads
 __device__ __forceinline__ float wave_sum(float v)
 {
-    v = plus_dpp<0xB1>(v);  // 1 0 3 2
-    v = plus_dpp<0x4E>(v);  // 2 3 0 1
-    v = plus_dpp<0x141>(v); // mirrored in 8
-    v = plus_dpp<0x140>(v); // mirrored in 16
-    const float a = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), 0)), b = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), 16));
-    const float c = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), 32)), d = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), 48));
+    const int s = (int)f32_bits(sum16(v));
+    const float a = bits_f32((uint32_t)__builtin_amdgcn_readlane(s, 0)), b = bits_f32((uint32_t)__builtin_amdgcn_readlane(s, 16));
+    const float c = bits_f32((uint32_t)__builtin_amdgcn_readlane(s, 32)), d = bits_f32((uint32_t)__builtin_amdgcn_readlane(s, 48));
     return (a + b) + (c + d);
 }
 
-// N sums over the wavefronts of a row, the same in all of them.  `box` holds N floats for each wavefront of the workgroup
-// and is not written again before every wavefront has passed another barrier.
+// N sums over the at most 16 wavefronts of a row, the same in all of them: lane w of every 16 fetches wavefront w's.  `box`
+// holds N floats for each wavefront of the workgroup and is not written again before every wavefront has passed another
+// barrier.
 template <uint32_t N> __device__ __forceinline__ void row_sum(float (&v)[N], float* box, uint32_t waves)
 {
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
     if (waves == 1u) return;
-    const uint32_t wave = threadIdx.x >> 6, first = wave / waves * waves; // of this row
+    const uint32_t wave = threadIdx.x >> 6, first = wave & ~(waves - 1u), w = threadIdx.x & 15u; // the host makes `waves` a power of two
     if ((threadIdx.x & 63u) == 0u) {
 #pragma unroll
         for (uint32_t i = 0; i < N; ++i) box[wave * N + i] = v[i];
     }
     __syncthreads();
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) v[i] = 0.0f;
-    for (uint32_t w = 0; w < waves; ++w) {
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i) v[i] += box[(first + w) * N + i];
-    }
+    for (uint32_t i = 0; i < N; ++i) v[i] = sum16(w < waves ? box[(first + w) * N + i] : 0.0f);
 }
 
 __device__ __forceinline__ float inverse_rms(float squares, uint64_t cols, float eps) { return 1.0f / sqrtf(squares / (float)cols + eps); }
@@ -54,25 +57,37 @@ __device__ __forceinline__ float inverse_rms(float squares, uint64_t cols, float
 
 // ---- forward --------------------------------------------------------------------------------------------------------
 
-// DT: type of the matrices, PT: of the parameters, V: groups of eight elements a lane holds
-template <int DT, int PT, uint32_t V> __global__ __launch_bounds__(1024) void k_norm(const HgNorm a)
+// The arguments as the kernel takes them: the runtime copies them at every launch, so few ranks mean few pointers.
+template <uint32_t N> struct NormArgs {
+    HcommGfxReduceNormDesc d;
+    const void* src[N];
+    uint32_t waves, rows_per_wg;
+};
+
+// DT: type of the matrices, PT: of the parameters, V: groups of eight elements a lane holds, ONE: a workgroup has one row
+// (then where it begins is a scalar), TAIL: rows end inside a group, NT: larger than the L2s, so that what is read once and
+// what is written passes by them (8,192 x 4,096 of eight ranks 153 -> 138 us; rows off 16-byte boundaries share lines, which
+// has to be fetched again then), N: most ranks
+template <int DT, int PT, uint32_t V, bool ONE, bool TAIL, bool NT, uint32_t N> __global__ __launch_bounds__(1024) void k_norm(const NormArgs<N> a)
 {
     __shared__ float box[2][MAX_WAVES];
-    constexpr uint32_t ES = ElemSize<DT>::v, PS = ElemSize<PT>::v, AHEAD = 4;
-    const uint32_t span = a.waves * 64u, local = threadIdx.x / span, t = threadIdx.x - local * span;
-    const uint64_t row = (uint64_t)blockIdx.x * a.rows_per_wg + local;
-    const uint64_t cols = row < a.d.rows ? a.d.cols : 0u; // a row that is not there has no columns
-    const uint32_t gate_row = a.d.gate && cols ? (uint32_t)row / (uint32_t)a.d.rowsPerGate : 0u; // the host keeps both below 2^31
+    constexpr uint32_t ES = ElemSize<DT>::v, PS = ElemSize<PT>::v, AHEAD = (DT == DT_F32 ? 4u : 8u) / V;
+    const uint32_t span = a.waves * 64u, local = ONE ? 0u : threadIdx.x / span, t = threadIdx.x - local * span;
+    const uint64_t row = ONE ? blockIdx.x : (uint64_t)blockIdx.x * a.rows_per_wg + local;
+    const uint64_t cols = ONE || row < a.d.rows ? a.d.cols : 0u; // a row that is not there has no columns
     float f[V][8];
-    for (uint32_t j0 = 0; j0 < a.d.k; j0 += AHEAD) {
-        Raw8<DT> x[AHEAD][V];
+    Raw8<DT> x[AHEAD][V], res[V];
+    Raw8<PT> post[V], pre[V], gate[V];
+    auto ask = [&](uint32_t j0) {
 #pragma unroll
         for (uint32_t j = 0; j < AHEAD; ++j)
             if (j0 + j < a.d.k) {
 #pragma unroll
                 for (uint32_t v = 0; v < V; ++v)
-                    x[j][v] = load8<DT>((const uint8_t*)a.src[j0 + j] + row * a.d.srcStride * ES, (v * span + t) * 8u, cols);
+                    x[j][v] = load8<DT, TAIL, NT>((const uint8_t*)a.src[j0 + j] + row * a.d.srcStride * ES, (v * span + t) * 8u, cols);
             }
+    };
+    auto add = [&](uint32_t j0) {
 #pragma unroll
         for (uint32_t j = 0; j < AHEAD; ++j)
             if (j0 + j < a.d.k) {
@@ -84,21 +99,27 @@ template <int DT, int PT, uint32_t V> __global__ __launch_bounds__(1024) void k_
                     for (uint32_t e = 0; e < 8u; ++e) f[v][e] = j0 + j == 0u ? g[e] : f[v][e] + g[e];
                 }
             }
-    }
-    Raw8<DT> res[V];
-    Raw8<PT> post[V], pre[V], gate[V];
+    };
+    ask(0);
+    // what the row's end needs is asked for before the ranks' sum is waited for
+    const uint32_t gate_row = a.d.gate && cols ? (uint32_t)row / (uint32_t)a.d.rowsPerGate : 0u; // the host keeps both below 2^31
 #pragma unroll
     for (uint32_t v = 0; v < V; ++v) {
         const uint32_t at = (v * span + t) * 8u;
-        if (a.d.residual) res[v] = load8<DT>((const uint8_t*)a.d.residual + row * a.d.residualStride * ES, at, cols);
-        if (a.d.postWeight) post[v] = load8<PT>(a.d.postWeight, at, cols);
-        if (a.d.preWeight) pre[v] = load8<PT>(a.d.preWeight, at, cols);
-        if (a.d.gate) gate[v] = load8<PT>((const uint8_t*)a.d.gate + (uint64_t)gate_row * a.d.gateStride * PS, at, cols);
+        if (a.d.residual) res[v] = load8<DT, TAIL, NT>((const uint8_t*)a.d.residual + row * a.d.residualStride * ES, at, cols);
+        if (a.d.postWeight) post[v] = load8<PT, TAIL>(a.d.postWeight, at, cols);
+        if (a.d.gate) gate[v] = load8<PT, TAIL>((const uint8_t*)a.d.gate + (uint64_t)gate_row * a.d.gateStride * PS, at, cols);
+        if (a.d.preWeight) pre[v] = load8<PT, TAIL>(a.d.preWeight, at, cols);
+    }
+    add(0);
+    for (uint32_t j0 = AHEAD; j0 < a.d.k; j0 += AHEAD) {
+        ask(j0);
+        add(j0);
     }
     if (a.d.sum) {
 #pragma unroll
         for (uint32_t v = 0; v < V; ++v)
-            store8<DT>((uint8_t*)a.d.sum + row * a.d.sumStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(f[v]));
+            store8<DT, TAIL, NT>((uint8_t*)a.d.sum + row * a.d.sumStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(f[v]));
     }
     if (a.d.postWeight) {
         float s[1] = {0.0f};
@@ -126,14 +147,14 @@ template <int DT, int PT, uint32_t V> __global__ __launch_bounds__(1024) void k_
             for (uint32_t e = 0; e < 8u; ++e) f[v][e] *= w[e];
         }
         if (a.d.residual) {
-            float x[8];
-            widen8<DT>(res[v], x);
+            float y[8];
+            widen8<DT>(res[v], y);
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e) f[v][e] = fmaf(a.d.residualScale, x[e], f[v][e]);
+            for (uint32_t e = 0; e < 8u; ++e) f[v][e] = fmaf(a.d.residualScale, y[e], f[v][e]);
         }
 #pragma unroll
         for (uint32_t e = 0; e < 8u; ++e) s[0] = fmaf(f[v][e], f[v][e], s[0]);
-        store8<DT>((uint8_t*)a.d.y + row * a.d.yStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(f[v]));
+        store8<DT, TAIL, NT>((uint8_t*)a.d.y + row * a.d.yStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(f[v]));
     }
     if (a.d.preWeight) {
         row_sum(s, box[1], a.waves);
@@ -144,72 +165,80 @@ template <int DT, int PT, uint32_t V> __global__ __launch_bounds__(1024) void k_
             widen8<PT>(pre[v], w);
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e) f[v][e] = f[v][e] * r * w[e];
-            store8<DT>((uint8_t*)a.d.z + row * a.d.zStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(f[v]));
+            store8<DT, TAIL, NT>((uint8_t*)a.d.z + row * a.d.zStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(f[v]));
         }
     }
 }
 
 // ---- gradient ---------------------------------------------------------------------------------------------------------
 
-template <int DT, int PT, uint32_t V, uint32_t MOST> __global__ __launch_bounds__(MOST) void k_norm_grad(const HgNormGrad a)
+// A run of rows to a workgroup: the parameters' gradients stay in registers over the run, and the row after the one at work
+// is on its way while the sums of this one cross the lanes.
+template <int DT, int PT, uint32_t V, uint32_t MOST, bool TAIL, bool NT> __global__ __launch_bounds__(MOST) void k_norm_grad(const HgNormGrad a)
 {
     __shared__ float box_a[MAX_WAVES * 3], box_b[MAX_WAVES];
     constexpr uint32_t ES = ElemSize<DT>::v, PS = ElemSize<PT>::v;
     const uint32_t span = a.waves * 64u, t = threadIdx.x;
     const uint64_t cols = a.d.cols;
     const bool has_post = a.d.postWeight != nullptr, has_pre = a.d.preWeight != nullptr, has_gate = a.d.gate != nullptr;
-    uint64_t row, end;
+    uint32_t row, end; // the host keeps rows below 2^31
     if (a.by_gate) {
-        const uint32_t per = (uint32_t)a.chunks_per_gate;
-        const uint64_t g = blockIdx.x / per, part = blockIdx.x % per;
-        const uint64_t g_end = min((g + 1u) * a.d.rowsPerGate, a.d.rows);
-        row = g * a.d.rowsPerGate + part * a.chunk_rows;
-        end = min(row + a.chunk_rows, g_end);
+        const uint32_t per = (uint32_t)a.chunks_per_gate, g = blockIdx.x / per, part = blockIdx.x - g * per;
+        const uint32_t begin = g * (uint32_t)a.d.rowsPerGate, stop = min(begin + (uint32_t)a.d.rowsPerGate, (uint32_t)a.d.rows);
+        row = min(begin + part * (uint32_t)a.chunk_rows, stop);
+        end = min(row + (uint32_t)a.chunk_rows, stop);
     } else {
-        row = (uint64_t)blockIdx.x * a.chunk_rows;
-        end = min(row + a.chunk_rows, a.d.rows);
+        row = blockIdx.x * (uint32_t)a.chunk_rows;
+        end = min(row + (uint32_t)a.chunk_rows, (uint32_t)a.d.rows);
     }
+    struct Row {
+        Raw8<DT> s[V], y[V], dy[V], dz[V];
+    };
+    auto ask = [&](Row& x, uint32_t r) {
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v) {
+            const uint32_t at = (v * span + t) * 8u;
+            x.s[v] = load8<DT, TAIL, NT>((const uint8_t*)a.d.sum + r * a.d.sumStride * ES, at, cols);
+            if (has_pre) {
+                x.y[v] = load8<DT, TAIL, NT>((const uint8_t*)a.d.y + r * a.d.yStride * ES, at, cols);
+                x.dz[v] = load8<DT, TAIL, NT>((const uint8_t*)a.d.dz + r * a.d.dzStride * ES, at, cols);
+            }
+            x.dy[v] = load8<DT, TAIL, NT>((const uint8_t*)a.d.dy + r * a.d.dyStride * ES, at, cols);
+        }
+    };
+    Row next;
+    if (row < end) ask(next, row);
     Raw8<PT> post[V], pre[V], gate[V];
     float d_post[V][8], d_pre[V][8], d_gate[V][8];
 #pragma unroll
     for (uint32_t v = 0; v < V; ++v) {
-        if (has_post) post[v] = load8<PT>(a.d.postWeight, (v * span + t) * 8u, cols);
-        if (has_pre) pre[v] = load8<PT>(a.d.preWeight, (v * span + t) * 8u, cols);
+        if (has_pre) pre[v] = load8<PT, TAIL>(a.d.preWeight, (v * span + t) * 8u, cols);
+        if (has_post) post[v] = load8<PT, TAIL>(a.d.postWeight, (v * span + t) * 8u, cols);
 #pragma unroll
         for (uint32_t e = 0; e < 8u; ++e) d_post[v][e] = d_pre[v][e] = d_gate[v][e] = 0.0f;
     }
     const float each = 1.0f / (float)cols;
-    uint64_t gate_row = has_gate && row < end ? (uint32_t)row / (uint32_t)a.d.rowsPerGate : 0u, gate_end = 0u; // row at which the next gate row begins
-    if (has_gate) {
-        gate_end = (gate_row + 1u) * a.d.rowsPerGate;
-        if (row < end) {
+    uint32_t gate_row = 0u, gate_end = 0u; // the row of the gate, and the row at which its next one begins
+    if (has_gate && row < end) {
+        gate_row = row / (uint32_t)a.d.rowsPerGate;
+        gate_end = (gate_row + 1u) * (uint32_t)a.d.rowsPerGate;
 #pragma unroll
-            for (uint32_t v = 0; v < V; ++v) gate[v] = load8<PT>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols);
-        }
+        for (uint32_t v = 0; v < V; ++v) gate[v] = load8<PT, TAIL>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols);
     }
     for (; row < end; ++row) {
-        Raw8<DT> xs[V], xy[V], xd[V], xz[V];
-#pragma unroll
-        for (uint32_t v = 0; v < V; ++v) {
-            const uint32_t at = (v * span + t) * 8u;
-            xs[v] = load8<DT>((const uint8_t*)a.d.sum + row * a.d.sumStride * ES, at, cols);
-            xd[v] = load8<DT>((const uint8_t*)a.d.dy + row * a.d.dyStride * ES, at, cols);
-            if (has_pre) {
-                xy[v] = load8<DT>((const uint8_t*)a.d.y + row * a.d.yStride * ES, at, cols);
-                xz[v] = load8<DT>((const uint8_t*)a.d.dz + row * a.d.dzStride * ES, at, cols);
-            }
-        }
+        const Row x = next;
+        if (row + 1u < end) ask(next, row + 1u);
         float q[3] = {0.0f, 0.0f, 0.0f}; // sum^2, y^2, dz preWeight y
 #pragma unroll
         for (uint32_t v = 0; v < V; ++v) {
             float s[8];
-            widen8<DT>(xs[v], s);
+            widen8<DT>(x.s[v], s);
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e) q[0] = fmaf(s[e], s[e], q[0]);
             if (has_pre) {
                 float y[8], z[8], w[8];
-                widen8<DT>(xy[v], y);
-                widen8<DT>(xz[v], z);
+                widen8<DT>(x.y[v], y);
+                widen8<DT>(x.dz[v], z);
                 widen8<PT>(pre[v], w);
 #pragma unroll
                 for (uint32_t e = 0; e < 8u; ++e) q[1] = fmaf(y[e], y[e], q[1]), q[2] = fmaf(z[e] * w[e], y[e], q[2]);
@@ -223,12 +252,12 @@ template <int DT, int PT, uint32_t V, uint32_t MOST> __global__ __launch_bounds_
 #pragma unroll
         for (uint32_t v = 0; v < V; ++v) {
             float s[8], d[8];
-            widen8<DT>(xs[v], s);
-            widen8<DT>(xd[v], d);
+            widen8<DT>(x.s[v], s);
+            widen8<DT>(x.dy[v], d);
             if (has_pre) {
                 float y[8], z[8], w[8];
-                widen8<DT>(xy[v], y);
-                widen8<DT>(xz[v], z);
+                widen8<DT>(x.y[v], y);
+                widen8<DT>(x.dz[v], z);
                 widen8<PT>(pre[v], w);
 #pragma unroll
                 for (uint32_t e = 0; e < 8u; ++e) {
@@ -238,10 +267,10 @@ template <int DT, int PT, uint32_t V, uint32_t MOST> __global__ __launch_bounds_
                 }
             }
             if (a.d.dResidual) {
-                float x[8];
+                float o[8];
 #pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e) x[e] = a.d.residualScale * d[e];
-                store8<DT>((uint8_t*)a.d.dResidual + row * a.d.dResidualStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(x));
+                for (uint32_t e = 0; e < 8u; ++e) o[e] = a.d.residualScale * d[e];
+                store8<DT, TAIL, NT>((uint8_t*)a.d.dResidual + row * a.d.dResidualStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(o));
             }
             float w1[8], g[8];
             if (has_post) widen8<PT>(post[v], w1);
@@ -267,7 +296,7 @@ template <int DT, int PT, uint32_t V, uint32_t MOST> __global__ __launch_bounds_
 #pragma unroll
             for (uint32_t v = 0; v < V; ++v) {
                 float s[8];
-                widen8<DT>(xs[v], s);
+                widen8<DT>(x.s[v], s);
 #pragma unroll
                 for (uint32_t e = 0; e < 8u; ++e) g1[v][e] = r1 * fmaf(-c1, s[e] * r1, g1[v][e]);
             }
@@ -276,16 +305,16 @@ template <int DT, int PT, uint32_t V, uint32_t MOST> __global__ __launch_bounds_
         }
 #pragma unroll
         for (uint32_t v = 0; v < V; ++v)
-            store8<DT>((uint8_t*)a.d.dSum + row * a.d.dSumStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(g1[v]));
+            store8<DT, TAIL, NT>((uint8_t*)a.d.dSum + row * a.d.dSumStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(g1[v]));
         if (has_gate && !a.by_gate && (row + 1u == gate_end || row + 1u == end)) { // whole gate rows in one run: theirs are done
-            const uint64_t g = gate_row++;
-            gate_end += a.d.rowsPerGate;
+            const uint32_t g = gate_row++;
+            gate_end += (uint32_t)a.d.rowsPerGate;
 #pragma unroll
             for (uint32_t v = 0; v < V; ++v) {
-                if (a.d.dGate) store8<PT>((uint8_t*)a.d.dGate + g * a.d.dGateStride * PS, (v * span + t) * 8u, cols, narrow8<PT>(d_gate[v]));
+                if (a.d.dGate) store8<PT, TAIL>((uint8_t*)a.d.dGate + g * a.d.dGateStride * PS, (v * span + t) * 8u, cols, narrow8<PT>(d_gate[v]));
 #pragma unroll
                 for (uint32_t e = 0; e < 8u; ++e) d_gate[v][e] = 0.0f;
-                if (row + 1u < end) gate[v] = load8<PT>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols);
+                if (row + 1u < end) gate[v] = load8<PT, TAIL>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols);
             }
         }
     }
@@ -293,9 +322,9 @@ template <int DT, int PT, uint32_t V, uint32_t MOST> __global__ __launch_bounds_
 #pragma unroll
     for (uint32_t v = 0; v < V; ++v) {
         const uint32_t at = (v * span + t) * 8u;
-        if (a.at_post >= 0) store8<DT_F32>(mine + (uint64_t)a.at_post * cols, at, cols, narrow8<DT_F32>(d_post[v]));
-        if (a.at_pre >= 0) store8<DT_F32>(mine + (uint64_t)a.at_pre * cols, at, cols, narrow8<DT_F32>(d_pre[v]));
-        if (a.at_gate >= 0) store8<DT_F32>(mine + (uint64_t)a.at_gate * cols, at, cols, narrow8<DT_F32>(d_gate[v]));
+        if (a.at_post >= 0) store8<DT_F32, TAIL>(mine + (uint64_t)a.at_post * cols, at, cols, narrow8<DT_F32>(d_post[v]));
+        if (a.at_pre >= 0) store8<DT_F32, TAIL>(mine + (uint64_t)a.at_pre * cols, at, cols, narrow8<DT_F32>(d_pre[v]));
+        if (a.at_gate >= 0) store8<DT_F32, TAIL>(mine + (uint64_t)a.at_gate * cols, at, cols, narrow8<DT_F32>(d_gate[v]));
     }
 }
 
@@ -337,25 +366,46 @@ template <int PT> __global__ __launch_bounds__(1024) void k_norm_sums(const HgNo
     }
 }
 
+template <int DT, int PT, uint32_t V, bool ONE, bool TAIL, bool NT, uint32_t N> int launch_norm_n(hipStream_t st, const HgNorm* a)
+{
+    NormArgs<N> n;
+    n.d = a->d, n.waves = a->waves, n.rows_per_wg = a->rows_per_wg;
+    for (uint32_t j = 0; j < N; ++j) n.src[j] = a->src[j];
+    hipLaunchKernelGGL((k_norm<DT, PT, V, ONE, TAIL, NT, N>), dim3(a->wgs), dim3(a->waves * 64u * a->rows_per_wg), 0, st, n);
+    return rc(hipGetLastError());
+}
+
+template <int DT, int PT, uint32_t V, bool ONE> int launch_norm_v(hipStream_t st, const HgNorm* a)
+{
+    if (a->d.cols % 8u)
+        return a->d.k <= 8u ? launch_norm_n<DT, PT, V, ONE, true, false, 8>(st, a) : launch_norm_n<DT, PT, V, ONE, true, false, HCOMM_GFX_MAX_RANKS>(st, a);
+    if (a->d.k > 8u) return launch_norm_n<DT, PT, V, ONE, false, true, HCOMM_GFX_MAX_RANKS>(st, a);
+    return a->stream ? launch_norm_n<DT, PT, V, ONE, false, true, 8>(st, a) : launch_norm_n<DT, PT, V, ONE, false, false, 8>(st, a);
+}
+
 template <int DT, int PT> int launch_norm(hipStream_t st, const HgNorm* a)
 {
-    const dim3 g(a->wgs), b(a->waves * 64u * a->rows_per_wg);
-    if (a->vecs == 1u) hipLaunchKernelGGL((k_norm<DT, PT, 1>), g, b, 0, st, *a);
-    else hipLaunchKernelGGL((k_norm<DT, PT, 2>), g, b, 0, st, *a);
+    if (a->vecs == 2u) return launch_norm_v<DT, PT, 2, true>(st, a);
+    return a->rows_per_wg == 1u ? launch_norm_v<DT, PT, 1, true>(st, a) : launch_norm_v<DT, PT, 1, false>(st, a);
+}
+
+template <int DT, int PT, bool TAIL, bool NT> int launch_norm_grad_t(hipStream_t st, const HgNormGrad* a)
+{
+    const dim3 g((uint32_t)a->chunks), b(a->waves * 64u);
+    if (a->vecs == 1u) {
+        if (a->waves <= 4u) hipLaunchKernelGGL((k_norm_grad<DT, PT, 1, 256, TAIL, NT>), g, b, 0, st, *a);
+        else hipLaunchKernelGGL((k_norm_grad<DT, PT, 1, 512, TAIL, NT>), g, b, 0, st, *a);
+    } else {
+        if (a->waves <= 8u) hipLaunchKernelGGL((k_norm_grad<DT, PT, 2, 512, TAIL, NT>), g, b, 0, st, *a);
+        else hipLaunchKernelGGL((k_norm_grad<DT, PT, 2, 1024, TAIL, NT>), g, b, 0, st, *a);
+    }
     return rc(hipGetLastError());
 }
 
 template <int DT, int PT> int launch_norm_grad(hipStream_t st, const HgNormGrad* a)
 {
-    const dim3 g((uint32_t)a->chunks), b(a->waves * 64u);
-    if (a->vecs == 1u) {
-        if (a->waves <= 4u) hipLaunchKernelGGL((k_norm_grad<DT, PT, 1, 256>), g, b, 0, st, *a);
-        else hipLaunchKernelGGL((k_norm_grad<DT, PT, 1, 1024>), g, b, 0, st, *a);
-    } else {
-        if (a->waves <= 4u) hipLaunchKernelGGL((k_norm_grad<DT, PT, 2, 256>), g, b, 0, st, *a);
-        else hipLaunchKernelGGL((k_norm_grad<DT, PT, 2, 1024>), g, b, 0, st, *a);
-    }
-    return rc(hipGetLastError());
+    if (a->d.cols % 8u) return launch_norm_grad_t<DT, PT, true, false>(st, a);
+    return a->stream ? launch_norm_grad_t<DT, PT, false, true>(st, a) : launch_norm_grad_t<DT, PT, false, false>(st, a);
 }
 
 } // namespace

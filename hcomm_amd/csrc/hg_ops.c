@@ -107,10 +107,15 @@ static int mx_view(HgMxView* v, Range* packed, Range* scales, const HcommGfxMxVi
            range_of(scales, in->scales, rows, blocks, in->scaleStride);
 }
 
-/* Launches of fewer workgroups than this (of HG_MX_UNROLL groups a lane) are spread over four times as many */
+/*
+ * A piece of a long row is one group a lane where that fills the GPU better: in every fold (dequantising 67.1M elements
+ * 26.3 -> 24.9 us, 14.3M results of seven ranks 22.9 -> 22.3, 8.4M 20.3 -> 18.8) and in launches of up to `few` workgroups of
+ * HG_MX_UNROLL groups a lane.  Large quantisations keep several groups in flight (67.1M elements 28.8 us; one group: 32.8).
+ */
 #define HG_MX_FEW_WGS 1024u
+#define HG_MX_ALWAYS 0xffffffffu
 
-static int mx_grid(HgMxGrid* g, uint64_t rows, uint64_t cols)
+static int mx_grid(HgMxGrid* g, uint64_t rows, uint64_t cols, uint32_t few)
 {
     const uint32_t most = HG_MX_UNROLL * 256u;
     if (cols > HG_MX_MAX_COLS) return HCCL_E_NOT_SUPPORT;
@@ -120,7 +125,7 @@ static int mx_grid(HgMxGrid* g, uint64_t rows, uint64_t cols)
     g->groups = (uint32_t)groups;
     g->rows_per_wg = groups < most && rows > 1 ? most / (uint32_t)groups : 1u;
     g->tile = most;
-    if (g->rows_per_wg == 1u && (groups + most - 1u) / most <= HG_MX_FEW_WGS / (rows < HG_MX_FEW_WGS ? rows : HG_MX_FEW_WGS)) g->tile = 256u;
+    if (g->rows_per_wg == 1u && (few == HG_MX_ALWAYS || (rows <= few && (groups + most - 1u) / most <= few / rows))) g->tile = 256u;
     g->tiles = g->rows_per_wg > 1u ? 1u : (uint32_t)((groups + g->tile - 1u) / g->tile);
     const uint64_t wgs = g->rows_per_wg > 1u ? rows / g->rows_per_wg + (rows % g->rows_per_wg != 0) : rows;
     if (wgs > HG_LIMIT_WGS / g->tiles) return HCCL_E_NOT_SUPPORT;
@@ -152,7 +157,7 @@ int32_t HcommGfxMxQuantizeOnThread(
         if (!clear_of(&r[1], r, 3, NULL) || !clear_of(&r[2], r, 3, NULL)) return HCCL_E_PARA;
         uint64_t all;
         const int run = rows > 1 && srcStride == cols && mx_is_run(&a.out, cols) && !__builtin_mul_overflow(rows, cols, &all) && all <= HG_MX_MAX_COLS;
-        if (rows && cols) rc = run ? mx_grid(&a.grid, 1, all) : mx_grid(&a.grid, rows, cols);
+        if (rows && cols) rc = run ? mx_grid(&a.grid, 1, all, HG_MX_FEW_WGS) : mx_grid(&a.grid, rows, cols, HG_MX_FEW_WGS);
     }
     if (rc == HCCL_SUCCESS) rc = ready(t);
     if (rc != HCCL_SUCCESS || rows == 0 || cols == 0) return rc;
@@ -195,7 +200,7 @@ int32_t HcommGfxMxReduceKOnThread(
         int run = rows > 1 && (!dst || dstStride == cols) && (!addend || addendStride == cols) && (!again || mx_is_run(&a.again, cols)) &&
                   !__builtin_mul_overflow(rows, cols, &all) && all <= HG_MX_MAX_COLS;
         for (uint32_t j = 0; j < k && run; ++j) run = mx_is_run(&a.src[j], cols);
-        if (rows && cols) rc = run ? mx_grid(&a.grid, 1, all) : mx_grid(&a.grid, rows, cols);
+        if (rows && cols) rc = run ? mx_grid(&a.grid, 1, all, HG_MX_ALWAYS) : mx_grid(&a.grid, rows, cols, HG_MX_ALWAYS);
     }
     if (rc == HCCL_SUCCESS) rc = ready(t);
     if (rc != HCCL_SUCCESS || rows == 0 || cols == 0) return rc;
@@ -269,16 +274,21 @@ int32_t HcommGfxMxProductKOnThread(
 
 /* ---- norms behind a fold ------------------------------------------------------------------------------------------------ */
 
-/* wavefronts to a row and groups of eight elements to a lane */
-static void row_shape(uint64_t cols, uint32_t* waves, uint32_t* vecs)
+/* wavefronts to a row and groups of eight elements to a lane: a second group where `most` wavefronts do not reach */
+static void row_shape(uint64_t cols, uint32_t most, uint32_t* waves, uint32_t* vecs)
 {
     const uint64_t per_wave = 64u * 8u;
     uint32_t w = 1, v = 1;
-    if (cols > per_wave * 16u) v = 2;
-    while (w < 16u && per_wave * v * w < cols) w *= 2u;
+    while (w < most && per_wave * w < cols) w *= 2u;
+    if (per_wave * w < cols) {
+        v = 2;
+        while (per_wave * v * w < cols) w *= 2u;
+    }
     *waves = w;
     *vecs = v;
 }
+
+#define HG_L2_BYTES (32ull << 20) /* of the eight XCDs together */
 
 static int norm_types(HcommDataType data, HcommDataType param)
 {
@@ -327,10 +337,11 @@ int32_t HcommGfxReduceNormOnThread(ThreadHandle thread, const HcommGfxReduceNorm
     for (uint32_t j = 0; j < desc->k; ++j) a.src[j] = desc->srcs[j];
     a.d.srcs = NULL;
     if (!a.d.gate || a.d.rowsPerGate > rows) a.d.rowsPerGate = rows;
-    row_shape(cols, &a.waves, &a.vecs);
+    row_shape(cols, 16, &a.waves, &a.vecs);
     a.rows_per_wg = a.waves < 4u ? 4u / a.waves : 1u;
     a.wgs = (uint32_t)((rows + a.rows_per_wg - 1u) / a.rows_per_wg);
     const uint64_t bytes = rows * cols * es * (1u + (desc->sum != NULL) + (desc->z != NULL));
+    a.stream = bytes + rows * cols * es * desc->k > HG_L2_BYTES;
     const HcommGfxLaunchRecord rec = record(HCOMM_GFX_KERNEL_NORM, (int)desc->dataType, HCOMM_REDUCE_SUM, desc->k, bytes, a.wgs, a.waves * 64u);
     return hg_submit_other(t, &rec, hg_launch_norm, &a);
 }
@@ -343,7 +354,7 @@ static void norm_grad_shape(HgNormGrad* a)
 {
     HcommGfxReduceNormGradDesc* d = &a->d;
     const uint64_t rows = d->rows;
-    row_shape(d->cols, &a->waves, &a->vecs);
+    row_shape(d->cols, 8, &a->waves, &a->vecs);
     const uint64_t most = HG_NORM_GRAD_WAVES / a->waves;
     if (!d->gate || d->rowsPerGate > rows) d->rowsPerGate = rows ? rows : 1u;
     a->gates = d->gate ? gate_rows(rows, d->rowsPerGate) : 0u;
@@ -428,6 +439,7 @@ int32_t HcommGfxReduceNormGradOnThread(ThreadHandle thread, const HcommGfxReduce
     }
     if (rc == HCCL_SUCCESS) rc = ready(t);
     if (rc != HCCL_SUCCESS || cols == 0) return rc;
+    a.stream = rows * cols * es * 4u > HG_L2_BYTES; /* sum, dy and what is written, at least */
     if (a.chunks) {
         const HcommGfxLaunchRecord rec = record(
             HCOMM_GFX_KERNEL_NORM_GRAD, (int)desc->dataType, 255, 1, rows * cols * es * (1u + (desc->dResidual != NULL)), a.chunks, a.waves * 64u);

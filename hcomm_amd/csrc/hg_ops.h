@@ -80,6 +80,7 @@ typedef struct {
     uint32_t vecs;        /* groups of eight elements a lane holds */
     uint32_t rows_per_wg;
     uint32_t wgs;
+    uint32_t stream;      /* moves more than the L2s hold */
 } HgNorm;
 
 /*
@@ -93,7 +94,7 @@ typedef struct {
     uint64_t gates;           /* rows of the gate */
     uint64_t chunks, chunk_rows, chunks_per_gate;
     uint32_t by_gate;
-    uint32_t waves, vecs;
+    uint32_t waves, vecs, stream;
     uint32_t sums;            /* rows of cols fp32 a run writes to the workspace: post, pre, gate as wanted */
     int at_post, at_pre, at_gate; /* which of them, -1: not there */
 } HgNormGrad;

@@ -18,15 +18,16 @@ typedef u32x4 __attribute__((aligned(4))) u32x4_at4;
 template <int DT> struct GroupVec { typedef u32x4_at2 type; };
 template <> struct GroupVec<DT_F32> { typedef u32x4_at4 type; };
 
-// elements [at, at + 8) of a row that holds `cols`; those past its end are 0.  NT: a cache hint for what is read (written)
-// once and by no launch that follows soon.
-template <int DT, bool NT = false> __device__ __forceinline__ Raw8<DT> load8(const void* row, uint64_t at, uint64_t cols)
+// Elements [at, at + 8) of a row that holds `cols`; those past its end are 0.  TAIL: a row may end inside a group of eight;
+// without it a group is there or not, and a load is one predicate and no branch of its own.  NT: a cache hint for what
+// is read (written) once and by no launch that follows soon.
+template <int DT, bool TAIL = true, bool NT = false> __device__ __forceinline__ Raw8<DT> load8(const void* row, uint32_t at, uint64_t cols)
 {
     constexpr uint32_t ES = ElemSize<DT>::v;
     typedef const __attribute__((address_space(1))) typename GroupVec<DT>::type cv;
     Raw8<DT> r;
     const uint8_t* p = (const uint8_t*)row + at * ES;
-    if (at + 8u <= cols) {
+    if (TAIL ? at + 8u <= cols : at < cols) {
 #pragma unroll
         for (uint32_t i = 0; i < Raw8<DT>::words / 4u; ++i) {
             const u32x4 v = NT ? __builtin_nontemporal_load((cv*)p + i) : ((cv*)p)[i];
@@ -35,7 +36,7 @@ template <int DT, bool NT = false> __device__ __forceinline__ Raw8<DT> load8(con
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < Raw8<DT>::words; ++i) r.w[i] = 0u;
-        if (at < cols) {
+        if (TAIL && at < cols) {
             const uint32_t n = (uint32_t)(cols - at);
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e)
@@ -78,19 +79,19 @@ template <int DT> __device__ __forceinline__ Raw8<DT> narrow8(const float (&f)[8
     return r;
 }
 
-template <int DT, bool NT = false> __device__ __forceinline__ void store8(void* row, uint64_t at, uint64_t cols, const Raw8<DT>& r)
+template <int DT, bool TAIL = true, bool NT = false> __device__ __forceinline__ void store8(void* row, uint32_t at, uint64_t cols, const Raw8<DT>& r)
 {
     constexpr uint32_t ES = ElemSize<DT>::v;
     typedef __attribute__((address_space(1))) typename GroupVec<DT>::type wv;
     uint8_t* p = (uint8_t*)row + at * ES;
-    if (at + 8u <= cols) {
+    if (TAIL ? at + 8u <= cols : at < cols) {
 #pragma unroll
         for (uint32_t i = 0; i < Raw8<DT>::words / 4u; ++i) {
             const typename GroupVec<DT>::type v = u32x4{r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]};
             if (NT) __builtin_nontemporal_store(v, (wv*)p + i);
             else ((wv*)p)[i] = v;
         }
-    } else if (at < cols) {
+    } else if (TAIL && at < cols) {
         const uint32_t n = (uint32_t)(cols - at);
 #pragma unroll
         for (uint32_t e = 0; e < 8u; ++e)
