@@ -42,10 +42,14 @@ template <bool ONE, uint32_t U> __device__ __forceinline__ Place<ONE> place_of(c
 
 // Eight elements of a dense matrix at a place, and where they go back.  What is quantised and the dense results pass by
 // the caches: 67.1M bf16 elements quantised 39 -> 28 us, 14.3M fp32 results of seven ranks 29 -> 23.
-template <int DT, bool NT, bool ONE> __device__ __forceinline__ Raw8<DT> load_at(const void* m, uint64_t stride, const Place<ONE>& p, uint64_t cols)
+template <int DT, bool NT, bool ONE> __device__ __forceinline__ Raw8<DT> ask_at(const void* m, uint64_t stride, const Place<ONE>& p, uint64_t cols)
 {
     const uint64_t at = (uint64_t)p.tile * 8u;
-    return load8<DT, true, NT>((const uint8_t*)m + (p.row * stride + at) * ElemSize<DT>::v, p.group * 8u, p.there ? cols - at : 0u);
+    return ask8<DT, true, NT>((const uint8_t*)m + (p.row * stride + at) * ElemSize<DT>::v, p.group * 8u, p.there ? cols - at : 0u, cols < 8u);
+}
+template <int DT, bool ONE> __device__ __forceinline__ void settle_at(Raw8<DT>& v, const Place<ONE>& p, uint64_t cols)
+{
+    settle8<DT, true>(v, p.group * 8u, p.there ? cols - (uint64_t)p.tile * 8u : 0u, cols < 8u);
 }
 template <int DT, bool ONE> __device__ __forceinline__ void store_at(void* m, uint64_t stride, const Place<ONE>& p, uint64_t cols, const Raw8<DT>& v)
 {
@@ -98,10 +102,12 @@ template <int DT, bool ONE, uint32_t U> __global__ __launch_bounds__(256) void k
 {
     Raw8<DT> x[U];
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) x[u] = load_at<DT, true>(a.src, a.src_stride, place_of<ONE, U>(a.grid, u), a.grid.cols);
+    for (uint32_t u = 0; u < U; ++u) x[u] = ask_at<DT, true>(a.src, a.src_stride, place_of<ONE, U>(a.grid, u), a.grid.cols);
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
+        const Place<ONE> p = place_of<ONE, U>(a.grid, u);
         float f[8];
+        settle_at(x[u], p, a.grid.cols);
         widen8<DT>(x[u], f);
         uint32_t m = 0;
 #pragma unroll
@@ -110,7 +116,6 @@ template <int DT, bool ONE, uint32_t U> __global__ __launch_bounds__(256) void k
             m = b > m ? b : m;
         }
         const uint32_t s = scale_of(quad_max(m));
-        const Place<ONE> p = place_of<ONE, U>(a.grid, u);
         if (p.there) put_group(a.out, p, encode8(f, s), s);
     }
 }
@@ -177,7 +182,7 @@ template <int DT, bool ONE, uint32_t U, uint32_t N, bool JOIN> __global__ __laun
         double v[8];             // JOIN: the sum
         float odd[8], near[8];   // the sum as what narrower types round it from, and rounded to fp32
         Raw8<DT> own;
-        if (JOIN && a.addend) own = load_at<DT, false>(a.addend, a.addend_stride, p, a.grid.cols);
+        if (JOIN && a.addend) own = ask_at<DT, false>(a.addend, a.addend_stride, p, a.grid.cols);
         for (uint32_t j0 = 0; j0 < (JOIN ? a.k : 1u); j0 += B) {
             uint32_t w[B], s[B];
             const uint32_t n = N == 1u ? 1u : min(a.k - j0, B);
@@ -195,6 +200,7 @@ template <int DT, bool ONE, uint32_t U, uint32_t N, bool JOIN> __global__ __laun
             const bool empty = !JOIN || (j0 == 0u && !a.addend);
             if (JOIN && j0 == 0u && a.addend) {
                 float x[8];
+                settle_at(own, p, a.grid.cols);
                 widen8<DT>(own, x);
 #pragma unroll
                 for (uint32_t e = 0; e < 8u; ++e) v[e] = (double)x[e];

@@ -75,6 +75,7 @@ template <int DT, int PT, uint32_t V, bool ONE, bool TAIL, bool NT, uint32_t N> 
     const uint32_t span = a.waves * 64u, local = ONE ? 0u : threadIdx.x / span, t = threadIdx.x - local * span;
     const uint64_t row = ONE ? blockIdx.x : (uint64_t)blockIdx.x * a.rows_per_wg + local;
     const uint64_t cols = ONE || row < a.d.rows ? a.d.cols : 0u; // a row that is not there has no columns
+    const bool tiny = a.d.cols < 8u;
     float f[V][8];
     Raw8<DT> x[AHEAD][V], res[V];
     Raw8<PT> post[V], pre[V], gate[V];
@@ -84,7 +85,7 @@ template <int DT, int PT, uint32_t V, bool ONE, bool TAIL, bool NT, uint32_t N> 
             if (j0 + j < a.d.k) {
 #pragma unroll
                 for (uint32_t v = 0; v < V; ++v)
-                    x[j][v] = load8<DT, TAIL, NT>((const uint8_t*)a.src[j0 + j] + row * a.d.srcStride * ES, (v * span + t) * 8u, cols);
+                    x[j][v] = ask8<DT, TAIL, NT>((const uint8_t*)a.src[j0 + j] + row * a.d.srcStride * ES, (v * span + t) * 8u, cols, tiny);
             }
     };
     auto add = [&](uint32_t j0) {
@@ -94,6 +95,7 @@ template <int DT, int PT, uint32_t V, bool ONE, bool TAIL, bool NT, uint32_t N> 
 #pragma unroll
                 for (uint32_t v = 0; v < V; ++v) {
                     float g[8];
+                    settle8<DT, TAIL>(x[j][v], (v * span + t) * 8u, cols, tiny);
                     widen8<DT>(x[j][v], g);
 #pragma unroll
                     for (uint32_t e = 0; e < 8u; ++e) f[v][e] = j0 + j == 0u ? g[e] : f[v][e] + g[e];
@@ -106,12 +108,20 @@ template <int DT, int PT, uint32_t V, bool ONE, bool TAIL, bool NT, uint32_t N> 
 #pragma unroll
     for (uint32_t v = 0; v < V; ++v) {
         const uint32_t at = (v * span + t) * 8u;
-        if (a.d.residual) res[v] = load8<DT, TAIL, NT>((const uint8_t*)a.d.residual + row * a.d.residualStride * ES, at, cols);
-        if (a.d.postWeight) post[v] = load8<PT, TAIL>(a.d.postWeight, at, cols);
-        if (a.d.gate) gate[v] = load8<PT, TAIL>((const uint8_t*)a.d.gate + (uint64_t)gate_row * a.d.gateStride * PS, at, cols);
-        if (a.d.preWeight) pre[v] = load8<PT, TAIL>(a.d.preWeight, at, cols);
+        if (a.d.residual) res[v] = ask8<DT, TAIL, NT>((const uint8_t*)a.d.residual + row * a.d.residualStride * ES, at, cols, tiny);
+        if (a.d.postWeight) post[v] = ask8<PT, TAIL, false>(a.d.postWeight, at, cols, tiny);
+        if (a.d.gate) gate[v] = ask8<PT, TAIL, false>((const uint8_t*)a.d.gate + (uint64_t)gate_row * a.d.gateStride * PS, at, cols, tiny);
+        if (a.d.preWeight) pre[v] = ask8<PT, TAIL, false>(a.d.preWeight, at, cols, tiny);
     }
     add(0);
+#pragma unroll
+    for (uint32_t v = 0; v < V; ++v) {
+        const uint32_t at = (v * span + t) * 8u;
+        if (a.d.residual) settle8<DT, TAIL>(res[v], at, cols, tiny);
+        if (a.d.postWeight) settle8<PT, TAIL>(post[v], at, cols, tiny);
+        if (a.d.gate) settle8<PT, TAIL>(gate[v], at, cols, tiny);
+        if (a.d.preWeight) settle8<PT, TAIL>(pre[v], at, cols, tiny);
+    }
     for (uint32_t j0 = AHEAD; j0 < a.d.k; j0 += AHEAD) {
         ask(j0);
         add(j0);
@@ -180,6 +190,7 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool TAIL, bool NT> __globa
     constexpr uint32_t ES = ElemSize<DT>::v, PS = ElemSize<PT>::v;
     const uint32_t span = a.waves * 64u, t = threadIdx.x;
     const uint64_t cols = a.d.cols;
+    const bool tiny = cols < 8u;
     const bool has_post = a.d.postWeight != nullptr, has_pre = a.d.preWeight != nullptr, has_gate = a.d.gate != nullptr;
     uint32_t row, end; // the host keeps rows below 2^31
     if (a.by_gate) {
@@ -198,12 +209,12 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool TAIL, bool NT> __globa
 #pragma unroll
         for (uint32_t v = 0; v < V; ++v) {
             const uint32_t at = (v * span + t) * 8u;
-            x.s[v] = load8<DT, TAIL, NT>((const uint8_t*)a.d.sum + r * a.d.sumStride * ES, at, cols);
+            x.s[v] = ask8<DT, TAIL, NT>((const uint8_t*)a.d.sum + r * a.d.sumStride * ES, at, cols, tiny);
             if (has_pre) {
-                x.y[v] = load8<DT, TAIL, NT>((const uint8_t*)a.d.y + r * a.d.yStride * ES, at, cols);
-                x.dz[v] = load8<DT, TAIL, NT>((const uint8_t*)a.d.dz + r * a.d.dzStride * ES, at, cols);
+                x.y[v] = ask8<DT, TAIL, NT>((const uint8_t*)a.d.y + r * a.d.yStride * ES, at, cols, tiny);
+                x.dz[v] = ask8<DT, TAIL, NT>((const uint8_t*)a.d.dz + r * a.d.dzStride * ES, at, cols, tiny);
             }
-            x.dy[v] = load8<DT, TAIL, NT>((const uint8_t*)a.d.dy + r * a.d.dyStride * ES, at, cols);
+            x.dy[v] = ask8<DT, TAIL, NT>((const uint8_t*)a.d.dy + r * a.d.dyStride * ES, at, cols, tiny);
         }
     };
     Row next;
@@ -212,8 +223,8 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool TAIL, bool NT> __globa
     float d_post[V][8], d_pre[V][8], d_gate[V][8];
 #pragma unroll
     for (uint32_t v = 0; v < V; ++v) {
-        if (has_pre) pre[v] = load8<PT, TAIL>(a.d.preWeight, (v * span + t) * 8u, cols);
-        if (has_post) post[v] = load8<PT, TAIL>(a.d.postWeight, (v * span + t) * 8u, cols);
+        if (has_pre) pre[v] = ask8<PT, TAIL, false>(a.d.preWeight, (v * span + t) * 8u, cols, tiny);
+        if (has_post) post[v] = ask8<PT, TAIL, false>(a.d.postWeight, (v * span + t) * 8u, cols, tiny);
 #pragma unroll
         for (uint32_t e = 0; e < 8u; ++e) d_post[v][e] = d_pre[v][e] = d_gate[v][e] = 0.0f;
     }
@@ -223,11 +234,25 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool TAIL, bool NT> __globa
         gate_row = row / (uint32_t)a.d.rowsPerGate;
         gate_end = (gate_row + 1u) * (uint32_t)a.d.rowsPerGate;
 #pragma unroll
-        for (uint32_t v = 0; v < V; ++v) gate[v] = load8<PT, TAIL>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols);
+        for (uint32_t v = 0; v < V; ++v) gate[v] = ask8<PT, TAIL, false>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols, tiny);
+    }
+#pragma unroll
+    for (uint32_t v = 0; v < V; ++v) {
+        const uint32_t at = (v * span + t) * 8u;
+        if (has_pre) settle8<PT, TAIL>(pre[v], at, cols, tiny);
+        if (has_post) settle8<PT, TAIL>(post[v], at, cols, tiny);
+        if (has_gate && row < end) settle8<PT, TAIL>(gate[v], at, cols, tiny);
     }
     for (; row < end; ++row) {
-        const Row x = next;
+        Row x = next;
         if (row + 1u < end) ask(next, row + 1u);
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v) {
+            const uint32_t at = (v * span + t) * 8u;
+            settle8<DT, TAIL>(x.s[v], at, cols, tiny);
+            settle8<DT, TAIL>(x.dy[v], at, cols, tiny);
+            if (has_pre) settle8<DT, TAIL>(x.y[v], at, cols, tiny), settle8<DT, TAIL>(x.dz[v], at, cols, tiny);
+        }
         float q[3] = {0.0f, 0.0f, 0.0f}; // sum^2, y^2, dz preWeight y
 #pragma unroll
         for (uint32_t v = 0; v < V; ++v) {
@@ -314,55 +339,69 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool TAIL, bool NT> __globa
                 if (a.d.dGate) store8<PT, TAIL>((uint8_t*)a.d.dGate + g * a.d.dGateStride * PS, (v * span + t) * 8u, cols, narrow8<PT>(d_gate[v]));
 #pragma unroll
                 for (uint32_t e = 0; e < 8u; ++e) d_gate[v][e] = 0.0f;
-                if (row + 1u < end) gate[v] = load8<PT, TAIL>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols);
+                if (row + 1u < end) {
+                    gate[v] = ask8<PT, TAIL, false>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols, tiny);
+                    settle8<PT, TAIL>(gate[v], (v * span + t) * 8u, cols, tiny);
+                }
             }
         }
     }
-    float* mine = (float*)a.d.workspace + (uint64_t)blockIdx.x * a.sums * cols;
+    float* mine = (float*)a.d.workspace + (uint64_t)blockIdx.x * a.sums * a.pitch;
 #pragma unroll
     for (uint32_t v = 0; v < V; ++v) {
-        const uint32_t at = (v * span + t) * 8u;
-        if (a.at_post >= 0) store8<DT_F32, TAIL>(mine + (uint64_t)a.at_post * cols, at, cols, narrow8<DT_F32>(d_post[v]));
-        if (a.at_pre >= 0) store8<DT_F32, TAIL>(mine + (uint64_t)a.at_pre * cols, at, cols, narrow8<DT_F32>(d_pre[v]));
-        if (a.at_gate >= 0) store8<DT_F32, TAIL>(mine + (uint64_t)a.at_gate * cols, at, cols, narrow8<DT_F32>(d_gate[v]));
+        const uint32_t at = (v * span + t) * 8u; // the workspace's rows hold whole groups
+        if (a.at_post >= 0) store8<DT_F32, false>(mine + (uint64_t)a.at_post * a.pitch, at, a.pitch, narrow8<DT_F32>(d_post[v]));
+        if (a.at_pre >= 0) store8<DT_F32, false>(mine + (uint64_t)a.at_pre * a.pitch, at, a.pitch, narrow8<DT_F32>(d_pre[v]));
+        if (a.at_gate >= 0) store8<DT_F32, false>(mine + (uint64_t)a.at_gate * a.pitch, at, a.pitch, narrow8<DT_F32>(d_gate[v]));
     }
 }
 
-// The runs' sums joined, in the order of the runs: a workgroup takes 64 columns of one result, its 16 wavefronts every
-// sixteenth run each.
+// The runs' sums joined, in a fixed order: a workgroup takes 64 columns of one result, four neighbours to a lane, and 64
+// of its lanes share a column's runs.
+#define SUM_COLS 64u
+
 template <int PT> __global__ __launch_bounds__(1024) void k_norm_sums(const HgNormGrad a)
 {
-    __shared__ float part[16][64];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint64_t col = (uint64_t)blockIdx.x * 64u + lane;
+    __shared__ float part[16][SUM_COLS];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, in = lane & 15u;
     const uint32_t results = (a.at_post >= 0) + (a.at_pre >= 0);
-    uint64_t first = 0u, n = a.chunks;
-    uint32_t which;
+    uint32_t first = 0u, n = (uint32_t)a.chunks, which;
     uint8_t* out;
     if (blockIdx.y < results) {
         const bool post = blockIdx.y == 0u && a.at_post >= 0;
         which = (uint32_t)(post ? a.at_post : a.at_pre);
         out = (uint8_t*)(post ? a.d.dPostWeight : a.d.dPreWeight);
     } else {
-        const uint64_t g = blockIdx.y - results;
+        const uint32_t g = blockIdx.y - results;
         which = (uint32_t)a.at_gate;
-        first = g * a.chunks_per_gate;
-        n = a.chunks_per_gate;
+        first = g * (uint32_t)a.chunks_per_gate;
+        n = (uint32_t)a.chunks_per_gate;
         out = (uint8_t*)a.d.dGate + g * a.d.dGateStride * ElemSize<PT>::v;
     }
-    float s = 0.0f;
-    if (col < a.d.cols) {
-        const float* p = (const float*)a.d.workspace + (first * a.sums + which) * a.d.cols + col;
+    const uint64_t step = a.sums * (a.pitch / 4u); // in vectors of four
+    cgvec* p = (cgvec*)a.d.workspace + first * step + which * (a.pitch / 4u) + blockIdx.x * (SUM_COLS / 4u) + in;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
-        for (uint64_t i = wave; i < n; i += 16u) s += p[i * a.sums * a.d.cols];
+    for (uint32_t i = wave * 4u + (lane >> 4); i < n; i += 64u) {
+        const u32x4 v = p[i * step];
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) s[e] += bits_f32(v[e]);
     }
-    part[wave][lane] = s;
+#pragma unroll
+    for (uint32_t e = 0; e < 4u; ++e) {
+        s[e] += __shfl_xor(s[e], 16);
+        s[e] += __shfl_xor(s[e], 32);
+        if (lane < 16u) part[wave][in * 4u + e] = s[e];
+    }
     __syncthreads();
-    if (wave == 0u && col < a.d.cols) {
-        for (uint32_t w = 1; w < 16u; ++w) s += part[w][lane];
-        if (PT == DT_F32) ((float*)out)[col] = s;
-        else if (PT == DT_BF16) ((__bf16*)out)[col] = (__bf16)s;
-        else ((_Float16*)out)[col] = (_Float16)s;
+    const uint32_t col = blockIdx.x * SUM_COLS + threadIdx.x;
+    if (threadIdx.x < SUM_COLS && col < a.d.cols) {
+        float t = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < 16u; ++w) t += part[w][threadIdx.x];
+        if (PT == DT_F32) ((float*)out)[col] = t;
+        else if (PT == DT_BF16) ((__bf16*)out)[col] = (__bf16)t;
+        else ((_Float16*)out)[col] = (_Float16)t;
     }
 }
 
@@ -447,7 +486,7 @@ int hg_launch_norm_sums(void* stream, const void* args)
     const HgNormGrad* a = (const HgNormGrad*)args;
     OnDeviceOf device((hipStream_t)stream);
     if (device.err != hipSuccess) return HCCL_E_RUNTIME;
-    const dim3 g((uint32_t)((a->d.cols + 63u) / 64u), (uint32_t)((a->at_post >= 0) + (a->at_pre >= 0) + (a->at_gate >= 0 ? a->gates : 0u))), b(1024);
+    const dim3 g((uint32_t)((a->d.cols + SUM_COLS - 1u) / SUM_COLS), (uint32_t)((a->at_post >= 0) + (a->at_pre >= 0) + (a->at_gate >= 0 ? a->gates : 0u))), b(1024);
     switch (a->d.paramType) {
         case HCOMM_DATA_TYPE_FP16: hipLaunchKernelGGL((k_norm_sums<DT_F16>), g, b, 0, (hipStream_t)stream, *a); break;
         case HCOMM_DATA_TYPE_BFP16: hipLaunchKernelGGL((k_norm_sums<DT_BF16>), g, b, 0, (hipStream_t)stream, *a); break;

@@ -374,12 +374,13 @@ static void norm_grad_shape(HgNormGrad* a)
         a->chunks = gate_rows(rows, a->chunk_rows);
     }
     a->sums = 0;
+    a->pitch = (uint32_t)(d->cols + 63u) / 64u * 64u;
     a->at_post = d->dPostWeight ? (int)a->sums++ : -1;
     a->at_pre = d->dPreWeight ? (int)a->sums++ : -1;
     a->at_gate = a->by_gate ? (int)a->sums++ : -1;
 }
 
-static uint64_t norm_grad_workspace(const HgNormGrad* a) { return a->chunks * a->sums * a->d.cols * sizeof(float); }
+static uint64_t norm_grad_workspace(const HgNormGrad* a) { return a->chunks * a->sums * a->pitch * sizeof(float); }
 
 int32_t HcommGfxReduceNormGradWorkspaceBytes(const HcommGfxReduceNormGradDesc* desc, uint64_t* bytes)
 {

@@ -95,7 +95,8 @@ typedef struct {
     uint64_t chunks, chunk_rows, chunks_per_gate;
     uint32_t by_gate;
     uint32_t waves, vecs, stream;
-    uint32_t sums;            /* rows of cols fp32 a run writes to the workspace: post, pre, gate as wanted */
+    uint32_t sums;            /* rows of `pitch` fp32 a run writes to the workspace: post, pre, gate as wanted */
+    uint32_t pitch;           /* cols rounded up to 64 */
     int at_post, at_pre, at_gate; /* which of them, -1: not there */
 } HgNormGrad;
 

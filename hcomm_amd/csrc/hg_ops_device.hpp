@@ -18,36 +18,58 @@ typedef u32x4 __attribute__((aligned(4))) u32x4_at4;
 template <int DT> struct GroupVec { typedef u32x4_at2 type; };
 template <> struct GroupVec<DT_F32> { typedef u32x4_at4 type; };
 
-// Elements [at, at + 8) of a row that holds `cols`; those past its end are 0.  TAIL: a row may end inside a group of eight;
-// without it a group is there or not, and a load is one predicate and no branch of its own.  NT: a cache hint for what
-// is read (written) once and by no launch that follows soon.
-template <int DT, bool TAIL = true, bool NT = false> __device__ __forceinline__ Raw8<DT> load8(const void* row, uint32_t at, uint64_t cols)
+// Elements [at, at + 8) of a row of which `cols` are left; those past its end are 0.  TAIL: a row may end inside a group of
+// eight; without it a group is there or not.  NT: a cache hint for what is read (written) once and by no launch that follows
+// soon.  A group that the row's end cuts is read as the row's last eight elements, which settle8, called where the group is
+// used, moves to where they belong: no load waits for another.  `short_row`: the whole row has fewer than eight (uniform).
+template <int DT, bool TAIL, bool NT> __device__ __forceinline__ Raw8<DT> ask8(const void* row, uint32_t at, uint64_t cols, bool short_row)
 {
-    constexpr uint32_t ES = ElemSize<DT>::v;
+    constexpr uint32_t ES = ElemSize<DT>::v, W = Raw8<DT>::words;
     typedef const __attribute__((address_space(1))) typename GroupVec<DT>::type cv;
     Raw8<DT> r;
-    const uint8_t* p = (const uint8_t*)row + at * ES;
-    if (TAIL ? at + 8u <= cols : at < cols) {
 #pragma unroll
-        for (uint32_t i = 0; i < Raw8<DT>::words / 4u; ++i) {
+    for (uint32_t i = 0; i < W; ++i) r.w[i] = 0u;
+    if (TAIL && short_row) {
+        // from the last element on, each moves those behind it up by one place
+#pragma unroll 1
+        for (uint32_t e = at == 0u ? (uint32_t)cols : 0u; e-- != 0u;) {
+            const uint32_t x = ld_elem<ES>((const uint8_t*)row + e * ES);
+#pragma unroll
+            for (uint32_t i = W; i-- != 0u;) {
+                const uint32_t below = i ? r.w[i ? i - 1u : 0u] : 0u;
+                r.w[i] = ES == 4u ? (i ? below : x) : (r.w[i] << 16) | (i ? below >> 16 : x);
+            }
+        }
+        return r;
+    }
+    if (at < cols) {
+        const int32_t back = TAIL && at + 8u > cols ? (int32_t)(at + 8u - (uint32_t)cols) : 0; // may reach in front of `row`, not of the whole row
+        const uint8_t* p = (const uint8_t*)row + (int64_t)((int32_t)at - back) * (int32_t)ES;
+#pragma unroll
+        for (uint32_t i = 0; i < W / 4u; ++i) {
             const u32x4 v = NT ? __builtin_nontemporal_load((cv*)p + i) : ((cv*)p)[i];
             r.w[4 * i] = v.x, r.w[4 * i + 1] = v.y, r.w[4 * i + 2] = v.z, r.w[4 * i + 3] = v.w;
         }
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < Raw8<DT>::words; ++i) r.w[i] = 0u;
-        if (TAIL && at < cols) {
-            const uint32_t n = (uint32_t)(cols - at);
-#pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e)
-                if (e < n) {
-                    const uint32_t x = ld_elem<ES>(p + e * ES);
-                    if (ES == 4) r.w[e] = x;
-                    else r.w[e / 2u] |= x << (16u * (e % 2u));
-                }
-        }
     }
     return r;
+}
+
+template <int DT, bool TAIL> __device__ __forceinline__ void settle8(Raw8<DT>& r, uint32_t at, uint64_t cols, bool short_row)
+{
+    if (!TAIL || short_row || at >= cols || at + 8u <= cols) return;
+    const uint32_t by = (at + 8u - (uint32_t)cols) * ElemSize<DT>::v; // bytes that lie in front
+    constexpr uint32_t W = Raw8<DT>::words;
+#pragma unroll
+    for (uint32_t step = 1; step < W; step *= 2u)
+#pragma unroll
+        for (uint32_t i = 0; i < W; ++i) {
+            const uint32_t from = i + step < W ? r.w[i + step < W ? i + step : i] : 0u;
+            r.w[i] = (by & (4u * step)) ? from : r.w[i];
+        }
+    if (ElemSize<DT>::v == 2u && (by & 2u)) {
+#pragma unroll
+        for (uint32_t i = 0; i < W; ++i) r.w[i] = (r.w[i] >> 16) | (i + 1u < W ? r.w[i + 1u < W ? i + 1u : i] << 16 : 0u);
+    }
 }
 
 template <int DT> __device__ __forceinline__ void widen8(const Raw8<DT>& r, float (&f)[8])
@@ -92,10 +114,17 @@ template <int DT, bool TAIL = true, bool NT = false> __device__ __forceinline__ 
             else ((wv*)p)[i] = v;
         }
     } else if (TAIL && at < cols) {
-        const uint32_t n = (uint32_t)(cols - at);
+        Raw8<DT> v = r;
+#pragma unroll 1
+        for (uint32_t e = 0, n = (uint32_t)(cols - at); e < n; ++e) {
+            st_elem<ES>(p + e * ES, ES == 4u ? v.w[0] : v.w[0] & 0xffffu);
+            // the next element takes the first one's place
 #pragma unroll
-        for (uint32_t e = 0; e < 8u; ++e)
-            if (e < n) st_elem<ES>(p + e * ES, ES == 4 ? r.w[e % Raw8<DT>::words] : (r.w[e / 2u] >> (16u * (e % 2u))) & 0xffffu);
+            for (uint32_t i = 0; i < Raw8<DT>::words; ++i) {
+                const uint32_t above = i + 1u < Raw8<DT>::words ? v.w[i + 1u < Raw8<DT>::words ? i + 1u : i] : 0u;
+                v.w[i] = ES == 4u ? above : (v.w[i] >> 16) | (above << 16);
+            }
+        }
     }
 }
 

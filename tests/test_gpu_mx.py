@@ -298,3 +298,23 @@ def test_two_streams_and_a_graph_give_the_eager_bits():
                 assert torch.equal(got, exp), step
     del keep
     h.HcommThreadFreeWithStream(threads)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_ends_of_rows(gpu_thread, t):
+    """Every place in a block at which a row can end, in rows shorter than a group, long ones and ones just past a workgroup's
+    piece; what lies in front of a row is not part of it."""
+    rng = np.random.default_rng(6)
+    for cols in list(range(1, 42)) + [2048 + d for d in (0, 1, 3, 7, 8, 9)] + [8192 + d for d in (1, 5, 31, 33)]:
+        rows = 3
+        src = Dense(rows, cols, t, cols + 9, 5, awkward(rows, cols, t, rng))
+        out, total = Mx(rows, cols, 1), Dense(rows, cols, t, cols + 2, 1)
+        ready()
+        view = h.mx_views([out.item])
+        h.check(h.HcommGfxMxQuantizeOnThread(gpu_thread, view, src.ptr, src.stride, rows, cols, DT[t]))
+        h.check(h.HcommGfxMxReduceKOnThread(gpu_thread, total.ptr, total.stride, DT[t], None, view, 1, src.ptr, src.stride, rows, cols))
+        sync(gpu_thread)
+        code, scale = ref.mx_encode(src.double())
+        assert np.array_equal(out.scale(), scale) and np.array_equal(out.code(), code), cols
+        close(total.double(), src.double() + ref.mx_values(code, scale, cols), t, 0.0, cols)
+        assert out.guards_hold() and total.guards_hold()

@@ -336,3 +336,10 @@ def test_rows_past_32_bits(gpu_thread):
     c.sum, c.y, c.z, c.ds, c.dres, c.dgate = (Far(i) for i in range(5, 11))
     c.stride = far
     c.run(gpu_thread)
+
+
+@pytest.mark.parametrize("t,p", [("bf16", "bf16"), ("fp16", "fp32"), ("fp32", "fp32")])
+def test_ends_of_rows(gpu_thread, t, p):
+    """Every place in a group of eight elements at which a row can end, around the sizes at which another wavefront joins."""
+    for cols in list(range(1, 18)) + [512 + d for d in range(-1, 9)] + [1030, 2047, 4099, 8193, 8198]:
+        Case(4, cols, t, k=2, p=p, per=3, pad=1).run(gpu_thread)
