@@ -1,94 +1,135 @@
 // hg_mx_product.hip - the product of two matrices in microscaled 4-bit floating point, summed over the ranks that share
 // its inner length: dst = sum over r of a[r] * transpose(b[r]).
 //
-// The matrix instruction of 16 x 16 x 128 takes the format as it is stored: lane l gives row l % 16 of an operand, 32
-// consecutive elements (one block, 16 bytes) and that block's scale byte, and the four lanes of a row cover 128
-// elements.  Which blocks those are is free, as long as both operands agree.  A chunk of 16 blocks of a row is given to
-// its four lanes in runs of four, so that a lane's scales for four instructions are one dword of the scale row, of
-// which every instruction selects its byte.
+// The matrix instructions take the format as it is stored.  16 x 16 x 128: lane l gives row l % 16 of an operand, block l / 16
+// of four neighbours (32 elements, 16 bytes) and that block's scale byte; 32 x 32 x 64: row l % 32, block l / 32 of two.
 #include "hg_ops_device.hpp"
 
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32_at1 __attribute__((aligned(1)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 __attribute__((aligned(2))) u32x2_at2;
 
 #define MX_FP4 4 /* element format operand of the matrix instruction */
 #define CHUNK_BLOCKS 16u
 
-// acc += a * b for byte T of each lane's scales
-template <int T> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 acc, uint32_t sa, uint32_t sb)
+// acc += a * b under the scales in byte 0
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 acc, uint32_t sa, uint32_t sb)
 {
     const i32x8 av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}, bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, MX_FP4, MX_FP4, T, (int)sa, T, (int)sb);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, MX_FP4, MX_FP4, 0, (int)sa, 0, (int)sb);
 }
 
-// what a lane holds of one row for one chunk: four blocks and their scales
+// What a lane holds of one row for one chunk of 16 blocks: of every four neighbours its own (the four lanes of a row read 64
+// bytes in one piece then), and the chunk's scales, of which instruction t takes byte lane / 16 of word t.
 struct Run {
     u32x4 block[4];
-    uint32_t scales;
+    u32x4 scales;
 };
 
-// blocks [first, first + 4) of a row of `blocks`; those past its end are 0 under scale 1
-__device__ __forceinline__ Run load_run(const HgMxView& v, uint64_t row, uint32_t first, uint32_t blocks)
+typedef u32x4 __attribute__((aligned(1))) u32x4_at1;
+
+// Blocks [first, first + 16) of a row of `blocks`.  No branch: loads of several runs are to be under way together.  Past the
+// row's end its last block is read once more, and settle_run, called where the run is used, takes care of it.  g: lane / 16
+// SHORT: the rows have fewer than 16 blocks, scales come byte by byte.
+template <bool SHORT> __device__ __forceinline__ Run load_run(const HgMxView& v, uint32_t row, uint32_t first, uint32_t blocks, uint32_t g)
 {
+    typedef const __attribute__((address_space(1))) uint8_t cg8;
     Run r;
-    cgvec* p = (cgvec*)(v.packed + row * v.packed_stride) + first;
-    const __attribute__((address_space(1))) uint8_t* s = (const __attribute__((address_space(1))) uint8_t*)(v.scales + row * v.scale_stride) + first;
-    if (first + 4u <= blocks) {
+    const uint8_t* p = v.packed + (uint64_t)row * v.packed_stride;
+    const uint8_t* s = v.scales + (uint64_t)row * v.scale_stride;
 #pragma unroll
-        for (uint32_t t = 0; t < 4u; ++t) r.block[t] = p[t];
-        r.scales = *(const __attribute__((address_space(1))) u32_at1*)s;
+    for (uint32_t t = 0; t < 4u; ++t) r.block[t] = ((cgvec*)p)[min(first + 4u * t + g, blocks - 1u)];
+    if (SHORT) {
+#pragma unroll
+        for (uint32_t t = 0; t < 4u; ++t) r.scales[t] = (uint32_t)((cg8*)s)[min(4u * t + g, blocks - 1u)];
     } else {
-        r.scales = 0x7f7f7f7fu;
-#pragma unroll
-        for (uint32_t t = 0; t < 4u; ++t) {
-            r.block[t] = u32x4{0u, 0u, 0u, 0u};
-            if (first + t < blocks) {
-                r.block[t] = p[t];
-                r.scales = (r.scales & ~(0xffu << (8u * t))) | ((uint32_t)s[t] << (8u * t));
-            }
-        }
+        r.scales = *(const __attribute__((address_space(1))) u32x4_at1*)(s + min(first, blocks - CHUNK_BLOCKS));
     }
     return r;
 }
 
-// elements past `cols` do not count, whatever the last block holds there (one operand's being 0 is enough)
-__device__ __forceinline__ void cut_run(Run& r, uint32_t first, uint32_t cols)
+// w shifted down by `by` bytes, 0 from 16 on
+__device__ __forceinline__ u32x4 down_by(u32x4 w, uint32_t by)
 {
-    const uint32_t last = (cols - 1u) / HCOMM_GFX_MX_BLOCK, n = cols - last * HCOMM_GFX_MX_BLOCK; // n elements of block `last` count
+#pragma unroll
+    for (uint32_t step = 1; step < 4u; step *= 2u)
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            const uint32_t from = i + step < 4u ? w[i + step < 4u ? i + step : i] : 0u;
+            w[i] = (by & (4u * step)) ? from : w[i];
+        }
+    u32x4 r;
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) {
+        r[i] = __builtin_amdgcn_alignbit(i < 3u ? w[i < 3u ? i + 1u : i] : 0u, w[i], 8u * (by % 4u));
+        r[i] = by < 16u ? r[i] : 0u;
+    }
+    return r;
+}
+
+// A row's last chunk: scales of blocks past the end become 0 (with 2^-127 on both sides the products are far below what
+// fp32 holds), elements of the last block past cols become 0.
+template <bool SHORT> __device__ __forceinline__ void settle_run(Run& r, uint32_t first, uint32_t blocks, uint32_t cols, uint32_t g)
+{
+    if (SHORT) {
+#pragma unroll
+        for (uint32_t t = 0; t < 4u; ++t) r.scales[t] = 4u * t + g < blocks ? r.scales[t] : 0u;
+    } else {
+        const uint32_t by = first - min(first, blocks - CHUNK_BLOCKS); // bytes that the fetch went back
+        r.scales = down_by(r.scales, by);
+    }
+    const uint32_t last = blocks - 1u, n = cols - last * HCOMM_GFX_MX_BLOCK; // n elements of it count
 #pragma unroll
     for (uint32_t t = 0; t < 4u; ++t)
-        if (first + t == last) {
 #pragma unroll
-            for (uint32_t i = 0; i < 4u; ++i) {
-                const uint32_t keep = n > 8u * i ? n - 8u * i : 0u;
-                r.block[t][i] &= keep >= 8u ? 0xffffffffu : (1u << (4u * keep)) - 1u;
-            }
+        for (uint32_t i = 0; i < 4u; ++i) {
+            const uint32_t keep = n > 8u * i ? n - 8u * i : 0u, mask = keep >= 8u ? 0xffffffffu : (1u << (4u * keep)) - 1u;
+            r.block[t][i] &= first + 4u * t + g == last ? mask : 0xffffffffu;
         }
 }
 
-template <int DT> __device__ __forceinline__ void put(void* dst, uint64_t i, float v)
+// four neighbours of a row of dst
+template <int DT> __device__ __forceinline__ void put4(void* row, uint32_t at, uint32_t n, f32x4 v)
 {
-    if (DT == DT_F32) ((__attribute__((address_space(1))) float*)dst)[i] = v;
-    else if (DT == DT_BF16) ((__attribute__((address_space(1))) __bf16*)dst)[i] = (__bf16)v;
-    else ((__attribute__((address_space(1))) _Float16*)dst)[i] = (_Float16)v;
+    constexpr uint32_t ES = ElemSize<DT>::v;
+    uint8_t* p = (uint8_t*)row + (uint64_t)at * ES;
+    const float f[8] = {v.x, v.y, v.z, v.w, 0.0f, 0.0f, 0.0f, 0.0f};
+    const Raw8<DT> r = narrow8<DT>(f);
+    if (at + 4u <= n) {
+        if (ES == 4u) *(__attribute__((address_space(1))) u32x4_at4*)p = u32x4{r.w[0], r.w[1], r.w[2 % Raw8<DT>::words], r.w[3 % Raw8<DT>::words]};
+        else *(__attribute__((address_space(1))) u32x2_at2*)p = u32x2{r.w[0], r.w[1]};
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e)
+            if (at + e < n) st_elem<ES>(p + e * ES, ES == 4u ? r.w[e] : (r.w[e / 2u] >> (16u * (e % 2u))) & 0xffffu);
+    }
 }
+
+// The arguments as the kernels take them: the runtime copies them at every launch, so few ranks carry few views.
+template <uint32_t N> struct ProductArgs {
+    HgMxView a[N], b[N];
+    void* dst;
+    uint64_t dst_stride;
+    uint32_t m, n, cols, k;
+};
 
 // ---- few rows: the operands go from memory straight into the matrix instructions --------------------------------------
 //
-// A workgroup owns 16 FA x 16 FB results; its four wavefronts share the inner length (chunk u of all ranks' chunks goes to
-// wavefront u % 4) and add their sums up through LDS in a fixed order.
-template <int DT, int FA, int FB> __global__ __launch_bounds__(256) void k_mx_product_direct(const HgMxProduct a)
+// A workgroup owns 16 FA x 16 FB results; its W wavefronts share the inner length (chunk u of all ranks' chunks goes to
+// wavefront u % W), each with the next chunk's loads on their way while it multiplies, and add their sums up through LDS in
+// a fixed order.
+template <int DT, int FA, int FB, uint32_t W, bool SHORT, uint32_t N> __global__ __launch_bounds__(64 * W) void k_mx_product_direct(const ProductArgs<N> a)
 {
-    __shared__ f32x4 part[3][FA * FB][64];
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ f32x4 part[W][FA * FB][64];
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, shift = SHORT ? 0u : 8u * g, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t tiles_n = (a.n + 16u * FB - 1u) / (16u * FB);
     const uint32_t tm = blockIdx.x / tiles_n, tn = blockIdx.x - tm * tiles_n;
     const uint32_t m0 = tm * 16u * FA, n0 = tn * 16u * FB;
     const uint32_t blocks = (a.cols + HCOMM_GFX_MX_BLOCK - 1u) / HCOMM_GFX_MX_BLOCK, chunks = (blocks + CHUNK_BLOCKS - 1u) / CHUNK_BLOCKS;
-    uint64_t row_a[FA], row_b[FB]; // rows past the end: the last one once more, its results are not stored
+    uint32_t row_a[FA], row_b[FB]; // rows past the end: the last one once more, its results are not stored
 #pragma unroll
     for (int i = 0; i < FA; ++i) row_a[i] = min(m0 + 16u * i + (lane & 15u), a.m - 1u);
 #pragma unroll
@@ -98,53 +139,68 @@ template <int DT, int FA, int FB> __global__ __launch_bounds__(256) void k_mx_pr
     for (int i = 0; i < FA; ++i)
 #pragma unroll
         for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    uint32_t rank = wave / chunks, chunk = wave - rank * chunks;
-    while (rank < a.k) {
-        const uint32_t first = chunk * CHUNK_BLOCKS + (lane >> 4) * 4u;
-        Run ra[FA], rb[FB];
+    struct Chunk {
+        Run a[FA], b[FB];
+        uint32_t first; // block of its rank
+    } c0, c1;
+    uint32_t rank = wave / chunks, chunk = wave - rank * chunks; // of the next loads
+    auto ask = [&](Chunk& c) {
+        const uint32_t first = chunk * CHUNK_BLOCKS;
+        c.first = first;
 #pragma unroll
-        for (int j = 0; j < FB; ++j) rb[j] = load_run(a.b[rank], row_b[j], first, blocks);
+        for (int j = 0; j < FB; ++j) c.b[j] = load_run<SHORT>(a.b[rank], row_b[j], first, blocks, g);
 #pragma unroll
-        for (int i = 0; i < FA; ++i) ra[i] = load_run(a.a[rank], row_a[i], first, blocks);
-        if (chunk == chunks - 1u) {
+        for (int i = 0; i < FA; ++i) c.a[i] = load_run<SHORT>(a.a[rank], row_a[i], first, blocks, g);
+        chunk += W;
+        while (chunk >= chunks) chunk -= chunks, ++rank;
+    };
+    auto multiply = [&](Chunk& c) {
+        if (c.first + CHUNK_BLOCKS >= blocks) {
 #pragma unroll
-            for (int i = 0; i < FA; ++i) cut_run(ra[i], first, a.cols);
+            for (int i = 0; i < FA; ++i) settle_run<SHORT>(c.a[i], c.first, blocks, a.cols, g);
+#pragma unroll
+            for (int j = 0; j < FB; ++j) settle_run<SHORT>(c.b[j], c.first, blocks, a.cols, g);
         }
 #pragma unroll
-        for (int i = 0; i < FA; ++i)
+        for (uint32_t t = 0; t < 4u; ++t)
 #pragma unroll
-            for (int j = 0; j < FB; ++j) {
-                acc[i][j] = mfma<0>(ra[i].block[0], rb[j].block[0], acc[i][j], ra[i].scales, rb[j].scales);
-                acc[i][j] = mfma<1>(ra[i].block[1], rb[j].block[1], acc[i][j], ra[i].scales, rb[j].scales);
-                acc[i][j] = mfma<2>(ra[i].block[2], rb[j].block[2], acc[i][j], ra[i].scales, rb[j].scales);
-                acc[i][j] = mfma<3>(ra[i].block[3], rb[j].block[3], acc[i][j], ra[i].scales, rb[j].scales);
-            }
-        chunk += 4u;
-        while (chunk >= chunks) chunk -= chunks, ++rank;
+            for (int i = 0; i < FA; ++i)
+#pragma unroll
+                for (int j = 0; j < FB; ++j)
+                    acc[i][j] = mfma(c.b[j].block[t], c.a[i].block[t], acc[i][j], c.b[j].scales[t] >> shift, c.a[i].scales[t] >> shift);
+    };
+    if (rank < a.k) {
+        ask(c0);
+        for (;;) {
+            const bool more1 = rank < a.k;
+            if (more1) ask(c1);
+            multiply(c0);
+            if (!more1) break;
+            const bool more0 = rank < a.k;
+            if (more0) ask(c0);
+            multiply(c1);
+            if (!more0) break;
+        }
     }
-    if (wave != 0u) {
 #pragma unroll
-        for (int i = 0; i < FA; ++i)
+    for (int i = 0; i < FA; ++i)
 #pragma unroll
-            for (int j = 0; j < FB; ++j) part[wave - 1u][i * FB + j][lane] = acc[i][j];
-    }
+        for (int j = 0; j < FB; ++j) part[wave][i * FB + j][lane] = acc[i][j];
     __syncthreads();
-    if (wave == 0u) {
+    // a lane holds four neighbours of a row of dst
 #pragma unroll
-        for (int i = 0; i < FA; ++i)
+    for (uint32_t f = 0; f < FA * FB; ++f)
+        if (f % W == wave) {
+            f32x4 v = part[0][f][lane];
 #pragma unroll
-            for (int j = 0; j < FB; ++j) {
-                f32x4 v = acc[i][j];
+            for (uint32_t w = 1; w < W; ++w) {
+                const f32x4 x = part[w][f][lane];
 #pragma unroll
-                for (int w = 0; w < 3; ++w) v += part[w][i * FB + j][lane];
-                const uint32_t col = n0 + 16u * j + (lane & 15u);
-#pragma unroll
-                for (uint32_t e = 0; e < 4u; ++e) {
-                    const uint32_t row = m0 + 16u * i + (lane >> 4) * 4u + e;
-                    if (row < a.m && col < a.n) put<DT>(a.dst, row * a.dst_stride + col, v[e]);
-                }
+                for (int e = 0; e < 4; ++e) v[e] += x[e];
             }
-    }
+            const uint32_t row = m0 + 16u * (f / FB) + (lane & 15u), col = n0 + 16u * (f % FB) + (lane >> 4) * 4u;
+            if (row < a.m) put4<DT>((uint8_t*)a.dst + row * a.dst_stride * ElemSize<DT>::v, col, a.n, v);
+        }
 }
 
 // ---- many rows: tiles through LDS ---------------------------------------------------------------------------------------
@@ -278,8 +334,55 @@ template <int N> __device__ __forceinline__ void behind_each(bool reads, bool lo
     }
 }
 
+// The results of a wavefront, 32 F x 32 F of them from (m0, n0) on, to dst.  Four neighbours of a row lie in a lane; by way of
+// LDS (32 KiB of the wavefront's own) they become runs of a row that a store instruction writes in one piece.  All copies have
+// arrived and all wavefronts are done with what they read when this begins.
+template <int DT, uint32_t F> __device__ __forceinline__ void store_results(const f32x16 (&acc)[F][F], lds_byte* mine, uint32_t lane, void* dst, uint64_t dst_stride, uint32_t m0, uint32_t n0, uint32_t rows, uint32_t cols)
+{
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    constexpr uint32_t ES = ElemSize<DT>::v, EDGE = 32u * F, PASS = EDGE * EDGE * ES > 32768u ? F / 2u : F; // fragments of rows at a time
+    constexpr uint32_t ROW = EDGE * ES, SWAP = (ROW / 16u < 32u ? ROW / 16u : 32u) - 1u;                     // bytes of a row; its chunks of 16 change places by row
+    constexpr uint32_t LANES = EDGE / 8u;                                                                    // that read a row
+#pragma unroll
+    for (uint32_t i0 = 0; i0 < F; i0 += PASS) {
+#pragma unroll
+        for (uint32_t i = 0; i < PASS; ++i)
+#pragma unroll
+            for (uint32_t j = 0; j < F; ++j)
+#pragma unroll
+                for (uint32_t q = 0; q < 4u; ++q) {
+                    const f32x16& v = acc[i0 + i][j];
+                    const uint32_t row = i * 32u + (lane & 31u), col = j * 32u + 8u * q + 4u * (lane >> 5); // of four results
+                    lds_byte* p = mine + row * ROW + (((col * ES / 16u) ^ (row & SWAP)) << 4) + col * ES % 16u;
+                    if (ES == 4u) *(lds_vec*)p = u32x4{f32_bits(v[4 * q]), f32_bits(v[4 * q + 1]), f32_bits(v[4 * q + 2]), f32_bits(v[4 * q + 3])};
+                    else {
+                        const float f[8] = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], 0.0f, 0.0f, 0.0f, 0.0f};
+                        const Raw8<DT> r = narrow8<DT>(f);
+                        *(lds_u64*)p = (uint64_t)r.w[1] << 32 | r.w[0];
+                    }
+                }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (uint32_t t = 0; t < PASS * 32u * LANES / 64u; ++t) {
+            const uint32_t row = t * (64u / LANES) + lane / LANES, col = (lane % LANES) * 8u;
+            Raw8<DT> r;
+#pragma unroll
+            for (uint32_t h = 0; h < Raw8<DT>::words / 4u; ++h) {
+                const u32x4 v = *(lds_vec*)(mine + row * ROW + (((col * ES / 16u + h) ^ (row & SWAP)) << 4));
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) r.w[4u * h + e] = v[e];
+            }
+            const uint32_t m = m0 + i0 * 32u + row;
+            if (m < rows) store8<DT>((uint8_t*)dst + m * dst_stride * ES, n0 + col, cols, r);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 // TAIL: rows end inside a block
-template <int DT, bool TAIL> __global__ __launch_bounds__(256) void k_mx_product_tile(const HgMxProduct a)
+template <int DT, bool TAIL, uint32_t N> __global__ __launch_bounds__(256) void k_mx_product_tile(const ProductArgs<N> a)
 {
     // four arrays, not one: the compiler then sees that the copies into one pair do not touch the pair that is read
     __shared__ __align__(1024) uint8_t a0[32768], b0[32768], a1[32768], b1[32768];
@@ -380,63 +483,161 @@ template <int DT, bool TAIL> __global__ __launch_bounds__(256) void k_mx_product
         STAGE(a0, b0, a1, b1, 1)
         STAGE(a1, b1, a0, b0, 0)
     }
-    // All copies have arrived, in this wavefront and in the others: the LDS is free for the results.  Four neighbours of
-    // a row lie in a lane; by way of LDS they become runs of a row that a store instruction writes in one piece.
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    constexpr uint32_t ES = ElemSize<DT>::v, PASS = ES == 4u ? 2u : 4u, CHUNKS = 128u * ES / 16u; // fragments of rows at a time; chunks of 16 bytes of a row
-    lds_byte* mine = (lds_byte*)(wave == 0u ? a0 : wave == 1u ? b0 : wave == 2u ? a1 : b1);
-#pragma unroll
-    for (uint32_t i0 = 0; i0 < 4u; i0 += PASS) {
-#pragma unroll
-        for (uint32_t i = 0; i < PASS; ++i)
-#pragma unroll
-            for (uint32_t j = 0; j < 4u; ++j)
-#pragma unroll
-                for (uint32_t q = 0; q < 4u; ++q) {
-                    const f32x16& v = acc[i0 + i][j];
-                    const uint32_t row = i * 32u + (lane & 31u), col = j * 32u + 8u * q + 4u * (lane >> 5); // of four results
-                    lds_byte* p = mine + row * 128u * ES + (((col * ES / 16u) ^ (row & (CHUNKS - 1u))) << 4) + col * ES % 16u;
-                    if (ES == 4u) *(lds_vec*)p = u32x4{f32_bits(v[4 * q]), f32_bits(v[4 * q + 1]), f32_bits(v[4 * q + 2]), f32_bits(v[4 * q + 3])};
-                    else {
-                        const float f[8] = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], 0.0f, 0.0f, 0.0f, 0.0f};
-                        const Raw8<DT> r = narrow8<DT>(f);
-                        *(lds_u64*)p = (uint64_t)r.w[1] << 32 | r.w[0];
-                    }
-                }
-        __builtin_amdgcn_wave_barrier();
-        // eight results a lane and step: 16 lanes to a row
-#pragma unroll
-        for (uint32_t t = 0; t < PASS * 8u; ++t) {
-            const uint32_t row = t * 4u + (lane >> 4), col = (lane & 15u) * 8u;
-            Raw8<DT> r;
-#pragma unroll
-            for (uint32_t h = 0; h < Raw8<DT>::words / 4u; ++h) {
-                const u32x4 v = *(lds_vec*)(mine + row * 128u * ES + (((col * ES / 16u + h) ^ (row & (CHUNKS - 1u))) << 4));
-#pragma unroll
-                for (uint32_t e = 0; e < 4u; ++e) r.w[4u * h + e] = v[e];
-            }
-            const uint32_t m = m0 + wm * 128u + i0 * 32u + row, n = n0 + wn * 128u + col;
-            if (m < a.m) store8<DT>((uint8_t*)a.dst + m * a.dst_stride * ES, n, a.n, r);
-        }
-        __builtin_amdgcn_wave_barrier();
-    }
+    store_results<DT, 4>(acc, (lds_byte*)(wave == 0u ? a0 : wave == 1u ? b0 : wave == 2u ? a1 : b1), lane, a.dst, a.dst_stride, m0 + wm * 128u, n0 + wn * 128u, a.m, a.n);
 }
 
-template <int DT> int launch(hipStream_t st, const HgMxProduct* a)
+// ---- fewer rows: smaller tiles, longer stages ---------------------------------------------------------------------------
+//
+// 64 F x 64 F results to a workgroup, 32 F x 32 F to a wavefront, and as many more columns to a stage of the same 64 KiB.  Such
+// launches are bound by how fast a CU gets its operands, so a stage is simply multiplied while the next one arrives.
+
+template <int DT, uint32_t F, bool TAIL, uint32_t N> __global__ __launch_bounds__(256) void k_mx_product_mid(const ProductArgs<N> a)
 {
-    const dim3 g(a->wgs), b(256);
+    __shared__ __align__(1024) uint8_t a0[32768], b0[32768], a1[32768], b1[32768];
+    __shared__ __align__(16) uint8_t scales[2][2][2048];
+    constexpr uint32_t ROWS = 64u * F, LONG = 32u / F, ROW = LONG * HCOMM_GFX_MX_BLOCK_BYTES; // rows of a tile; blocks and bytes of a row of a stage
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1u;
+    const uint32_t tiles_n = (a.n + ROWS - 1u) / ROWS;
+    const uint32_t tile = block_id(8u), tm = tile / tiles_n, tn = tile - tm * tiles_n, m0 = tm * ROWS, n0 = tn * ROWS;
+    const uint32_t blocks = (a.cols + HCOMM_GFX_MX_BLOCK - 1u) / HCOMM_GFX_MX_BLOCK, stages = (blocks + LONG - 1u) / LONG;
+    f32x16 acc[F][F];
+#pragma unroll
+    for (uint32_t i = 0; i < F; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < F; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    // the ranks' matrices have the same strides (the host sees to it)
+    const uint32_t last_a = min(a.m - m0, ROWS) - 1u, last_b = min(a.n - n0, ROWS) - 1u;
+    const uint32_t stride_a = (uint32_t)a.a[0].packed_stride, stride_b = (uint32_t)a.b[0].packed_stride;
+    // what this lane copies in every one of its wavefront's eight copies: place lane % LONG of row lane / LONG behind the copy's first
+    const uint32_t copy_row = wave * 8u * (2u * F) + lane / LONG, place = lane % LONG;
+    // and the 16 scales that it fetches: the first 128 threads of a's rows, the others of b's
+    const uint32_t half = threadIdx.x >> 7, scale_row = (threadIdx.x & 127u) / (LONG / 16u), scale_part = (threadIdx.x & 127u) % (LONG / 16u) * 16u;
+    const uint32_t scale_at = min(scale_row, half ? last_b : last_a) * (uint32_t)(half ? a.b[0].scale_stride : a.a[0].scale_stride);
+    u32x4 fetched;
+    uint32_t back; // bytes that the fetch went back
+    auto copy = [&](lds_byte* to, const HgMxView& v, uint32_t row0, uint32_t last, uint32_t stride, uint32_t first) {
+        const __amdgpu_buffer_rsrc_t r =
+            __builtin_amdgcn_make_buffer_rsrc(v.packed + (uint64_t)row0 * v.packed_stride, 0, (int)(last * stride + blocks * HCOMM_GFX_MX_BLOCK_BYTES), HG_BUFFER_WORD3);
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) {
+            const uint32_t row = copy_row + i * 2u * F, block = min(first + ((place & ~7u) | ((place ^ row) & 7u)), blocks - 1u);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + (wave * 8u + i) * 1024u), 16,
+                                                     (int)(row * stride + block * HCOMM_GFX_MX_BLOCK_BYTES), 0, 0, 0);
+        }
+    };
+    auto ask = [&](lds_byte* to_a, lds_byte* to_b, uint32_t rank, uint32_t first) {
+        const HgMxView &va = a.a[rank], &vb = a.b[rank];
+        copy(to_a, va, m0, last_a, stride_a, first);
+        copy(to_b, vb, n0, last_b, stride_b, first);
+        const uint32_t want = first + scale_part, from = min(want, blocks - 16u); // the host takes this form from 16 blocks on
+        back = want - from;
+        const uint8_t* s = half ? vb.scales + (uint64_t)n0 * vb.scale_stride : va.scales + (uint64_t)m0 * va.scale_stride;
+        fetched = *(const __attribute__((address_space(1))) u32x4_at1*)(s + from + scale_at);
+    };
+    auto meet = [&](uint32_t set) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // scales past the rows' last block become 0, on both sides: the products are far below what fp32 holds
+        *(u32x4*)&scales[set][half][scale_row * LONG + scale_part] = down_by(fetched, back);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    const uint32_t r = lane & 31u, g = lane >> 5;
+    auto multiply = [&](lds_byte* la, lds_byte* lb, uint32_t set, uint32_t first) {
+#pragma unroll
+        for (uint32_t q = 0; q < LONG / 8u; ++q) {
+            uint64_t sa[F], sb[F];
+#pragma unroll
+            for (uint32_t i = 0; i < F; ++i) {
+                sa[i] = *(lds_u64*)(lds_byte*)&scales[set][0][(wm * 32u * F + i * 32u + r) * LONG + q * 8u];
+                sb[i] = *(lds_u64*)(lds_byte*)&scales[set][1][(wn * 32u * F + i * 32u + r) * LONG + q * 8u];
+            }
+#pragma unroll
+            for (uint32_t t = 0; t < 4u; ++t) {
+                const uint32_t at = r * ROW + (q * 8u + ((2u * t + g) ^ (r & 7u))) * 16u;
+                u32x4 x[F], y[F];
+#pragma unroll
+                for (uint32_t i = 0; i < F; ++i) {
+                    x[i] = *(lds_vec*)(la + (wm * 32u * F + i * 32u) * ROW + at);
+                    y[i] = *(lds_vec*)(lb + (wn * 32u * F + i * 32u) * ROW + at);
+                }
+                if (TAIL) { // elements of the last block past cols do not count, whatever it holds there
+                    const uint32_t n = first + q * 8u + 2u * t + g == blocks - 1u ? a.cols - (blocks - 1u) * HCOMM_GFX_MX_BLOCK : HCOMM_GFX_MX_BLOCK;
+#pragma unroll
+                    for (uint32_t w = 0; w < 4u; ++w) {
+                        const uint32_t keep = n > 8u * w ? n - 8u * w : 0u, mask = keep >= 8u ? 0xffffffffu : (1u << (4u * keep)) - 1u;
+#pragma unroll
+                        for (uint32_t i = 0; i < F; ++i) x[i][w] &= mask;
+                    }
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < F; ++i)
+#pragma unroll
+                    for (uint32_t j = 0; j < F; ++j)
+                        acc[i][j] = mfma32<0>(y[j], x[i], acc[i][j], (uint32_t)(sb[j] >> (16u * t + 8u * g)), (uint32_t)(sa[i] >> (16u * t + 8u * g)));
+            }
+        }
+    };
+    uint32_t rank = 0, first = 0; // of the stage that was asked for last
+    ask((lds_byte*)a0, (lds_byte*)b0, 0u, 0u);
+    for (uint32_t left = a.k * stages;;) {
+        meet(0);
+        uint32_t now = first;
+        if (--left) {
+            first = first + LONG < blocks ? first + LONG : (++rank, 0u);
+            ask((lds_byte*)a1, (lds_byte*)b1, rank, first);
+        }
+        multiply((lds_byte*)a0, (lds_byte*)b0, 0, now);
+        if (!left) break;
+        meet(1);
+        now = first;
+        if (--left) {
+            first = first + LONG < blocks ? first + LONG : (++rank, 0u);
+            ask((lds_byte*)a0, (lds_byte*)b0, rank, first);
+        }
+        multiply((lds_byte*)a1, (lds_byte*)b1, 1, now);
+        if (!left) break;
+    }
+    store_results<DT, F>(acc, (lds_byte*)(wave == 0u ? a0 : wave == 1u ? b0 : wave == 2u ? a1 : b1), lane, a.dst, a.dst_stride, m0 + wm * 32u * F, n0 + wn * 32u * F, a.m, a.n);
+}
+
+template <int DT, bool SHORT, uint32_t N> int launch(hipStream_t st, const HgMxProduct* a)
+{
+    ProductArgs<N> p;
+    for (uint32_t j = 0; j < N; ++j) p.a[j] = a->a[j], p.b[j] = a->b[j];
+    p.dst = a->dst, p.dst_stride = a->dst_stride, p.m = a->m, p.n = a->n, p.cols = a->cols, p.k = a->k;
+    const dim3 g(a->wgs);
     switch (a->form) {
-        case HG_PRODUCT_DIRECT_16: hipLaunchKernelGGL((k_mx_product_direct<DT, 1, 1>), g, b, 0, st, *a); break;
-        case HG_PRODUCT_DIRECT_32: hipLaunchKernelGGL((k_mx_product_direct<DT, 2, 2>), g, b, 0, st, *a); break;
+        case HG_PRODUCT_DIRECT_16: hipLaunchKernelGGL((k_mx_product_direct<DT, 1, 1, 8, SHORT, N>), g, dim3(512), 0, st, p); break;
+        case HG_PRODUCT_DIRECT_32: hipLaunchKernelGGL((k_mx_product_direct<DT, 2, 2, 8, SHORT, N>), g, dim3(512), 0, st, p); break;
+        case HG_PRODUCT_MID_64:
+            if (a->cols % HCOMM_GFX_MX_BLOCK) hipLaunchKernelGGL((k_mx_product_mid<DT, 1, true, N>), g, dim3(256), 0, st, p);
+            else hipLaunchKernelGGL((k_mx_product_mid<DT, 1, false, N>), g, dim3(256), 0, st, p);
+            break;
+        case HG_PRODUCT_MID_128:
+            if (a->cols % HCOMM_GFX_MX_BLOCK) hipLaunchKernelGGL((k_mx_product_mid<DT, 2, true, N>), g, dim3(256), 0, st, p);
+            else hipLaunchKernelGGL((k_mx_product_mid<DT, 2, false, N>), g, dim3(256), 0, st, p);
+            break;
         case HG_PRODUCT_TILE:
-            if (a->cols % HCOMM_GFX_MX_BLOCK) hipLaunchKernelGGL((k_mx_product_tile<DT, true>), g, b, 0, st, *a);
-            else hipLaunchKernelGGL((k_mx_product_tile<DT, false>), g, b, 0, st, *a);
+            if (a->cols % HCOMM_GFX_MX_BLOCK) hipLaunchKernelGGL((k_mx_product_tile<DT, true, N>), g, dim3(256), 0, st, p);
+            else hipLaunchKernelGGL((k_mx_product_tile<DT, false, N>), g, dim3(256), 0, st, p);
             break;
         default: return HCCL_E_INTERNAL;
     }
     return rc(hipGetLastError());
+}
+
+template <int DT, uint32_t N> int launch_length(hipStream_t st, const HgMxProduct* a)
+{
+    return a->cols <= HCOMM_GFX_MX_BLOCK * (CHUNK_BLOCKS - 1u) ? launch<DT, true, N>(st, a) : launch<DT, false, N>(st, a);
+}
+
+template <int DT> int launch_ranks(hipStream_t st, const HgMxProduct* a)
+{
+    if (a->k == 1u) return launch_length<DT, 1>(st, a);
+    return a->k <= 8u ? launch_length<DT, 8>(st, a) : launch_length<DT, HCOMM_GFX_MAX_RANKS>(st, a);
 }
 
 } // namespace
@@ -449,9 +650,9 @@ int hg_launch_mx_product(void* stream, const void* args)
     OnDeviceOf device((hipStream_t)stream);
     if (device.err != hipSuccess) return HCCL_E_RUNTIME;
     switch (a->dtype) {
-        case DT_F16: return launch<DT_F16>((hipStream_t)stream, a);
-        case DT_BF16: return launch<DT_BF16>((hipStream_t)stream, a);
-        case DT_F32: return launch<DT_F32>((hipStream_t)stream, a);
+        case DT_F16: return launch_ranks<DT_F16>((hipStream_t)stream, a);
+        case DT_BF16: return launch_ranks<DT_BF16>((hipStream_t)stream, a);
+        case DT_F32: return launch_ranks<DT_F32>((hipStream_t)stream, a);
         default: return HCCL_E_PARA;
     }
 }

@@ -3,6 +3,7 @@
  * checked here: strides that hold a row, ranges whose ends do not wrap, counts that fit the grid.
  */
 #include <string.h>
+#include <stdlib.h>
 
 #include "hg_host.h"
 #include "hg_ops.h"
@@ -99,8 +100,8 @@ static int mx_view(HgMxView* v, Range* packed, Range* scales, const HcommGfxMxVi
     const uint64_t blocks = mx_blocks(cols);
     v->packed = (uint8_t*)in->packed;
     v->scales = (uint8_t*)in->scales;
-    v->packed_stride = in->packedStride;
-    v->scale_stride = in->scaleStride;
+    v->packed_stride = rows > 1 ? in->packedStride : blocks * HCOMM_GFX_MX_BLOCK_BYTES; /* a single row has no next one */
+    v->scale_stride = rows > 1 ? in->scaleStride : blocks;
     if ((uintptr_t)in->packed % HCOMM_GFX_MX_BLOCK_BYTES != 0) return 0;
     if (rows > 1 && in->packedStride % HCOMM_GFX_MX_BLOCK_BYTES != 0) return 0;
     return range_of(packed, in->packed, rows, blocks * HCOMM_GFX_MX_BLOCK_BYTES, in->packedStride) &&
@@ -217,14 +218,25 @@ int32_t HcommGfxMxReduceKOnThread(
 
 /* ---- product --------------------------------------------------------------------------------------------------------- */
 
+static int env_form(void) { const char* e = getenv("HG_FORM"); return e ? atoi(e) : -1; }
+/* what the tile form asks for: a whole stage of columns, and ranks whose matrices have the same strides */
+static int product_tiles(const HgMxProduct* a)
+{
+    if (mx_blocks(a->cols) < 16u) return 0;
+    for (uint32_t j = 1; j < a->k; ++j)
+        if (a->a[j].packed_stride != a->a[0].packed_stride || a->a[j].scale_stride != a->a[0].scale_stride ||
+            a->b[j].packed_stride != a->b[0].packed_stride || a->b[j].scale_stride != a->b[0].scale_stride)
+            return 0;
+    return 1;
+}
+
 static void product_form(HgMxProduct* a)
 {
-    uint32_t edge = a->m <= 16u ? 16u : 32u;
-    a->form = edge == 16u ? HG_PRODUCT_DIRECT_16 : HG_PRODUCT_DIRECT_32;
-    if (a->m > 256u && a->n > 256u) {
-        a->form = HG_PRODUCT_TILE;
-        edge = 256u;
-    }
+    static const uint32_t edges[] = {16u, 32u, 64u, 128u, 256u};
+    a->form = a->m <= 16u ? HG_PRODUCT_DIRECT_16 : HG_PRODUCT_DIRECT_32;
+    if (a->m > 256u && a->n > 256u && product_tiles(a)) a->form = HG_PRODUCT_TILE;
+    if (env_form() >= 0 && (env_form() < 2 || product_tiles(a))) a->form = env_form();
+    const uint32_t edge = edges[a->form];
     a->wgs = (a->m + edge - 1u) / edge * ((a->n + edge - 1u) / edge);
 }
 

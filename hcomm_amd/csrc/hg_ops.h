@@ -54,7 +54,7 @@ typedef struct {
     int dtype;
 } HgMxReduce;
 
-enum { HG_PRODUCT_DIRECT_16 = 0, HG_PRODUCT_DIRECT_32 = 1, HG_PRODUCT_TILE = 2 }; /* results of a workgroup: 16 x 16, 32 x 32, 256 x 256 */
+enum { HG_PRODUCT_DIRECT_16 = 0, HG_PRODUCT_DIRECT_32, HG_PRODUCT_MID_64, HG_PRODUCT_MID_128, HG_PRODUCT_TILE }; /* edge of a workgroup's results: 16, 32, 64, 128, 256 */
 
 typedef struct {
     HgMxView a[HCOMM_GFX_MAX_RANKS];

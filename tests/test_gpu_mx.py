@@ -318,3 +318,20 @@ def test_ends_of_rows(gpu_thread, t):
         assert np.array_equal(out.scale(), scale) and np.array_equal(out.code(), code), cols
         close(total.double(), src.double() + ref.mx_values(code, scale, cols), t, 0.0, cols)
         assert out.guards_hold() and total.guards_hold()
+
+
+@pytest.mark.parametrize("m,n,cols,k", [(70, 90, 480, 2), (70, 90, 481, 1), (70, 200, 1009, 3), (130, 140, 2080, 2), (300, 400, 500, 3), (400, 300, 2049, 2)])
+def test_product_of_ranks_with_strides_of_their_own(gpu_thread, m, n, cols, k):
+    """Every rank's matrices padded by another number of blocks, then the same sizes with equal strides."""
+    rng = np.random.default_rng(m + n + cols)
+    for pads in ([0] * k, list(range(k))):
+        a = [random_mx(m, cols, rng, p, p, unit=120, tail=0x5) for p in pads]
+        b = [random_mx(n, cols, rng, 2 * p, p, unit=118, tail=0xD) for p in pads]
+        dst = Dense(m, n, "fp32", n + 1, 1)
+        ready()
+        h.check(h.HcommGfxMxProductKOnThread(gpu_thread, dst.ptr, n + 1, DT["fp32"], h.mx_views([x.item for x in a]), h.mx_views([x.item for x in b]), k, m, n, cols))
+        sync(gpu_thread)
+        want = sum(x.values() @ y.values().T for x, y in zip(a, b))
+        magnitude = sum(np.abs(x.values()) @ np.abs(y.values()).T for x, y in zip(a, b))
+        close(dst.double(), want, "fp32", k * cols * 2.0 ** -23 * magnitude, "dst")
+        assert dst.guards_hold()
