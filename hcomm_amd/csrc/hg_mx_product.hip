@@ -22,6 +22,18 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 acc, uint32_t sa, 
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, MX_FP4, MX_FP4, 0, (int)sa, 0, (int)sb);
 }
 
+// the words of a block of which the first n elements count
+__device__ __forceinline__ u32x4 kept(uint32_t n)
+{
+    u32x4 m;
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) {
+        const uint32_t keep = n > 8u * i ? n - 8u * i : 0u;
+        m[i] = keep >= 8u ? 0xffffffffu : (1u << (4u * keep)) - 1u;
+    }
+    return m;
+}
+
 // What a lane holds of one row for one chunk of 16 blocks: of every four neighbours its own (the four lanes of a row read 64
 // bytes in one piece then), and the chunk's scales, of which instruction t takes byte lane / 16 of word t.
 struct Run {
@@ -81,14 +93,12 @@ template <bool SHORT> __device__ __forceinline__ void settle_run(Run& r, uint32_
         const uint32_t by = first - min(first, blocks - CHUNK_BLOCKS); // bytes that the fetch went back
         r.scales = down_by(r.scales, by);
     }
-    const uint32_t last = blocks - 1u, n = cols - last * HCOMM_GFX_MX_BLOCK; // n elements of it count
+    const uint32_t last = blocks - 1u;
+    const u32x4 mask = kept(cols - last * HCOMM_GFX_MX_BLOCK);
 #pragma unroll
     for (uint32_t t = 0; t < 4u; ++t)
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
-            const uint32_t keep = n > 8u * i ? n - 8u * i : 0u, mask = keep >= 8u ? 0xffffffffu : (1u << (4u * keep)) - 1u;
-            r.block[t][i] &= first + 4u * t + g == last ? mask : 0xffffffffu;
-        }
+        for (uint32_t i = 0; i < 4u; ++i) r.block[t][i] &= first + 4u * t + g == last ? mask[i] : 0xffffffffu;
 }
 
 // four neighbours of a row of dst
@@ -275,13 +285,7 @@ __device__ __forceinline__ uint64_t fetch_scales(const Side& s, const HgMxView& 
 __device__ __forceinline__ void cut_rows(lds_byte* la, uint32_t block, uint32_t n)
 {
     lds_vec* p = (lds_vec*)(la + threadIdx.x * 128u + ((block ^ (threadIdx.x & 7u)) << 4));
-    u32x4 v = *p;
-#pragma unroll
-    for (uint32_t q = 0; q < 4u; ++q) {
-        const uint32_t keep = n > 8u * q ? n - 8u * q : 0u;
-        v[q] &= keep >= 8u ? 0xffffffffu : (1u << (4u * keep)) - 1u;
-    }
-    *p = v;
+    *p = *p & kept(n);
 }
 
 // what a wavefront multiplies: four fragments of 32 rows and 64 columns of each operand
@@ -486,20 +490,22 @@ template <int DT, bool TAIL, uint32_t N> __global__ __launch_bounds__(256) void 
     store_results<DT, 4>(acc, (lds_byte*)(wave == 0u ? a0 : wave == 1u ? b0 : wave == 2u ? a1 : b1), lane, a.dst, a.dst_stride, m0 + wm * 128u, n0 + wn * 128u, a.m, a.n);
 }
 
-// ---- fewer rows: smaller tiles, longer stages ---------------------------------------------------------------------------
+// ---- fewer rows: smaller tiles, more stages under way -------------------------------------------------------------------
 //
-// 64 F x 64 F results to a workgroup, 32 F x 32 F to a wavefront, and as many more columns to a stage of the same 64 KiB.  Such
-// launches are bound by how fast a CU gets its operands, so a stage is simply multiplied while the next one arrives.
+// 64 F x 64 F results to a workgroup, 32 F x 32 F to a wavefront, stages of 32 KiB.  Such launches are bound by how fast a CU
+// gets its operands, so of four buffers three are filled while the fourth is multiplied.
 
 template <int DT, uint32_t F, bool TAIL, uint32_t N> __global__ __launch_bounds__(256) void k_mx_product_mid(const ProductArgs<N> a)
 {
-    __shared__ __align__(1024) uint8_t a0[32768], b0[32768], a1[32768], b1[32768];
-    __shared__ __align__(16) uint8_t scales[2][2][2048];
-    constexpr uint32_t ROWS = 64u * F, LONG = 32u / F, ROW = LONG * HCOMM_GFX_MX_BLOCK_BYTES; // rows of a tile; blocks and bytes of a row of a stage
+    // an array to a stage: the compiler then sees that the copies into one do not touch the one that is read
+    __shared__ __align__(1024) uint8_t s0[32768], s1[32768], s2[32768], s3[32768];
+    __shared__ __align__(16) uint8_t scales[4][2][1024];
+    constexpr uint32_t ROWS = 64u * F, LONG = 16u / F, ROW = LONG * HCOMM_GFX_MX_BLOCK_BYTES; // rows of a tile; blocks and bytes of a row of a stage
+    constexpr uint32_t HALF = 16384u;                                                        // of a buffer: a's rows, then b's
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1u;
     const uint32_t tiles_n = (a.n + ROWS - 1u) / ROWS;
     const uint32_t tile = block_id(8u), tm = tile / tiles_n, tn = tile - tm * tiles_n, m0 = tm * ROWS, n0 = tn * ROWS;
-    const uint32_t blocks = (a.cols + HCOMM_GFX_MX_BLOCK - 1u) / HCOMM_GFX_MX_BLOCK, stages = (blocks + LONG - 1u) / LONG;
+    const uint32_t blocks = (a.cols + HCOMM_GFX_MX_BLOCK - 1u) / HCOMM_GFX_MX_BLOCK, total = a.k * ((blocks + LONG - 1u) / LONG);
     f32x16 acc[F][F];
 #pragma unroll
     for (uint32_t i = 0; i < F; ++i)
@@ -510,42 +516,58 @@ template <int DT, uint32_t F, bool TAIL, uint32_t N> __global__ __launch_bounds_
     // the ranks' matrices have the same strides (the host sees to it)
     const uint32_t last_a = min(a.m - m0, ROWS) - 1u, last_b = min(a.n - n0, ROWS) - 1u;
     const uint32_t stride_a = (uint32_t)a.a[0].packed_stride, stride_b = (uint32_t)a.b[0].packed_stride;
-    // what this lane copies in every one of its wavefront's eight copies: place lane % LONG of row lane / LONG behind the copy's first
-    const uint32_t copy_row = wave * 8u * (2u * F) + lane / LONG, place = lane % LONG;
-    // and the 16 scales that it fetches: the first 128 threads of a's rows, the others of b's
-    const uint32_t half = threadIdx.x >> 7, scale_row = (threadIdx.x & 127u) / (LONG / 16u), scale_part = (threadIdx.x & 127u) % (LONG / 16u) * 16u;
+    // what this lane copies in each of its wavefront's four copies of a side: place lane % LONG of row lane / LONG behind the copy's first
+    const uint32_t copy_row = wave * 4u * (4u * F) + lane / LONG, place = lane % LONG;
+    // and the eight scales that it fetches: the first two wavefronts of a's rows, the others of b's
+    const uint32_t half = wave >> 1, scale_row = (threadIdx.x & 127u) / (LONG / 8u), scale_part = (threadIdx.x & 127u) % (LONG / 8u) * 8u;
     const uint32_t scale_at = min(scale_row, half ? last_b : last_a) * (uint32_t)(half ? a.b[0].scale_stride : a.a[0].scale_stride);
-    u32x4 fetched;
-    uint32_t back; // bytes that the fetch went back
+    struct Stage {
+        uint64_t fetched;
+        uint32_t back, first; // how many scales the fetch went back; the stage's first block
+    } q0, q1, q2, q3;
     auto copy = [&](lds_byte* to, const HgMxView& v, uint32_t row0, uint32_t last, uint32_t stride, uint32_t first) {
         const __amdgpu_buffer_rsrc_t r =
             __builtin_amdgcn_make_buffer_rsrc(v.packed + (uint64_t)row0 * v.packed_stride, 0, (int)(last * stride + blocks * HCOMM_GFX_MX_BLOCK_BYTES), HG_BUFFER_WORD3);
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) {
-            const uint32_t row = copy_row + i * 2u * F, block = min(first + ((place & ~7u) | ((place ^ row) & 7u)), blocks - 1u);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + (wave * 8u + i) * 1024u), 16,
+        for (uint32_t i = 0; i < 4u; ++i) {
+            const uint32_t row = copy_row + i * 4u * F, block = min(first + ((place & ~7u) | ((place ^ row) & 7u)), blocks - 1u);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + (wave * 4u + i) * 1024u), 16,
                                                      (int)(row * stride + block * HCOMM_GFX_MX_BLOCK_BYTES), 0, 0, 0);
         }
     };
-    auto ask = [&](lds_byte* to_a, lds_byte* to_b, uint32_t rank, uint32_t first) {
+    uint32_t rank = 0, first = 0; // of the next stage to ask for; behind the last one that stage again and again, so that what is under way can be counted
+    auto ask = [&](lds_byte* to, Stage& q) {
         const HgMxView &va = a.a[rank], &vb = a.b[rank];
-        copy(to_a, va, m0, last_a, stride_a, first);
-        copy(to_b, vb, n0, last_b, stride_b, first);
-        const uint32_t want = first + scale_part, from = min(want, blocks - 16u); // the host takes this form from 16 blocks on
-        back = want - from;
+        copy(to, va, m0, last_a, stride_a, first);
+        copy(to + HALF, vb, n0, last_b, stride_b, first);
+        const uint32_t want = first + scale_part, from = min(want, blocks - 8u); // the host takes this form from 8 blocks on
         const uint8_t* s = half ? vb.scales + (uint64_t)n0 * vb.scale_stride : va.scales + (uint64_t)m0 * va.scale_stride;
-        fetched = *(const __attribute__((address_space(1))) u32x4_at1*)(s + from + scale_at);
+        q.fetched = *(const __attribute__((address_space(1))) u64_at1*)(s + from + scale_at);
+        q.back = want - from;
+        q.first = first;
+        const bool ends = first + LONG >= blocks, more = rank + 1u < a.k;
+        first = ends ? (more ? 0u : first) : first + LONG;
+        rank = ends && more ? rank + 1u : rank;
     };
-    auto meet = [&](uint32_t set) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // The oldest stage asked for has arrived: what is under way is at most the two stages asked for after it, nine loads each.
+    uint32_t done = 0;
+    auto meet = [&](lds_byte* in, uint32_t set, const Stage& q) {
+        asm volatile("s_waitcnt vmcnt(18)" ::: "memory");
+        if (TAIL && lane < 16u * F) { // elements of the last block past cols do not count: they become 0 in the rows of a that this wavefront has copied
+            const uint32_t last = blocks - 1u - q.first, row = wave * 16u * F + lane; // last: the block in its stage, if it is there
+            const uint32_t n = last < LONG ? a.cols - (blocks - 1u) * HCOMM_GFX_MX_BLOCK : HCOMM_GFX_MX_BLOCK, at = last < LONG ? last : 0u;
+            lds_vec* p = (lds_vec*)(in + row * ROW + ((at & ~7u) | ((at ^ row) & 7u)) * HCOMM_GFX_MX_BLOCK_BYTES);
+            *p = *p & kept(n);
+        }
         // scales past the rows' last block become 0, on both sides: the products are far below what fp32 holds
-        *(u32x4*)&scales[set][half][scale_row * LONG + scale_part] = down_by(fetched, back);
+        *(lds_u64*)(lds_byte*)&scales[set][half][scale_row * LONG + scale_part] = q.back < 8u ? q.fetched >> (8u * q.back) : 0u;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        ++done;
     };
     const uint32_t r = lane & 31u, g = lane >> 5;
-    auto multiply = [&](lds_byte* la, lds_byte* lb, uint32_t set, uint32_t first) {
+    auto multiply = [&](lds_byte* from, uint32_t set) {
 #pragma unroll
         for (uint32_t q = 0; q < LONG / 8u; ++q) {
             uint64_t sa[F], sb[F];
@@ -560,17 +582,8 @@ template <int DT, uint32_t F, bool TAIL, uint32_t N> __global__ __launch_bounds_
                 u32x4 x[F], y[F];
 #pragma unroll
                 for (uint32_t i = 0; i < F; ++i) {
-                    x[i] = *(lds_vec*)(la + (wm * 32u * F + i * 32u) * ROW + at);
-                    y[i] = *(lds_vec*)(lb + (wn * 32u * F + i * 32u) * ROW + at);
-                }
-                if (TAIL) { // elements of the last block past cols do not count, whatever it holds there
-                    const uint32_t n = first + q * 8u + 2u * t + g == blocks - 1u ? a.cols - (blocks - 1u) * HCOMM_GFX_MX_BLOCK : HCOMM_GFX_MX_BLOCK;
-#pragma unroll
-                    for (uint32_t w = 0; w < 4u; ++w) {
-                        const uint32_t keep = n > 8u * w ? n - 8u * w : 0u, mask = keep >= 8u ? 0xffffffffu : (1u << (4u * keep)) - 1u;
-#pragma unroll
-                        for (uint32_t i = 0; i < F; ++i) x[i][w] &= mask;
-                    }
+                    x[i] = *(lds_vec*)(from + (wm * 32u * F + i * 32u) * ROW + at);
+                    y[i] = *(lds_vec*)(from + HALF + (wn * 32u * F + i * 32u) * ROW + at);
                 }
 #pragma unroll
                 for (uint32_t i = 0; i < F; ++i)
@@ -580,27 +593,30 @@ template <int DT, uint32_t F, bool TAIL, uint32_t N> __global__ __launch_bounds_
             }
         }
     };
-    uint32_t rank = 0, first = 0; // of the stage that was asked for last
-    ask((lds_byte*)a0, (lds_byte*)b0, 0u, 0u);
-    for (uint32_t left = a.k * stages;;) {
-        meet(0);
-        uint32_t now = first;
-        if (--left) {
-            first = first + LONG < blocks ? first + LONG : (++rank, 0u);
-            ask((lds_byte*)a1, (lds_byte*)b1, rank, first);
-        }
-        multiply((lds_byte*)a0, (lds_byte*)b0, 0, now);
-        if (!left) break;
-        meet(1);
-        now = first;
-        if (--left) {
-            first = first + LONG < blocks ? first + LONG : (++rank, 0u);
-            ask((lds_byte*)a0, (lds_byte*)b0, rank, first);
-        }
-        multiply((lds_byte*)a1, (lds_byte*)b1, 1, now);
-        if (!left) break;
+    ask((lds_byte*)s0, q0);
+    ask((lds_byte*)s1, q1);
+    ask((lds_byte*)s2, q2);
+    // the buffer of the stage before, which all wavefronts are done with when they have met, takes the third stage from here
+#pragma unroll 1
+    for (;;) {
+        meet((lds_byte*)s0, 0, q0);
+        ask((lds_byte*)s3, q3);
+        multiply((lds_byte*)s0, 0);
+        if (done == total) break;
+        meet((lds_byte*)s1, 1, q1);
+        ask((lds_byte*)s0, q0);
+        multiply((lds_byte*)s1, 1);
+        if (done == total) break;
+        meet((lds_byte*)s2, 2, q2);
+        ask((lds_byte*)s1, q1);
+        multiply((lds_byte*)s2, 2);
+        if (done == total) break;
+        meet((lds_byte*)s3, 3, q3);
+        ask((lds_byte*)s2, q2);
+        multiply((lds_byte*)s3, 3);
+        if (done == total) break;
     }
-    store_results<DT, F>(acc, (lds_byte*)(wave == 0u ? a0 : wave == 1u ? b0 : wave == 2u ? a1 : b1), lane, a.dst, a.dst_stride, m0 + wm * 32u * F, n0 + wn * 32u * F, a.m, a.n);
+    store_results<DT, F>(acc, (lds_byte*)(wave == 0u ? s0 : wave == 1u ? s1 : wave == 2u ? s2 : s3), lane, a.dst, a.dst_stride, m0 + wm * 32u * F, n0 + wn * 32u * F, a.m, a.n);
 }
 
 template <int DT, bool SHORT, uint32_t N> int launch(hipStream_t st, const HgMxProduct* a)

@@ -3,7 +3,6 @@
  * checked here: strides that hold a row, ranges whose ends do not wrap, counts that fit the grid.
  */
 #include <string.h>
-#include <stdlib.h>
 
 #include "hg_host.h"
 #include "hg_ops.h"
@@ -218,8 +217,8 @@ int32_t HcommGfxMxReduceKOnThread(
 
 /* ---- product --------------------------------------------------------------------------------------------------------- */
 
-static int env_form(void) { const char* e = getenv("HG_FORM"); return e ? atoi(e) : -1; }
-/* what the tile form asks for: a whole stage of columns, and ranks whose matrices have the same strides */
+/* what the forms through LDS ask for: a whole stage of columns (8 blocks; with fewer than 16 the direct forms are ahead anyway), and ranks
+ * whose matrices have the same strides */
 static int product_tiles(const HgMxProduct* a)
 {
     if (mx_blocks(a->cols) < 16u) return 0;
@@ -230,14 +229,33 @@ static int product_tiles(const HgMxProduct* a)
     return 1;
 }
 
+static uint32_t product_wgs(const HgMxProduct* a, uint32_t edge) { return (a->m + edge - 1u) / edge * ((a->n + edge - 1u) / edge); }
+
+/*
+ * The largest tiles of which there are enough for the CUs.  Measured, us for an inner length of 8,192 and n = 8,192 (edge 16 / 32 /
+ * 64 / 128 / 256): m = 16: 12.3 / 11.3 / 12.4 / 23 / 47, m = 64: 33 / 21 / 13 / 23 / 47, m = 256: 121 / 76 / 25.5 / 25.1 / 50,
+ * m = 512: 240 / 151 / 48 / 30 / 50, m = 1,024: 477 / 299 / 92 / 59 / 54, m = 4,096: 1,894 / 1,186 / 389 / 212 / 140; 200 x 200 x 512:
+ * 2.7 / 3.1 / 3.5 / 4.8 / 10.4, 300 x 300 x 4,096: 7.1 / 6.8 / 7.3 / 14 / 32.
+ */
 static void product_form(HgMxProduct* a)
 {
-    static const uint32_t edges[] = {16u, 32u, 64u, 128u, 256u};
-    a->form = a->m <= 16u ? HG_PRODUCT_DIRECT_16 : HG_PRODUCT_DIRECT_32;
-    if (a->m > 256u && a->n > 256u && product_tiles(a)) a->form = HG_PRODUCT_TILE;
-    if (env_form() >= 0 && (env_form() < 2 || product_tiles(a))) a->form = env_form();
-    const uint32_t edge = edges[a->form];
-    a->wgs = (a->m + edge - 1u) / edge * ((a->n + edge - 1u) / edge);
+    uint32_t edge = 16u;
+    a->form = HG_PRODUCT_DIRECT_16;
+    const int tiles = product_tiles(a);
+    if (tiles && product_wgs(a, 256u) >= 128u) {
+        edge = 256u;
+        a->form = HG_PRODUCT_TILE;
+    } else if (tiles && product_wgs(a, 128u) >= 128u) {
+        edge = 128u;
+        a->form = HG_PRODUCT_MID_128;
+    } else if (tiles && a->m > 32u && a->n > 32u && product_wgs(a, 64u) >= 64u) {
+        edge = 64u;
+        a->form = HG_PRODUCT_MID_64;
+    } else if (a->m > 16u && a->n > 16u && product_wgs(a, 32u) >= 64u) {
+        edge = 32u;
+        a->form = HG_PRODUCT_DIRECT_32;
+    }
+    a->wgs = product_wgs(a, edge);
 }
 
 int32_t HcommGfxMxProductKOnThread(
