@@ -33,15 +33,29 @@ __device__ __forceinline__ float wave_sum(float v)
     return (a + b) + (c + d);
 }
 
-// N sums over the at most 16 wavefronts of a row, the same in all of them: lane w of every 16 fetches wavefront w's.  `box`
-// holds N floats for each wavefront of the workgroup and is not written again before every wavefront has passed another
-// barrier.
-template <uint32_t N> __device__ __forceinline__ void row_sum(float (&v)[N], float* box, uint32_t waves)
+// What a workgroup has: one row, several of whole wavefronts (1 or 2 each), or several of 8, 16 or 32 lanes.
+enum { ONE_ROW, WAVES, LANES };
+
+// N sums over the `span` lanes that share a row, the same in all of them.  Across wavefronts, at most 16: lane w of every 16 fetches wavefront w's sum from `box`, which holds N floats for each wavefront of
+// the workgroup and is not written again before every wavefront has passed another barrier.
+template <uint32_t N, int SHARE> __device__ __forceinline__ void row_sum(float (&v)[N], float* box, uint32_t span)
 {
+    if (SHARE == LANES) {
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) {
+            v[i] = plus_dpp<0xB1>(v[i]);
+            v[i] = plus_dpp<0x4E>(v[i]);
+            v[i] = plus_dpp<0x141>(v[i]);
+            if (span >= 16u) v[i] = plus_dpp<0x140>(v[i]);
+            if (span >= 32u) v[i] += __shfl_xor(v[i], 16);
+        }
+        return;
+    }
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+    const uint32_t waves = span / 64u;
     if (waves == 1u) return;
-    const uint32_t wave = threadIdx.x >> 6, first = wave & ~(waves - 1u), w = threadIdx.x & 15u; // the host makes `waves` a power of two
+    const uint32_t wave = threadIdx.x >> 6, first = SHARE == ONE_ROW ? 0u : wave & ~1u, w = threadIdx.x & 15u;
     if ((threadIdx.x & 63u) == 0u) {
 #pragma unroll
         for (uint32_t i = 0; i < N; ++i) box[wave * N + i] = v[i];
@@ -61,18 +75,19 @@ __device__ __forceinline__ float inverse_rms(float squares, uint64_t cols, float
 template <uint32_t N> struct NormArgs {
     HcommGfxReduceNormDesc d;
     const void* src[N];
-    uint32_t waves, rows_per_wg;
+    uint32_t span, rows_per_wg;
 };
 
-// DT: type of the matrices, PT: of the parameters, V: groups of eight elements a lane holds, ONE: a workgroup has one row
-// (then where it begins is a scalar), TAIL: rows end inside a group, NT: larger than the L2s, so that what is read once and
+// DT: type of the matrices, PT: of the parameters, V: groups of eight elements a lane holds, SHARE: a workgroup has one row
+// (where it begins is a scalar then), several of whole wavefronts, or several of fewer lanes, TAIL: rows end inside a group, NT: larger than the L2s, so that what is read once and
 // what is written passes by them (8,192 x 4,096 of eight ranks 153 -> 138 us; rows off 16-byte boundaries share lines, which
 // has to be fetched again then), N: most ranks
-template <int DT, int PT, uint32_t V, bool ONE, bool TAIL, bool NT, uint32_t N> __global__ __launch_bounds__(1024) void k_norm(const NormArgs<N> a)
+template <int DT, int PT, uint32_t V, int SHARE, bool TAIL, bool NT, uint32_t N> __global__ __launch_bounds__(1024) void k_norm(const NormArgs<N> a)
 {
     __shared__ float box[2][MAX_WAVES];
     constexpr uint32_t ES = ElemSize<DT>::v, PS = ElemSize<PT>::v, AHEAD = (DT == DT_F32 ? 4u : 8u) / V;
-    const uint32_t span = a.waves * 64u, local = ONE ? 0u : threadIdx.x / span, t = threadIdx.x - local * span;
+    constexpr bool ONE = SHARE == ONE_ROW;
+    const uint32_t span = a.span, local = ONE ? 0u : threadIdx.x >> __builtin_ctz(span), t = threadIdx.x - local * span;
     const uint64_t row = ONE ? blockIdx.x : (uint64_t)blockIdx.x * a.rows_per_wg + local;
     const uint64_t cols = ONE || row < a.d.rows ? a.d.cols : 0u; // a row that is not there has no columns
     const bool tiny = a.d.cols < 8u;
@@ -137,7 +152,7 @@ template <int DT, int PT, uint32_t V, bool ONE, bool TAIL, bool NT, uint32_t N> 
         for (uint32_t v = 0; v < V; ++v)
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e) s[0] = fmaf(f[v][e], f[v][e], s[0]);
-        row_sum(s, box[0], a.waves);
+        row_sum<1, SHARE>(s, box[0], span);
         const float r = inverse_rms(s[0], a.d.cols, a.d.eps);
 #pragma unroll
         for (uint32_t v = 0; v < V; ++v) {
@@ -167,7 +182,7 @@ template <int DT, int PT, uint32_t V, bool ONE, bool TAIL, bool NT, uint32_t N> 
         store8<DT, TAIL, NT>((uint8_t*)a.d.y + row * a.d.yStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(f[v]));
     }
     if (a.d.preWeight) {
-        row_sum(s, box[1], a.waves);
+        row_sum<1, SHARE>(s, box[1], span);
         const float r = inverse_rms(s[0], a.d.cols, a.d.eps);
 #pragma unroll
         for (uint32_t v = 0; v < V; ++v) {
@@ -184,11 +199,24 @@ template <int DT, int PT, uint32_t V, bool ONE, bool TAIL, bool NT, uint32_t N> 
 
 // A run of rows to a workgroup: the parameters' gradients stay in registers over the run, and the row after the one at work
 // is on its way while the sums of this one cross the lanes.
-template <int DT, int PT, uint32_t V, uint32_t MOST, bool TAIL, bool NT> __global__ __launch_bounds__(MOST) void k_norm_grad(const HgNormGrad a)
+// SUB: rows of 8, 16 or 32 lanes, several to a wavefront, each taking every so many units of the run's rows (a unit: the rows
+// of one row of the gate where its gradient is written at once, else one row); their sums are joined at the run's end.
+// LEAN: rows too long for that many registers are read once more where they are needed again, out of the L2.
+//
+// Which of them, for 33.5M elements in bf16, us:
+//   SUB up to 256 columns: 99 at 64 columns, 419 with a wavefront to each row (56 of its lanes idle);
+//   V = 1 up to 4,096: 88 to 95, 4.5 TB/s of 5.1 that a copy reaches;
+//   V = 2 up to 8,192, 8 wavefronts of 256 registers, the second group's sums in LDS: 88 to 112 (fp32 195; 258 with these sums
+//   in registers that spill); LEAN with V = 1 and 16 wavefronts: 200;
+//   LEAN with V = 2 above: 228 to 255, 815 and more with everything held and spilled.  A row's loads are waited for three
+//   times there, with one workgroup to a CU: bound by their latency.
+template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool TAIL, bool NT> __global__ __launch_bounds__(MOST) void k_norm_grad(const HgNormGrad a)
 {
     __shared__ float box_a[MAX_WAVES * 3], box_b[MAX_WAVES];
     constexpr uint32_t ES = ElemSize<DT>::v, PS = ElemSize<PT>::v;
-    const uint32_t span = a.waves * 64u, t = threadIdx.x;
+    constexpr bool PASS = NT && !LEAN;
+    const uint32_t span = a.span;
+    uint32_t t = SUB ? threadIdx.x & (span - 1u) : threadIdx.x;
     const uint64_t cols = a.d.cols;
     const bool tiny = cols < 8u;
     const bool has_post = a.d.postWeight != nullptr, has_pre = a.d.preWeight != nullptr, has_gate = a.d.gate != nullptr;
@@ -202,158 +230,228 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool TAIL, bool NT> __globa
         row = blockIdx.x * (uint32_t)a.chunk_rows;
         end = min(row + (uint32_t)a.chunk_rows, (uint32_t)a.d.rows);
     }
+    const uint32_t sets = 64u >> __builtin_ctz(span), unit = a.unit; // of lanes; rows a set takes before it leaves out the other sets'
+    if (SUB) row += (threadIdx.x >> __builtin_ctz(span)) * unit;
+    uint32_t unit_end = SUB ? row + unit : 0u;
+    auto after = [&](uint32_t r) { return SUB && r + 1u == unit_end ? r + 1u + (sets - 1u) * unit : r + 1u; };
     struct Row {
-        Raw8<DT> s[V], y[V], dy[V], dz[V];
+        Raw8<DT> s, y, dy, dz;
     };
-    auto ask = [&](Row& x, uint32_t r) {
-#pragma unroll
-        for (uint32_t v = 0; v < V; ++v) {
-            const uint32_t at = (v * span + t) * 8u;
-            x.s[v] = ask8<DT, TAIL, NT>((const uint8_t*)a.d.sum + r * a.d.sumStride * ES, at, cols, tiny);
-            if (has_pre) {
-                x.y[v] = ask8<DT, TAIL, NT>((const uint8_t*)a.d.y + r * a.d.yStride * ES, at, cols, tiny);
-                x.dz[v] = ask8<DT, TAIL, NT>((const uint8_t*)a.d.dz + r * a.d.dzStride * ES, at, cols, tiny);
-            }
-            x.dy[v] = ask8<DT, TAIL, NT>((const uint8_t*)a.d.dy + r * a.d.dyStride * ES, at, cols, tiny);
+    constexpr uint32_t HELD = LEAN ? 1u : V; // groups whose rows and parameters stay in registers
+    auto ask_one = [&](const void* m, uint64_t stride, uint32_t r, uint32_t v) {
+        return ask8<DT, TAIL, PASS>((const uint8_t*)m + r * stride * ES, (v * span + t) * 8u, cols, tiny);
+    };
+    auto ask = [&](Row& x, uint32_t r, uint32_t v, bool with_dy) {
+        x.s = ask_one(a.d.sum, a.d.sumStride, r, v);
+        if (has_pre) x.y = ask_one(a.d.y, a.d.yStride, r, v), x.dz = ask_one(a.d.dz, a.d.dzStride, r, v);
+        if (with_dy) x.dy = ask_one(a.d.dy, a.d.dyStride, r, v);
+    };
+    auto settle = [&](Raw8<DT>& x, uint32_t v) { settle8<DT, TAIL>(x, (v * span + t) * 8u, cols, tiny); };
+    auto settle_row = [&](Row& x, uint32_t v, bool with_dy) {
+        settle(x.s, v);
+        if (has_pre) settle(x.y, v), settle(x.dz, v);
+        if (with_dy) settle(x.dy, v);
+    };
+    auto param = [&](const void* m, uint32_t v) {
+        Raw8<PT> p = ask8<PT, TAIL, false>(m, (v * span + t) * 8u, cols, tiny);
+        settle8<PT, TAIL>(p, (v * span + t) * 8u, cols, tiny);
+        return p;
+    };
+    // What a lane asks for behind this is not asked for before it: LEAN has room for little at a time.
+    auto apart = [] {
+        if (LEAN) {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    Row next;
-    if (row < end) ask(next, row);
-    Raw8<PT> post[V], pre[V], gate[V];
-    float d_post[V][8], d_pre[V][8], d_gate[V][8];
+    Row next[HELD];
+    auto ask_next = [&](uint32_t r) {
 #pragma unroll
-    for (uint32_t v = 0; v < V; ++v) {
-        if (has_pre) pre[v] = ask8<PT, TAIL, false>(a.d.preWeight, (v * span + t) * 8u, cols, tiny);
-        if (has_post) post[v] = ask8<PT, TAIL, false>(a.d.postWeight, (v * span + t) * 8u, cols, tiny);
+        for (uint32_t v = 0; v < HELD; ++v) ask(next[v], r, v, true);
+    };
+    if (!LEAN && row < end) ask_next(row);
+    Raw8<PT> post[HELD], pre[HELD], gate[HELD];
+    if (!LEAN) {
 #pragma unroll
-        for (uint32_t e = 0; e < 8u; ++e) d_post[v][e] = d_pre[v][e] = d_gate[v][e] = 0.0f;
+        for (uint32_t v = 0; v < HELD; ++v) {
+            if (has_pre) pre[v] = param(a.d.preWeight, v);
+            if (has_post) post[v] = param(a.d.postWeight, v);
+        }
     }
+    float d_post[8], d_pre[8], d_gate[8];
+#pragma unroll
+    for (uint32_t e = 0; e < 8u; ++e) d_post[e] = d_pre[e] = d_gate[e] = 0.0f;
+    // the second group's sums and results stay in LDS
+    enum { POST, PRE, GATE, RESULT };
+    __shared__ __align__(16) float4 second[V > 1u ? 4 : 1][2][V > 1u ? MOST : 1u];
+    auto keep = [&](int which, const float (&d)[8]) {
+        second[which][0][t] = make_float4(d[0], d[1], d[2], d[3]);
+        second[which][1][t] = make_float4(d[4], d[5], d[6], d[7]);
+    };
+    auto kept = [&](int which, float (&d)[8]) {
+        const float4 l = second[which][0][t], h = second[which][1][t];
+        d[0] = l.x, d[1] = l.y, d[2] = l.z, d[3] = l.w, d[4] = h.x, d[5] = h.y, d[6] = h.z, d[7] = h.w;
+    };
+    if (V > 1u) keep(POST, d_post), keep(PRE, d_pre), keep(GATE, d_gate);
     const float each = 1.0f / (float)cols;
     uint32_t gate_row = 0u, gate_end = 0u; // the row of the gate, and the row at which its next one begins
-    if (has_gate && row < end) {
-        gate_row = row / (uint32_t)a.d.rowsPerGate;
+    auto take_gate = [&](uint32_t r) {
+        gate_row = r / (uint32_t)a.d.rowsPerGate;
         gate_end = (gate_row + 1u) * (uint32_t)a.d.rowsPerGate;
+        if (!LEAN) {
 #pragma unroll
-        for (uint32_t v = 0; v < V; ++v) gate[v] = ask8<PT, TAIL, false>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols, tiny);
-    }
+            for (uint32_t v = 0; v < HELD; ++v) gate[v] = param((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, v);
+        }
+    };
+    if (has_gate && row < end) take_gate(row);
+    while (row < end) {
+        const uint32_t following = after(row);
+        if (LEAN) asm volatile("" : "+v"(t)); // no addresses held from row to row
+        Row x[HELD];
+        if (!LEAN) {
 #pragma unroll
-    for (uint32_t v = 0; v < V; ++v) {
-        const uint32_t at = (v * span + t) * 8u;
-        if (has_pre) settle8<PT, TAIL>(pre[v], at, cols, tiny);
-        if (has_post) settle8<PT, TAIL>(post[v], at, cols, tiny);
-        if (has_gate && row < end) settle8<PT, TAIL>(gate[v], at, cols, tiny);
-    }
-    for (; row < end; ++row) {
-        Row x = next;
-        if (row + 1u < end) ask(next, row + 1u);
+            for (uint32_t v = 0; v < HELD; ++v) x[v] = next[v];
+            if (following < end) ask_next(following);
 #pragma unroll
-        for (uint32_t v = 0; v < V; ++v) {
-            const uint32_t at = (v * span + t) * 8u;
-            settle8<DT, TAIL>(x.s[v], at, cols, tiny);
-            settle8<DT, TAIL>(x.dy[v], at, cols, tiny);
-            if (has_pre) settle8<DT, TAIL>(x.y[v], at, cols, tiny), settle8<DT, TAIL>(x.dz[v], at, cols, tiny);
+            for (uint32_t v = 0; v < HELD; ++v) settle_row(x[v], v, true);
         }
         float q[3] = {0.0f, 0.0f, 0.0f}; // sum^2, y^2, dz preWeight y
 #pragma unroll
         for (uint32_t v = 0; v < V; ++v) {
+            Row& h = x[LEAN ? 0u : v];
+            if (LEAN) ask(h, row, v, false), settle_row(h, v, false);
             float s[8];
-            widen8<DT>(x.s[v], s);
+            widen8<DT>(h.s, s);
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e) q[0] = fmaf(s[e], s[e], q[0]);
             if (has_pre) {
                 float y[8], z[8], w[8];
-                widen8<DT>(x.y[v], y);
-                widen8<DT>(x.dz[v], z);
-                widen8<PT>(pre[v], w);
+                widen8<DT>(h.y, y);
+                widen8<DT>(h.dz, z);
+                widen8<PT>(LEAN ? param(a.d.preWeight, v) : pre[LEAN ? 0u : v], w);
 #pragma unroll
                 for (uint32_t e = 0; e < 8u; ++e) q[1] = fmaf(y[e], y[e], q[1]), q[2] = fmaf(z[e] * w[e], y[e], q[2]);
             }
         }
-        row_sum(q, box_a, a.waves);
+        row_sum<3, SUB ? LANES : ONE_ROW>(q, box_a, span);
         const float r1 = inverse_rms(q[0], cols, a.d.eps), r2 = has_pre ? inverse_rms(q[1], cols, a.d.eps) : 0.0f;
         const float c2 = r2 * (q[2] * each); // mean of dz preWeight y / rms(y): r2 alone never underflows, its powers do
-        float g1[V][8]; // g D postWeight, or g D
         float p[1] = {0.0f};
-#pragma unroll
-        for (uint32_t v = 0; v < V; ++v) {
+        // adds to the parameters' gradients and to p; o: g D postWeight, or g D
+        auto group = [&](uint32_t v, float (&to_post)[8], float (&to_pre)[8], float (&to_gate)[8], float (&o)[8]) {
+            apart();
+            Row& h = x[LEAN ? 0u : v];
+            if (LEAN) ask(h, row, v, true), settle_row(h, v, true);
             float s[8], d[8];
-            widen8<DT>(x.s[v], s);
-            widen8<DT>(x.dy[v], d);
+            widen8<DT>(h.s, s);
+            widen8<DT>(h.dy, d);
             if (has_pre) {
                 float y[8], z[8], w[8];
-                widen8<DT>(x.y[v], y);
-                widen8<DT>(x.dz[v], z);
-                widen8<PT>(pre[v], w);
+                widen8<DT>(h.y, y);
+                widen8<DT>(h.dz, z);
+                widen8<PT>(LEAN ? param(a.d.preWeight, v) : pre[LEAN ? 0u : v], w);
 #pragma unroll
                 for (uint32_t e = 0; e < 8u; ++e) {
                     const float n = y[e] * r2;
-                    d_pre[v][e] = fmaf(z[e], n, d_pre[v][e]);
+                    to_pre[e] = fmaf(z[e], n, to_pre[e]);
                     d[e] = fmaf(r2, fmaf(z[e], w[e], -c2 * n), d[e]);
                 }
             }
             if (a.d.dResidual) {
-                float o[8];
+                float res[8];
 #pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e) o[e] = a.d.residualScale * d[e];
-                store8<DT, TAIL, NT>((uint8_t*)a.d.dResidual + row * a.d.dResidualStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(o));
+                for (uint32_t e = 0; e < 8u; ++e) res[e] = a.d.residualScale * d[e];
+                store8<DT, TAIL, NT>((uint8_t*)a.d.dResidual + row * a.d.dResidualStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(res));
             }
-            float w1[8], g[8];
-            if (has_post) widen8<PT>(post[v], w1);
-            if (has_gate) widen8<PT>(gate[v], g);
+            float w[8], g[8];
+            if (has_post) widen8<PT>(LEAN ? param(a.d.postWeight, v) : post[LEAN ? 0u : v], w);
+            if (has_gate) widen8<PT>(LEAN ? param((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, v) : gate[LEAN ? 0u : v], g);
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e) {
                 const float n = has_post ? s[e] * r1 : s[e];
                 if (has_gate) {
-                    d_gate[v][e] = fmaf(d[e], has_post ? n * w1[e] : n, d_gate[v][e]);
+                    to_gate[e] = fmaf(d[e], has_post ? n * w[e] : n, to_gate[e]);
                     d[e] *= g[e];
                 }
                 if (has_post) {
-                    d_post[v][e] = fmaf(d[e], n, d_post[v][e]);
-                    d[e] *= w1[e];
+                    to_post[e] = fmaf(d[e], n, to_post[e]);
+                    d[e] *= w[e];
                     p[0] = fmaf(d[e], s[e], p[0]);
                 }
-                g1[v][e] = d[e];
+                o[e] = d[e];
             }
+        };
+        float first[8];
+        group(0u, d_post, d_pre, d_gate, first);
+        if (V > 1u) {
+            float post2[8], pre2[8], gate2[8], o[8];
+            kept(POST, post2), kept(PRE, pre2), kept(GATE, gate2);
+            group(1u, post2, pre2, gate2, o);
+            keep(POST, post2), keep(PRE, pre2), keep(GATE, gate2), keep(RESULT, o);
         }
+        float c1 = 0.0f;
         if (has_post) {
-            row_sum(p, box_b, a.waves);
-            const float c1 = r1 * (p[0] * each);
-#pragma unroll
-            for (uint32_t v = 0; v < V; ++v) {
-                float s[8];
-                widen8<DT>(x.s[v], s);
-#pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e) g1[v][e] = r1 * fmaf(-c1, s[e] * r1, g1[v][e]);
-            }
-        } else if (a.waves > 1u) {
+            row_sum<1, SUB ? LANES : ONE_ROW>(p, box_b, span);
+            c1 = r1 * (p[0] * each);
+        } else if (span > 64u) {
             __syncthreads(); // box_a is free for the next row
         }
+        auto finish = [&](uint32_t v, float (&o)[8]) {
+            apart();
+            if (has_post) {
+                Row& h = x[LEAN ? 0u : v];
+                if (LEAN) h.s = ask_one(a.d.sum, a.d.sumStride, row, v), settle(h.s, v);
+                float s[8];
+                widen8<DT>(h.s, s);
 #pragma unroll
-        for (uint32_t v = 0; v < V; ++v)
-            store8<DT, TAIL, NT>((uint8_t*)a.d.dSum + row * a.d.dSumStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(g1[v]));
-        if (has_gate && !a.by_gate && (row + 1u == gate_end || row + 1u == end)) { // whole gate rows in one run: theirs are done
-            const uint32_t g = gate_row++;
-            gate_end += (uint32_t)a.d.rowsPerGate;
+                for (uint32_t e = 0; e < 8u; ++e) o[e] = r1 * fmaf(-c1, s[e] * r1, o[e]);
+            }
+            store8<DT, TAIL, NT>((uint8_t*)a.d.dSum + row * a.d.dSumStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(o));
+        };
+        finish(0u, first);
+        if (V > 1u) {
+            float o[8];
+            kept(RESULT, o);
+            finish(1u, o);
+        }
+        if (has_gate && !a.by_gate && (following >= gate_end || following >= end)) {
+            if (a.d.dGate) { // whole rows of the gate in one run: this one is done
+                uint8_t* to = (uint8_t*)a.d.dGate + gate_row * a.d.dGateStride * PS;
+                store8<PT, TAIL>(to, t * 8u, cols, narrow8<PT>(d_gate));
 #pragma unroll
-            for (uint32_t v = 0; v < V; ++v) {
-                if (a.d.dGate) store8<PT, TAIL>((uint8_t*)a.d.dGate + g * a.d.dGateStride * PS, (v * span + t) * 8u, cols, narrow8<PT>(d_gate[v]));
-#pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e) d_gate[v][e] = 0.0f;
-                if (row + 1u < end) {
-                    gate[v] = ask8<PT, TAIL, false>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols, tiny);
-                    settle8<PT, TAIL>(gate[v], (v * span + t) * 8u, cols, tiny);
+                for (uint32_t e = 0; e < 8u; ++e) d_gate[e] = 0.0f;
+                if (V > 1u) {
+                    float o[8];
+                    kept(GATE, o);
+                    store8<PT, TAIL>(to, (span + t) * 8u, cols, narrow8<PT>(o));
+                    keep(GATE, d_gate);
                 }
             }
+            if (following < end) take_gate(following);
         }
+        if (SUB && row + 1u == unit_end) unit_end = following + unit;
+        row = following;
     }
+    // this run's sums; rows that shared a wavefront's lanes are joined first
     float* mine = (float*)a.d.workspace + (uint64_t)blockIdx.x * a.sums * a.pitch;
+    auto leave = [&](int at, int which, float (&d)[8]) {
+        if (at < 0) return;
+        if (SUB) {
 #pragma unroll
-    for (uint32_t v = 0; v < V; ++v) {
-        const uint32_t at = (v * span + t) * 8u; // the workspace's rows hold whole groups
-        if (a.at_post >= 0) store8<DT_F32, false>(mine + (uint64_t)a.at_post * a.pitch, at, a.pitch, narrow8<DT_F32>(d_post[v]));
-        if (a.at_pre >= 0) store8<DT_F32, false>(mine + (uint64_t)a.at_pre * a.pitch, at, a.pitch, narrow8<DT_F32>(d_pre[v]));
-        if (a.at_gate >= 0) store8<DT_F32, false>(mine + (uint64_t)a.at_gate * a.pitch, at, a.pitch, narrow8<DT_F32>(d_gate[v]));
-    }
+            for (uint32_t e = 0; e < 8u; ++e)
+                for (uint32_t far = span; far < 64u; far *= 2u) d[e] += __shfl_xor(d[e], (int)far);
+        }
+        // the workspace's rows hold whole groups
+        if (!SUB || threadIdx.x < span) store8<DT_F32, false>(mine + (uint64_t)at * a.pitch, t * 8u, a.pitch, narrow8<DT_F32>(d));
+        if (V > 1u) {
+            float o[8];
+            kept(which, o);
+            store8<DT_F32, false>(mine + (uint64_t)at * a.pitch, (span + t) * 8u, a.pitch, narrow8<DT_F32>(o));
+        }
+    };
+    leave(a.at_post, POST, d_post);
+    leave(a.at_pre, PRE, d_pre);
+    leave(a.at_gate, GATE, d_gate);
 }
 
 // The runs' sums joined, in a fixed order: a workgroup takes 64 columns of one result, four neighbours to a lane, and 64
@@ -405,39 +503,37 @@ template <int PT> __global__ __launch_bounds__(1024) void k_norm_sums(const HgNo
     }
 }
 
-template <int DT, int PT, uint32_t V, bool ONE, bool TAIL, bool NT, uint32_t N> int launch_norm_n(hipStream_t st, const HgNorm* a)
+template <int DT, int PT, uint32_t V, int SHARE, bool TAIL, bool NT, uint32_t N> int launch_norm_n(hipStream_t st, const HgNorm* a)
 {
     NormArgs<N> n;
-    n.d = a->d, n.waves = a->waves, n.rows_per_wg = a->rows_per_wg;
+    n.d = a->d, n.span = a->span, n.rows_per_wg = a->rows_per_wg;
     for (uint32_t j = 0; j < N; ++j) n.src[j] = a->src[j];
-    hipLaunchKernelGGL((k_norm<DT, PT, V, ONE, TAIL, NT, N>), dim3(a->wgs), dim3(a->waves * 64u * a->rows_per_wg), 0, st, n);
+    hipLaunchKernelGGL((k_norm<DT, PT, V, SHARE, TAIL, NT, N>), dim3(a->wgs), dim3(a->span * a->rows_per_wg), 0, st, n);
     return rc(hipGetLastError());
 }
 
-template <int DT, int PT, uint32_t V, bool ONE> int launch_norm_v(hipStream_t st, const HgNorm* a)
+template <int DT, int PT, uint32_t V, int SHARE> int launch_norm_v(hipStream_t st, const HgNorm* a)
 {
     if (a->d.cols % 8u)
-        return a->d.k <= 8u ? launch_norm_n<DT, PT, V, ONE, true, false, 8>(st, a) : launch_norm_n<DT, PT, V, ONE, true, false, HCOMM_GFX_MAX_RANKS>(st, a);
-    if (a->d.k > 8u) return launch_norm_n<DT, PT, V, ONE, false, true, HCOMM_GFX_MAX_RANKS>(st, a);
-    return a->stream ? launch_norm_n<DT, PT, V, ONE, false, true, 8>(st, a) : launch_norm_n<DT, PT, V, ONE, false, false, 8>(st, a);
+        return a->d.k <= 8u ? launch_norm_n<DT, PT, V, SHARE, true, false, 8>(st, a) : launch_norm_n<DT, PT, V, SHARE, true, false, HCOMM_GFX_MAX_RANKS>(st, a);
+    if (a->d.k > 8u) return launch_norm_n<DT, PT, V, SHARE, false, true, HCOMM_GFX_MAX_RANKS>(st, a);
+    return a->stream ? launch_norm_n<DT, PT, V, SHARE, false, true, 8>(st, a) : launch_norm_n<DT, PT, V, SHARE, false, false, 8>(st, a);
 }
 
 template <int DT, int PT> int launch_norm(hipStream_t st, const HgNorm* a)
 {
-    if (a->vecs == 2u) return launch_norm_v<DT, PT, 2, true>(st, a);
-    return a->rows_per_wg == 1u ? launch_norm_v<DT, PT, 1, true>(st, a) : launch_norm_v<DT, PT, 1, false>(st, a);
+    if (a->vecs == 2u) return launch_norm_v<DT, PT, 2, ONE_ROW>(st, a);
+    if (a->span < 64u) return launch_norm_v<DT, PT, 1, LANES>(st, a);
+    return a->rows_per_wg == 1u ? launch_norm_v<DT, PT, 1, ONE_ROW>(st, a) : launch_norm_v<DT, PT, 1, WAVES>(st, a);
 }
 
 template <int DT, int PT, bool TAIL, bool NT> int launch_norm_grad_t(hipStream_t st, const HgNormGrad* a)
 {
-    const dim3 g((uint32_t)a->chunks), b(a->waves * 64u);
-    if (a->vecs == 1u) {
-        if (a->waves <= 4u) hipLaunchKernelGGL((k_norm_grad<DT, PT, 1, 256, TAIL, NT>), g, b, 0, st, *a);
-        else hipLaunchKernelGGL((k_norm_grad<DT, PT, 1, 512, TAIL, NT>), g, b, 0, st, *a);
-    } else {
-        if (a->waves <= 8u) hipLaunchKernelGGL((k_norm_grad<DT, PT, 2, 512, TAIL, NT>), g, b, 0, st, *a);
-        else hipLaunchKernelGGL((k_norm_grad<DT, PT, 2, 1024, TAIL, NT>), g, b, 0, st, *a);
-    }
+    const dim3 g((uint32_t)a->chunks), b(a->span < 64u ? 64u : a->span);
+    if (a->span > 512u) hipLaunchKernelGGL((k_norm_grad<DT, PT, 2, 1024, false, true, TAIL, NT>), g, b, 0, st, *a);
+    else if (a->vecs == 2u) hipLaunchKernelGGL((k_norm_grad<DT, PT, 2, 512, false, false, TAIL, NT>), g, b, 0, st, *a);
+    else if (a->span >= 64u) hipLaunchKernelGGL((k_norm_grad<DT, PT, 1, 512, false, false, TAIL, NT>), g, b, 0, st, *a);
+    else hipLaunchKernelGGL((k_norm_grad<DT, PT, 1, 64, true, false, TAIL, NT>), g, b, 0, st, *a);
     return rc(hipGetLastError());
 }
 

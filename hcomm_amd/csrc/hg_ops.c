@@ -304,18 +304,13 @@ int32_t HcommGfxMxProductKOnThread(
 
 /* ---- norms behind a fold ------------------------------------------------------------------------------------------------ */
 
-/* wavefronts to a row and groups of eight elements to a lane: a second group where `most` wavefronts do not reach */
-static void row_shape(uint64_t cols, uint32_t most, uint32_t* waves, uint32_t* vecs)
+/* Lanes to a row of `cols` with `vecs` groups of eight elements each: 8, 16 or 32 of a wavefront, or whole wavefronts. */
+static uint32_t row_span(uint64_t cols, uint32_t vecs)
 {
-    const uint64_t per_wave = 64u * 8u;
-    uint32_t w = 1, v = 1;
-    while (w < most && per_wave * w < cols) w *= 2u;
-    if (per_wave * w < cols) {
-        v = 2;
-        while (per_wave * v * w < cols) w *= 2u;
-    }
-    *waves = w;
-    *vecs = v;
+    const uint32_t lanes = (uint32_t)((cols + 8u * vecs - 1u) / (8u * vecs));
+    for (uint32_t s = 8; s <= 32u; s *= 2u)
+        if (lanes <= s) return s;
+    return (lanes + 63u) / 64u * 64u;
 }
 
 #define HG_L2_BYTES (32ull << 20) /* of the eight XCDs together */
@@ -367,40 +362,58 @@ int32_t HcommGfxReduceNormOnThread(ThreadHandle thread, const HcommGfxReduceNorm
     for (uint32_t j = 0; j < desc->k; ++j) a.src[j] = desc->srcs[j];
     a.d.srcs = NULL;
     if (!a.d.gate || a.d.rowsPerGate > rows) a.d.rowsPerGate = rows;
-    row_shape(cols, 16, &a.waves, &a.vecs);
-    a.rows_per_wg = a.waves < 4u ? 4u / a.waves : 1u;
+    /*
+     * One group of eight to a lane as far as 1024 lanes reach: two in half the lanes take longer where rows are few (one row of
+     * 8,192 bf16, 4 partials: 6.2 us against 5.2) and about as long where they are many (5,461 x 6,144: 119 against 98;
+     * 4,096 x 8,192: 108 against 118).  Rows of up to 256 share a wavefront: 524,288 x 64 took 349 us with one each, 93 so.
+     */
+    a.vecs = cols > 8192u ? 2u : 1u;
+    a.span = row_span(cols, a.vecs);
+    a.rows_per_wg = a.span <= 128u && a.vecs == 1u ? 256u / a.span : 1u;
     a.wgs = (uint32_t)((rows + a.rows_per_wg - 1u) / a.rows_per_wg);
     const uint64_t bytes = rows * cols * es * (1u + (desc->sum != NULL) + (desc->z != NULL));
     a.stream = bytes + rows * cols * es * desc->k > HG_L2_BYTES;
-    const HcommGfxLaunchRecord rec = record(HCOMM_GFX_KERNEL_NORM, (int)desc->dataType, HCOMM_REDUCE_SUM, desc->k, bytes, a.wgs, a.waves * 64u);
+    const HcommGfxLaunchRecord rec = record(HCOMM_GFX_KERNEL_NORM, (int)desc->dataType, HCOMM_REDUCE_SUM, desc->k, bytes, a.wgs, a.span);
     return hg_submit_other(t, &rec, hg_launch_norm, &a);
 }
 
-/* Runs of rows for about this many wavefronts: enough to keep every CU loading, few enough that the runs' sums stay a small part of the traffic. */
-#define HG_NORM_GRAD_WAVES 2048u
+/*
+ * Runs of rows: as many as run at once, with up to 8 wavefronts to each of the CUs (their registers allow no more).  Enough to
+ * keep every CU loading, few enough that the runs' sums stay a small part of the traffic; a few more than that would have the
+ * card wait for a second turn (5,461 x 6,144 bf16: 341 runs of 6 wavefronts 129 us).
+ */
+#define HG_NORM_GRAD_CUS 256u
+#define HG_NORM_GRAD_WAVES 8u
 
 /* the geometry, from the sizes and from which parameters' gradients are wanted alone */
 static void norm_grad_shape(HgNormGrad* a)
 {
     HcommGfxReduceNormGradDesc* d = &a->d;
     const uint64_t rows = d->rows;
-    row_shape(d->cols, 8, &a->waves, &a->vecs);
-    const uint64_t most = HG_NORM_GRAD_WAVES / a->waves;
+    a->vecs = d->cols > 4096u ? 2u : 1u;
+    a->span = row_span(d->cols, a->vecs);
+    const uint32_t waves = a->span < 64u ? 1u : a->span / 64u;
+    const uint64_t most = HG_NORM_GRAD_CUS * (waves > HG_NORM_GRAD_WAVES ? 1u : HG_NORM_GRAD_WAVES / waves);
+    const uint64_t sets = a->span < 64u ? 64u / a->span : 1u; /* of lanes to a wavefront, a row each */
     if (!d->gate || d->rowsPerGate > rows) d->rowsPerGate = rows ? rows : 1u;
     a->gates = d->gate ? gate_rows(rows, d->rowsPerGate) : 0u;
     const int gate_wanted = d->gate && d->dGate;
     a->by_gate = gate_wanted && a->gates < most;
     a->chunks = a->chunk_rows = a->chunks_per_gate = 0;
+    a->unit = 1;
     if (rows && a->by_gate) {
         uint64_t per = most / a->gates;
         if (per > d->rowsPerGate) per = d->rowsPerGate;
         a->chunk_rows = (d->rowsPerGate + per - 1u) / per;
+        if (a->chunk_rows < sets) a->chunk_rows = sets;
         a->chunks_per_gate = (d->rowsPerGate + a->chunk_rows - 1u) / a->chunk_rows;
         a->chunks = a->chunks_per_gate * a->gates;
     } else if (rows) {
         /* with a gradient of the gate to write, whole gate rows */
         const uint64_t unit = gate_wanted ? d->rowsPerGate : 1u, units = gate_rows(rows, unit);
-        a->chunk_rows = (units + most - 1u) / most * unit;
+        a->unit = (uint32_t)unit;
+        const uint64_t each = (units + most - 1u) / most;
+        a->chunk_rows = (each < sets ? sets : each) * unit;
         a->chunks = gate_rows(rows, a->chunk_rows);
     }
     a->sums = 0;
@@ -473,7 +486,7 @@ int32_t HcommGfxReduceNormGradOnThread(ThreadHandle thread, const HcommGfxReduce
     a.stream = rows * cols * es * 4u > HG_L2_BYTES; /* sum, dy and what is written, at least */
     if (a.chunks) {
         const HcommGfxLaunchRecord rec = record(
-            HCOMM_GFX_KERNEL_NORM_GRAD, (int)desc->dataType, 255, 1, rows * cols * es * (1u + (desc->dResidual != NULL)), a.chunks, a.waves * 64u);
+            HCOMM_GFX_KERNEL_NORM_GRAD, (int)desc->dataType, 255, 1, rows * cols * es * (1u + (desc->dResidual != NULL)), a.chunks, a.span);
         rc = hg_submit_other(t, &rec, hg_launch_norm_grad, &a);
     }
     if (rc == HCCL_SUCCESS && a.sums) {

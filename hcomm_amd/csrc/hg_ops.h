@@ -76,7 +76,7 @@ int hg_launch_mx_product(void* stream, const void* args);  /* HgMxProduct */
 typedef struct {
     HcommGfxReduceNormDesc d; /* .srcs is not followed on the device: */
     const void* src[HCOMM_GFX_MAX_RANKS];
-    uint32_t waves;       /* wavefronts that share a row */
+    uint32_t span;        /* lanes that share a row: 8, 16, 32 or whole wavefronts */
     uint32_t vecs;        /* groups of eight elements a lane holds */
     uint32_t rows_per_wg;
     uint32_t wgs;
@@ -94,7 +94,8 @@ typedef struct {
     uint64_t gates;           /* rows of the gate */
     uint64_t chunks, chunk_rows, chunks_per_gate;
     uint32_t by_gate;
-    uint32_t waves, vecs, stream;
+    uint32_t span, vecs, stream;
+    uint32_t unit;            /* rows that one set of lanes takes at a time where several share a wavefront */
     uint32_t sums;            /* rows of `pitch` fp32 a run writes to the workspace: post, pre, gate as wanted */
     uint32_t pitch;           /* cols rounded up to 64 */
     int at_post, at_pre, at_gate; /* which of them, -1: not there */

@@ -343,3 +343,39 @@ def test_ends_of_rows(gpu_thread, t, p):
     """Every place in a group of eight elements at which a row can end, around the sizes at which another wavefront joins."""
     for cols in list(range(1, 18)) + [512 + d for d in range(-1, 9)] + [1030, 2047, 4099, 8193, 8198]:
         Case(4, cols, t, k=2, p=p, per=3, pad=1).run(gpu_thread)
+
+
+@pytest.mark.parametrize("rows,per", [(6200, 2), (6149, 3), (700, 2), (1030, 257), (530, 0), (300, 1000), (9, 1), (1, 1)])
+@pytest.mark.parametrize("cols,t,p", [(64, "bf16", "fp32"), (65, "fp32", "fp32"), (128, "fp16", "fp16"), (203, "bf16", "bf16"), (256, "fp32", "fp32"), (257, "bf16", "fp32")])
+def test_rows_that_share_a_wavefront(gpu_thread, rows, per, cols, t, p):
+    """8, 16 and 32 lanes to a row and the first length of a wavefront of its own; gates inside a set of lanes' rows and across sets."""
+    Case(rows, cols, t, k=2, per=per, p=p, pad=5 * (cols % 2)).run(gpu_thread)
+
+
+@pytest.mark.parametrize("rows,per", [(530, 2), (519, 0), (260, 100)])
+@pytest.mark.parametrize("cols,t,p", [(4104, "fp32", "fp32"), (6007, "bf16", "fp32"), (8192, "fp16", "fp16"), (8201, "bf16", "bf16"), (12296, "bf16", "fp32"), (16384, "fp32", "fp32")])
+def test_more_rows_than_runs_of_long_ones(gpu_thread, rows, per, cols, t, p):
+    Case(rows, cols, t, k=1, per=per, p=p).run(gpu_thread)
+
+
+@pytest.mark.parametrize("cols", [40, 130, 4099, 8200, 16377])
+@pytest.mark.parametrize("t", ["bf16", "fp32"])
+def test_gradients_over_their_inputs(gpu_thread, cols, t):
+    """dSum over the sum or dy, dResidual over dy or y: the bits of a call with outputs of its own."""
+    a = Case(20, cols, t, k=1, per=3)
+    torch.cuda.synchronize()
+    h.check(a.forward(gpu_thread))
+    h.check(h.HcommGfxReduceNormGradOnThread(gpu_thread, a.gradient_desc()))
+    h.check(h.HcommGfxThreadSynchronize(gpu_thread))
+    results = ("ds", "dres", "dpost", "dpre", "dgate")
+    want = {n: getattr(a, n).view.clone() for n in results}
+    for ds, dres in (("sum", "dy"), ("sum", "y"), ("dy", "y"), ("dy", "dres"), ("sum", "dres")):
+        b = Case(20, cols, t, k=1, per=3)
+        torch.cuda.synchronize()
+        h.check(b.forward(gpu_thread))
+        d = b.gradient_desc(dSum=getattr(b, ds).ptr, dResidual=getattr(b, dres).ptr)
+        torch.cuda.synchronize()
+        h.check(h.HcommGfxReduceNormGradOnThread(gpu_thread, d))
+        h.check(h.HcommGfxThreadSynchronize(gpu_thread))
+        for n, got in zip(results, (ds, dres, "dpost", "dpre", "dgate")):
+            assert torch.equal(getattr(b, got).view, want[n]), (ds, dres, n)
