@@ -173,87 +173,84 @@ template <uint32_t B> __device__ __forceinline__ void fold_wide(double (&to)[8],
 }
 
 // JOIN: there is an addend or there are more than eight ranks, so that fp64 has to join exact sums
-template <int DT, bool ONE, uint32_t U, uint32_t N, bool JOIN> __global__ __launch_bounds__(256) void k_mx_reduce(const FoldArgs<N> a)
+template <int DT, bool ONE, uint32_t N, bool JOIN> __global__ __launch_bounds__(256) void k_mx_reduce(const FoldArgs<N> a)
 {
     constexpr uint32_t B = N < FOLD_BATCH ? N : FOLD_BATCH;
-#pragma unroll 1
-    for (uint32_t u = 0; u < U; ++u) {
-        const Place<ONE> p = place_of<ONE, U>(a.grid, u);
-        double v[8];             // JOIN: the sum
-        float odd[8], near[8];   // the sum as what narrower types round it from, and rounded to fp32
-        Raw8<DT> own;
-        if (JOIN && a.addend) own = ask_at<DT, false>(a.addend, a.addend_stride, p, a.grid.cols);
-        for (uint32_t j0 = 0; j0 < (JOIN ? a.k : 1u); j0 += B) {
-            uint32_t w[B], s[B];
-            const uint32_t n = N == 1u ? 1u : min(a.k - j0, B);
+    const Place<ONE> p = place_of<ONE, 1>(a.grid, 0u);
+    double v[8];             // JOIN: the sum
+    float odd[8], near[8];   // the sum as what narrower types round it from, and rounded to fp32
+    Raw8<DT> own;
+    if (JOIN && a.addend) own = ask_at<DT, false>(a.addend, a.addend_stride, p, a.grid.cols);
+    for (uint32_t j0 = 0; j0 < (JOIN ? a.k : 1u); j0 += B) {
+        uint32_t w[B], s[B];
+        const uint32_t n = N == 1u ? 1u : min(a.k - j0, B);
 #pragma unroll
-            for (uint32_t j = 0; j < B; ++j) {
-                w[j] = 0u, s[j] = 127u;
-                if (j < n && p.there) {
-                    const HgMxView& r = a.src[j0 + j];
-                    const uint8_t* packed = r.packed + (p.row * r.packed_stride + (uint64_t)p.tile * 4u);
-                    const uint8_t* scales = r.scales + (p.row * r.scale_stride + (p.tile >> 2));
-                    w[j] = *(const __attribute__((address_space(1))) uint32_t*)(packed + p.group * 4u);
-                    s[j] = ((const __attribute__((address_space(1))) uint8_t*)scales)[p.group >> 2];
-                }
-            }
-            const bool empty = !JOIN || (j0 == 0u && !a.addend);
-            if (JOIN && j0 == 0u && a.addend) {
-                float x[8];
-                settle_at(own, p, a.grid.cols);
-                widen8<DT>(own, x);
-#pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e) v[e] = (double)x[e];
-            }
-            uint32_t lo = 255u, hi = 0u; // scales that have a nonzero element under them
-#pragma unroll
-            for (uint32_t j = 0; j < B; ++j) {
-                const bool any = (w[j] & 0x77777777u) != 0u || s[j] == 255u;
-                lo = any && s[j] < lo ? s[j] : lo;
-                hi = any && s[j] > hi ? s[j] : hi;
-            }
-            if (N == 1u || !(hi > lo + 17u || hi > 240u)) {
-                float f[8];
-                decode8(w[0], scale_f32(s[0]), f);
-#pragma unroll
-                for (uint32_t j = 1; j < B; ++j)
-                    if (j < n) {
-                        float x[8];
-                        decode8(w[j], scale_f32(s[j]), x);
-#pragma unroll
-                        for (uint32_t e = 0; e < 8u; ++e) f[e] += x[e];
-                    }
-#pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e) {
-                    if (JOIN) v[e] = empty ? (double)f[e] : v[e] + (double)f[e];
-                    else odd[e] = near[e] = f[e];
-                }
-            } else if (JOIN) {
-                fold_wide(v, empty, w, s, n);
-            } else {
-                double x[8];
-                fold_wide(x, true, w, s, n);
-#pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e) odd[e] = to_odd(x[e]), near[e] = (float)x[e];
+        for (uint32_t j = 0; j < B; ++j) {
+            w[j] = 0u, s[j] = 127u;
+            if (j < n && p.there) {
+                const HgMxView& r = a.src[j0 + j];
+                const uint8_t* packed = r.packed + (p.row * r.packed_stride + (uint64_t)p.tile * 4u);
+                const uint8_t* scales = r.scales + (p.row * r.scale_stride + (p.tile >> 2));
+                w[j] = *(const __attribute__((address_space(1))) uint32_t*)(packed + p.group * 4u);
+                s[j] = ((const __attribute__((address_space(1))) uint8_t*)scales)[p.group >> 2];
             }
         }
-        if (JOIN) {
+        const bool empty = !JOIN || (j0 == 0u && !a.addend);
+        if (JOIN && j0 == 0u && a.addend) {
+            float x[8];
+            settle_at(own, p, a.grid.cols);
+            widen8<DT>(own, x);
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e) odd[e] = to_odd(v[e]), near[e] = (float)v[e];
+            for (uint32_t e = 0; e < 8u; ++e) v[e] = (double)x[e];
         }
-        if (a.dst) store_at<DT>(a.dst, a.dst_stride, p, a.grid.cols, DT == DT_F32 ? narrow8<DT>(near) : narrow8<DT>(odd));
-        if (a.again.packed) {
-            const int64_t left = (int64_t)(a.grid.cols - ((uint64_t)p.tile + p.group) * 8u); // elements to the row's end
-            uint32_t m = 0;
+        uint32_t lo = 255u, hi = 0u; // scales that have a nonzero element under them
+#pragma unroll
+        for (uint32_t j = 0; j < B; ++j) {
+            const bool any = (w[j] & 0x77777777u) != 0u || s[j] == 255u;
+            lo = any && s[j] < lo ? s[j] : lo;
+            hi = any && s[j] > hi ? s[j] : hi;
+        }
+        if (N == 1u || !(hi > lo + 17u || hi > 240u)) {
+            float f[8];
+            decode8(w[0], scale_f32(s[0]), f);
+#pragma unroll
+            for (uint32_t j = 1; j < B; ++j)
+                if (j < n) {
+                    float x[8];
+                    decode8(w[j], scale_f32(s[j]), x);
+#pragma unroll
+                    for (uint32_t e = 0; e < 8u; ++e) f[e] += x[e];
+                }
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e) {
-                if (left <= (int64_t)e) odd[e] = 0.0f; // elements past it do not count, whatever the inputs hold there
-                const uint32_t b = f32_bits(odd[e]) & 0x7fffffffu;
-                m = b > m ? b : m;
+                if (JOIN) v[e] = empty ? (double)f[e] : v[e] + (double)f[e];
+                else odd[e] = near[e] = f[e];
             }
-            const uint32_t s = scale_of(quad_max(m));
-            if (p.there) put_group(a.again, p, encode8(odd, s), s);
+        } else if (JOIN) {
+            fold_wide(v, empty, w, s, n);
+        } else {
+            double x[8];
+            fold_wide(x, true, w, s, n);
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) odd[e] = to_odd(x[e]), near[e] = (float)x[e];
         }
+    }
+    if (JOIN) {
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) odd[e] = to_odd(v[e]), near[e] = (float)v[e];
+    }
+    if (a.dst) store_at<DT>(a.dst, a.dst_stride, p, a.grid.cols, DT == DT_F32 ? narrow8<DT>(near) : narrow8<DT>(odd));
+    if (a.again.packed) {
+        const int64_t left = (int64_t)(a.grid.cols - ((uint64_t)p.tile + p.group) * 8u); // elements to the row's end
+        uint32_t m = 0;
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) {
+            if (left <= (int64_t)e) odd[e] = 0.0f; // elements past it do not count, whatever the inputs hold there
+            const uint32_t b = f32_bits(odd[e]) & 0x7fffffffu;
+            m = b > m ? b : m;
+        }
+        const uint32_t s = scale_of(quad_max(m));
+        if (p.there) put_group(a.again, p, encode8(odd, s), s);
     }
 }
 
@@ -265,9 +262,9 @@ template <class K, class A> int launch(hipStream_t st, uint32_t wgs, K kernel, c
 
 template <int DT> int quantize(hipStream_t st, const HgMxQuantize& a)
 {
-    if (a.grid.rows_per_wg > 1u) return launch(st, a.grid.wgs, k_mx_quantize<DT, false, HG_MX_UNROLL>, a);
-    if (a.grid.tile == 256u) return launch(st, a.grid.wgs, k_mx_quantize<DT, true, 1>, a);
-    return launch(st, a.grid.wgs, k_mx_quantize<DT, true, HG_MX_UNROLL>, a);
+    const bool one = a.grid.rows_per_wg == 1u;
+    if (a.grid.tile == 256u) return one ? launch(st, a.grid.wgs, k_mx_quantize<DT, true, 1>, a) : launch(st, a.grid.wgs, k_mx_quantize<DT, false, 1>, a);
+    return one ? launch(st, a.grid.wgs, k_mx_quantize<DT, true, HG_MX_UNROLL>, a) : launch(st, a.grid.wgs, k_mx_quantize<DT, false, HG_MX_UNROLL>, a);
 }
 
 template <int DT, uint32_t N, bool JOIN> int reduce_n(hipStream_t st, const HgMxReduce& a)
@@ -277,8 +274,7 @@ template <int DT, uint32_t N, bool JOIN> int reduce_n(hipStream_t st, const HgMx
     for (uint32_t j = 0; j < N; ++j) f.src[j] = a.src[j];
     f.again = a.again;
     f.dst = a.dst, f.addend = a.addend, f.dst_stride = a.dst_stride, f.addend_stride = a.addend_stride, f.k = a.k;
-    if (a.grid.rows_per_wg > 1u) return launch(st, a.grid.wgs, k_mx_reduce<DT, false, HG_MX_UNROLL, N, JOIN>, f);
-    return launch(st, a.grid.wgs, k_mx_reduce<DT, true, 1, N, JOIN>, f);
+    return a.grid.rows_per_wg > 1u ? launch(st, a.grid.wgs, k_mx_reduce<DT, false, N, JOIN>, f) : launch(st, a.grid.wgs, k_mx_reduce<DT, true, N, JOIN>, f);
 }
 
 template <int DT> int reduce(hipStream_t st, const HgMxReduce& a)

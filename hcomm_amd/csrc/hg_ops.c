@@ -108,26 +108,28 @@ static int mx_view(HgMxView* v, Range* packed, Range* scales, const HcommGfxMxVi
 }
 
 /*
- * A piece of a long row is one group a lane where that fills the GPU better: in every fold (dequantising 67.1M elements
- * 26.3 -> 24.9 us, 14.3M results of seven ranks 22.9 -> 22.3, 8.4M 20.3 -> 18.8) and in launches of up to `few` workgroups of
- * HG_MX_UNROLL groups a lane.  Large quantisations keep several groups in flight (67.1M elements 28.8 us; one group: 32.8).
+ * A workgroup takes 256 groups, one to a lane, where that fills the GPU better: in every fold (dequantising 67.1M elements
+ * 26.3 -> 24.9 us, 14.3M results of seven ranks 22.9 -> 22.3, 1,024 rows of 1,001 of eight ranks 7.5 -> 4.8) and in launches of up
+ * to `few` workgroups of HG_MX_UNROLL groups a lane (1,024 x 1,001 quantised 8.5 -> 6.0).  Large quantisations keep several
+ * groups in flight (67.1M elements 28.8 us; one group: 32.8).  Rows of up to half of that share a workgroup.
  */
 #define HG_MX_FEW_WGS 1024u
 #define HG_MX_ALWAYS 0xffffffffu
 
 static int mx_grid(HgMxGrid* g, uint64_t rows, uint64_t cols, uint32_t few)
 {
-    const uint32_t most = HG_MX_UNROLL * 256u;
+    uint32_t most = HG_MX_UNROLL * 256u;
     if (cols > HG_MX_MAX_COLS) return HCCL_E_NOT_SUPPORT;
     const uint64_t groups = mx_blocks(cols) * 4u;
     g->rows = rows;
     g->cols = cols;
     g->groups = (uint32_t)groups;
-    g->rows_per_wg = groups < most && rows > 1 ? most / (uint32_t)groups : 1u;
+    const uint64_t in_row = (groups + most - 1u) / most, rows_of_wg = groups <= most / 2u ? most / groups : 1u;
+    if (few == HG_MX_ALWAYS || rows / rows_of_wg <= few / in_row) most = 256u;
     g->tile = most;
-    if (g->rows_per_wg == 1u && (few == HG_MX_ALWAYS || (rows <= few && (groups + most - 1u) / most <= few / rows))) g->tile = 256u;
-    g->tiles = g->rows_per_wg > 1u ? 1u : (uint32_t)((groups + g->tile - 1u) / g->tile);
-    const uint64_t wgs = g->rows_per_wg > 1u ? rows / g->rows_per_wg + (rows % g->rows_per_wg != 0) : rows;
+    g->rows_per_wg = groups <= most / 2u && rows > 1 ? most / (uint32_t)groups : 1u;
+    g->tiles = g->rows_per_wg > 1u ? 1u : (uint32_t)((groups + most - 1u) / most);
+    const uint64_t wgs = rows / g->rows_per_wg + (rows % g->rows_per_wg != 0);
     if (wgs > HG_LIMIT_WGS / g->tiles) return HCCL_E_NOT_SUPPORT;
     g->wgs = (uint32_t)wgs * g->tiles;
     return HCCL_SUCCESS;

@@ -21,15 +21,15 @@ typedef struct {
 
 /*
  * Quantise and fold walk a matrix in groups of eight elements (a quarter of a block, one dword of elements), four
- * neighbouring lanes to a block.  A workgroup of 256 lanes takes a piece of `tile` groups of one row, or, where a row has
- * fewer groups than HG_MX_UNROLL * 256, `rows_per_wg` whole rows.  Host: every matrix that is one run of memory counts as one row.
+ * neighbouring lanes to a block.  A workgroup of 256 lanes takes a piece of `tile` groups of one row, or, where two rows or more
+ * have that many groups together, `rows_per_wg` whole rows.  Host: every matrix that is one run of memory counts as one row.
  */
 #define HG_MX_UNROLL 4u
 
 typedef struct {
     uint64_t rows, cols;
     uint32_t groups;      /* of a row: 4 * ceil(cols / 32) */
-    uint32_t tile;        /* groups to a workgroup that lies in one row: 256 or HG_MX_UNROLL * 256 */
+    uint32_t tile;        /* groups to a workgroup: 256 or HG_MX_UNROLL * 256 */
     uint32_t tiles;       /* workgroups to a row */
     uint32_t rows_per_wg;
     uint32_t wgs;

@@ -335,3 +335,25 @@ def test_product_of_ranks_with_strides_of_their_own(gpu_thread, m, n, cols, k):
         magnitude = sum(np.abs(x.values()) @ np.abs(y.values()).T for x, y in zip(a, b))
         close(dst.double(), want, "fp32", k * cols * 2.0 ** -23 * magnitude, "dst")
         assert dst.guards_hold()
+
+
+AROUND = [(rows, cols) for rows in (1, 3, 300) for cols in (992, 1024, 1025, 1056, 2048, 2049, 4064, 4096, 4097, 8193)]
+
+
+@pytest.mark.parametrize("rows,cols", AROUND + [(140000, 33), (8300, 1000), (2100, 4090), (1100, 4100)])
+def test_rows_around_what_a_workgroup_holds(gpu_thread, rows, cols):
+    """One row, a few and many of the lengths at which a workgroup goes from several rows to one and to pieces of one, and
+    the fold of what was quantised with itself."""
+    rng = np.random.default_rng(rows + cols)
+    src = Dense(rows, cols, "bf16", cols + 1, 1, rng.standard_normal((rows, cols)))
+    out, dst, again = Mx(rows, cols, 1, 1), Dense(rows, cols, "fp32", cols + 2, 1), Mx(rows, cols, 2, 3)
+    ready()
+    h.check(h.HcommGfxMxQuantizeOnThread(gpu_thread, h.mx_views([out.item]), src.ptr, src.stride, rows, cols, DT["bf16"]))
+    h.check(h.HcommGfxMxReduceKOnThread(gpu_thread, dst.ptr, dst.stride, DT["fp32"], h.mx_views([again.item]), h.mx_views([out.item] * 2), 2, None, 0,
+                                        rows, cols))
+    sync(gpu_thread)
+    code, scale = ref.mx_encode(src.double())
+    assert np.array_equal(out.scale(), scale) and np.array_equal(out.code(), code) and out.guards_hold()
+    twice = 2 * out.values()
+    assert np.array_equal(dst.double(), twice) and dst.guards_hold()
+    assert np.array_equal(again.values(), ref.mx_values(*ref.mx_encode(twice), cols)) and again.guards_hold()
