@@ -7,7 +7,7 @@
 #include "hg_host.h"
 #include "hg_ops.h"
 
-#define HG_LIMIT_WGS 0x7fffffffull
+#define HG_LIMIT_LANES 0xffffffffull /* of a launch: the hardware counts them in 32 bits */
 #define HG_LIMIT_ROWS 0x7fffffffull
 
 static uint64_t elem_size(int dtype)
@@ -130,7 +130,7 @@ static int mx_grid(HgMxGrid* g, uint64_t rows, uint64_t cols, uint32_t few)
     g->rows_per_wg = groups <= most / 2u && rows > 1 ? most / (uint32_t)groups : 1u;
     g->tiles = g->rows_per_wg > 1u ? 1u : (uint32_t)((groups + most - 1u) / most);
     const uint64_t wgs = rows / g->rows_per_wg + (rows % g->rows_per_wg != 0);
-    if (wgs > HG_LIMIT_WGS / g->tiles) return HCCL_E_NOT_SUPPORT;
+    if (wgs > HG_LIMIT_LANES / 256u / g->tiles) return HCCL_E_NOT_SUPPORT;
     g->wgs = (uint32_t)wgs * g->tiles;
     return HCCL_SUCCESS;
 }
@@ -231,7 +231,7 @@ static int product_tiles(const HgMxProduct* a)
     return 1;
 }
 
-static uint32_t product_wgs(const HgMxProduct* a, uint32_t edge) { return (a->m + edge - 1u) / edge * ((a->n + edge - 1u) / edge); }
+static uint64_t product_wgs(const HgMxProduct* a, uint32_t edge) { return (uint64_t)((a->m + edge - 1u) / edge) * ((a->n + edge - 1u) / edge); }
 
 /*
  * The largest tiles of which there are enough for the CUs.  Measured, us for an inner length of 8,192 and n = 8,192 (edge 16 / 32 /
@@ -239,7 +239,7 @@ static uint32_t product_wgs(const HgMxProduct* a, uint32_t edge) { return (a->m 
  * m = 512: 240 / 151 / 48 / 30 / 50, m = 1,024: 477 / 299 / 92 / 59 / 54, m = 4,096: 1,894 / 1,186 / 389 / 212 / 140; 200 x 200 x 512:
  * 2.7 / 3.1 / 3.5 / 4.8 / 10.4, 300 x 300 x 4,096: 7.1 / 6.8 / 7.3 / 14 / 32.
  */
-static void product_form(HgMxProduct* a)
+static int product_form(HgMxProduct* a)
 {
     uint32_t edge = 16u;
     a->form = HG_PRODUCT_DIRECT_16;
@@ -257,7 +257,8 @@ static void product_form(HgMxProduct* a)
         edge = 32u;
         a->form = HG_PRODUCT_DIRECT_32;
     }
-    a->wgs = product_wgs(a, edge);
+    a->wgs = (uint32_t)product_wgs(a, edge);
+    return product_wgs(a, edge) <= HG_LIMIT_LANES / 512u; /* the direct forms' workgroups */
 }
 
 int32_t HcommGfxMxProductKOnThread(
@@ -274,9 +275,7 @@ int32_t HcommGfxMxProductKOnThread(
     if (!es || cols == 0) return HCCL_E_PARA;
     HgMxProduct p;
     memset(&p, 0, sizeof(p));
-    /* 16 results an edge at least: the number of workgroups stays below 2^31 */
     int rc = m > HG_LIMIT_ROWS - 512u || n > HG_LIMIT_ROWS - 512u || mx_blocks(cols) * HCOMM_GFX_MX_BLOCK_BYTES >= HG_MX_PRODUCT_STRIDE ? HCCL_E_NOT_SUPPORT : HCCL_SUCCESS;
-    if (rc == HCCL_SUCCESS && (m + 15u) / 16u * ((n + 15u) / 16u) > HG_LIMIT_WGS) rc = HCCL_E_NOT_SUPPORT;
     if (rc == HCCL_SUCCESS) {
         Range r[1 + 4 * HCOMM_GFX_MAX_RANKS];
         memset(r, 0, sizeof(r));
@@ -289,17 +288,17 @@ int32_t HcommGfxMxProductKOnThread(
             if (n > 1 && (b[j].packedStride >= HG_MX_PRODUCT_STRIDE || b[j].scaleStride >= HG_MX_PRODUCT_STRIDE)) rc = HCCL_E_NOT_SUPPORT;
         }
         if (!clear_of(&r[0], r, 1 + 4 * k, NULL)) return HCCL_E_PARA;
+        p.m = (uint32_t)m;
+        p.n = (uint32_t)n;
+        p.cols = (uint32_t)cols;
+        p.k = k;
+        if (rc == HCCL_SUCCESS && !product_form(&p)) rc = HCCL_E_NOT_SUPPORT;
     }
     if (rc == HCCL_SUCCESS) rc = ready(t);
     if (rc != HCCL_SUCCESS || m == 0 || n == 0) return rc;
     p.dst = dst;
     p.dst_stride = m > 1 ? dstStride : n;
-    p.m = (uint32_t)m;
-    p.n = (uint32_t)n;
-    p.cols = (uint32_t)cols;
-    p.k = k;
     p.dtype = (int)dstType;
-    product_form(&p);
     const HcommGfxLaunchRecord rec = record(HCOMM_GFX_KERNEL_MX_PRODUCT, p.dtype, HCOMM_REDUCE_SUM, k, m * n * es, p.wgs, p.form);
     return hg_submit_other(t, &rec, hg_launch_mx_product, &p);
 }
@@ -358,21 +357,22 @@ int32_t HcommGfxReduceNormOnThread(ThreadHandle thread, const HcommGfxReduceNorm
             if (!dense_range(&r[SRC + j], desc->srcs[j], rows, cols, desc->srcStride, es)) return HCCL_E_PARA;
         const uint32_t n = SRC + desc->k;
         if (!clear_of(&r[SUM], r, n, &r[SRC]) || !clear_of(&r[Y], r, n, &r[RES]) || !clear_of(&r[Z], r, n, NULL)) return HCCL_E_PARA;
+        /*
+         * One group of eight to a lane as far as 1024 lanes reach: two in half the lanes take longer where rows are few (one row of
+         * 8,192 bf16, 4 partials: 6.2 us against 5.2) and about as long where they are many (5,461 x 6,144: 119 against 98;
+         * 4,096 x 8,192: 108 against 118).  Rows of up to 256 share a wavefront: 524,288 x 64 took 349 us with one each, 93 so.
+         */
+        a.vecs = cols > 8192u ? 2u : 1u;
+        a.span = row_span(cols, a.vecs);
+        a.rows_per_wg = a.span <= 128u && a.vecs == 1u ? 256u / a.span : 1u;
+        a.wgs = (uint32_t)((rows + a.rows_per_wg - 1u) / a.rows_per_wg);
+        if (a.wgs > HG_LIMIT_LANES / (a.span * a.rows_per_wg)) rc = HCCL_E_NOT_SUPPORT;
     }
     if (rc == HCCL_SUCCESS) rc = ready(t);
     if (rc != HCCL_SUCCESS || rows == 0 || cols == 0) return rc;
     for (uint32_t j = 0; j < desc->k; ++j) a.src[j] = desc->srcs[j];
     a.d.srcs = NULL;
     if (!a.d.gate || a.d.rowsPerGate > rows) a.d.rowsPerGate = rows;
-    /*
-     * One group of eight to a lane as far as 1024 lanes reach: two in half the lanes take longer where rows are few (one row of
-     * 8,192 bf16, 4 partials: 6.2 us against 5.2) and about as long where they are many (5,461 x 6,144: 119 against 98;
-     * 4,096 x 8,192: 108 against 118).  Rows of up to 256 share a wavefront: 524,288 x 64 took 349 us with one each, 93 so.
-     */
-    a.vecs = cols > 8192u ? 2u : 1u;
-    a.span = row_span(cols, a.vecs);
-    a.rows_per_wg = a.span <= 128u && a.vecs == 1u ? 256u / a.span : 1u;
-    a.wgs = (uint32_t)((rows + a.rows_per_wg - 1u) / a.rows_per_wg);
     const uint64_t bytes = rows * cols * es * (1u + (desc->sum != NULL) + (desc->z != NULL));
     a.stream = bytes + rows * cols * es * desc->k > HG_L2_BYTES;
     const HcommGfxLaunchRecord rec = record(HCOMM_GFX_KERNEL_NORM, (int)desc->dataType, HCOMM_REDUCE_SUM, desc->k, bytes, a.wgs, a.span);

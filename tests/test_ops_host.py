@@ -229,3 +229,21 @@ def test_a_thread_in_another_batch_is_refused(rec):
         stop.set()
         t.join()
     assert h.HcommGfxMxQuantizeOnThread(rec, view(), C_, 64, 4, 64, DT.BFP16) == R.SUCCESS
+
+
+def test_launches_of_more_lanes_than_a_grid_counts(rec):
+    """A limit of its own, next to it the last size that is taken; nothing of a refused call is queued."""
+    big = lambda at: at << 20  # noqa: E731  (apart from one another by more than the matrices are long)
+    fold = lambda cols: h.HcommGfxMxReduceKOnThread(rec, big(A), 0, DT.BFP16, None, h.mx_views([(big(B), 0, big(C_), 0)]), 1, None, 0, 1, cols)  # noqa: E731
+    last = ((1 << 24) - 1) * 256 * 8
+    assert last > 1 << 34 and fold((1 << 34) + 32) == R.E_NOT_SUPPORT and fold(1 << 34) == R.SUCCESS
+    rows = lambda n: h.HcommGfxMxReduceKOnThread(rec, big(A), 64, DT.BFP16, None, h.mx_views([(big(B), 32, big(C_), 2)]), 1, None, 0, n, 33)  # noqa: E731
+    assert rows(32 * ((1 << 24) - 1)) == R.SUCCESS and rows(32 * ((1 << 24) - 1) + 1) == R.E_NOT_SUPPORT
+    norm = lambda n: h.HcommGfxReduceNormOnThread(rec, h.ReduceNormDesc(  # noqa: E731
+        rows=n, cols=64, dataType=DT.BFP16, paramType=DT.BFP16, residualScale=1.0, eps=1e-5, srcs=[big(A)], srcStride=64, y=big(B), yStride=64))
+    assert norm(32 * ((1 << 24) - 1)) == R.SUCCESS and norm(32 * ((1 << 24) - 1) + 1) == R.E_NOT_SUPPORT and norm(1 << 31) == R.E_NOT_SUPPORT
+    one = lambda m, n: h.HcommGfxMxProductKOnThread(rec, big(A), n, DT.BFP16, h.mx_views([(big(B), 16, big(C_), 1)]),  # noqa: E731
+                                                    h.mx_views([(big(D), 16, big(E), 1)]), 1, m, n, 32)
+    assert one(1, 16 * ((1 << 23) - 1)) == R.SUCCESS and one(1, 16 * ((1 << 23) - 1) + 1) == R.E_NOT_SUPPORT
+    assert one(1 << 16, (1 << 17) - 32) == R.SUCCESS and one(1 << 16, 1 << 17) == R.E_NOT_SUPPORT
+    assert [r.kind for r in h.launch_log(rec)] == [Kernel.MX_REDUCE] * 2 + [Kernel.NORM] + [Kernel.MX_PRODUCT] * 2
