@@ -42,25 +42,27 @@ struct Run {
 };
 
 typedef u32x4 __attribute__((aligned(1))) u32x4_at1;
+typedef const __attribute__((address_space(1))) uint8_t cg8;
 
-// Blocks [first, first + 16) of a row of `blocks`.  No branch: loads of several runs are to be under way together.  Past the
-// row's end its last block is read once more, and settle_run, called where the run is used, takes care of it.  g: lane / 16
-// SHORT: the rows have fewer than 16 blocks, scales come byte by byte.
-template <bool SHORT> __device__ __forceinline__ Run load_run(const HgMxView& v, uint32_t row, uint32_t first, uint32_t blocks, uint32_t g)
+// Blocks [first, first + 16) of a row of `blocks`, 16 at least.  No branch: loads of several runs are to be under way together.
+// Past the row's end its last block is read once more, and settle_run, called where the run is used, takes care of it.  g: lane / 16
+__device__ __forceinline__ Run load_run(const HgMxView& v, uint32_t row, uint32_t first, uint32_t blocks, uint32_t g)
 {
-    typedef const __attribute__((address_space(1))) uint8_t cg8;
     Run r;
     const uint8_t* p = v.packed + (uint64_t)row * v.packed_stride;
     const uint8_t* s = v.scales + (uint64_t)row * v.scale_stride;
 #pragma unroll
     for (uint32_t t = 0; t < 4u; ++t) r.block[t] = ((cgvec*)p)[min(first + 4u * t + g, blocks - 1u)];
-    if (SHORT) {
-#pragma unroll
-        for (uint32_t t = 0; t < 4u; ++t) r.scales[t] = (uint32_t)((cg8*)s)[min(4u * t + g, blocks - 1u)];
-    } else {
-        r.scales = *(const __attribute__((address_space(1))) u32x4_at1*)(s + min(first, blocks - CHUNK_BLOCKS));
-    }
+    r.scales = *(const __attribute__((address_space(1))) u32x4_at1*)(s + min(first, blocks - CHUNK_BLOCKS));
     return r;
+}
+
+// Four blocks from `first` on as the t-th of a run, in rows of fewer than 16; this lane's scale alone in word t.
+__device__ __forceinline__ void load_four(Run& r, uint32_t t, const HgMxView& v, uint32_t row, uint32_t first, uint32_t blocks, uint32_t g)
+{
+    const uint32_t b = min(first + g, blocks - 1u);
+    r.block[t] = ((cgvec*)(v.packed + (uint64_t)row * v.packed_stride))[b];
+    r.scales[t] = (uint32_t)((cg8*)(v.scales + (uint64_t)row * v.scale_stride))[b];
 }
 
 // w shifted down by `by` bytes, 0 from 16 on
@@ -84,21 +86,25 @@ __device__ __forceinline__ u32x4 down_by(u32x4 w, uint32_t by)
 
 // A row's last chunk: scales of blocks past the end become 0 (with 2^-127 on both sides the products are far below what
 // fp32 holds), elements of the last block past cols become 0.
-template <bool SHORT> __device__ __forceinline__ void settle_run(Run& r, uint32_t first, uint32_t blocks, uint32_t cols, uint32_t g)
+__device__ __forceinline__ void settle_run(Run& r, uint32_t first, uint32_t blocks, uint32_t cols, uint32_t g)
 {
-    if (SHORT) {
-#pragma unroll
-        for (uint32_t t = 0; t < 4u; ++t) r.scales[t] = 4u * t + g < blocks ? r.scales[t] : 0u;
-    } else {
-        const uint32_t by = first - min(first, blocks - CHUNK_BLOCKS); // bytes that the fetch went back
-        r.scales = down_by(r.scales, by);
-    }
+    const uint32_t by = first - min(first, blocks - CHUNK_BLOCKS); // bytes that the fetch went back
+    r.scales = down_by(r.scales, by);
     const uint32_t last = blocks - 1u;
     const u32x4 mask = kept(cols - last * HCOMM_GFX_MX_BLOCK);
 #pragma unroll
     for (uint32_t t = 0; t < 4u; ++t)
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i) r.block[t][i] &= first + 4u * t + g == last ? mask[i] : 0xffffffffu;
+}
+
+__device__ __forceinline__ void settle_four(Run& r, uint32_t t, uint32_t first, uint32_t blocks, uint32_t cols, uint32_t g)
+{
+    const uint32_t last = blocks - 1u;
+    const u32x4 mask = kept(cols - last * HCOMM_GFX_MX_BLOCK);
+    r.scales[t] = first + g <= last ? r.scales[t] : 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) r.block[t][i] &= first + g == last ? mask[i] : 0xffffffffu;
 }
 
 // four neighbours of a row of dst
@@ -131,14 +137,17 @@ template <uint32_t N> struct ProductArgs {
 // A workgroup owns 16 FA x 16 FB results; its W wavefronts share the inner length (chunk u of all ranks' chunks goes to
 // wavefront u % W), each with the next chunk's loads on their way while it multiplies, and add their sums up through LDS in
 // a fixed order.
+// SHORT: ranks of fewer than 16 blocks.  A chunk holds fours of blocks there, EACH of them: those of one rank, so that the
+// ranks spread over the wavefronts, or with a single wavefront the next four of all ranks' fours.
 template <int DT, int FA, int FB, uint32_t W, bool SHORT, uint32_t N> __global__ __launch_bounds__(64 * W) void k_mx_product_direct(const ProductArgs<N> a)
 {
-    __shared__ f32x4 part[W][FA * FB][64];
+    __shared__ f32x4 part[W > 1u ? W : 1u][W > 1u ? FA * FB : 1][W > 1u ? 64 : 1];
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, shift = SHORT ? 0u : 8u * g, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t tiles_n = (a.n + 16u * FB - 1u) / (16u * FB);
     const uint32_t tm = blockIdx.x / tiles_n, tn = blockIdx.x - tm * tiles_n;
     const uint32_t m0 = tm * 16u * FA, n0 = tn * 16u * FB;
     const uint32_t blocks = (a.cols + HCOMM_GFX_MX_BLOCK - 1u) / HCOMM_GFX_MX_BLOCK, chunks = (blocks + CHUNK_BLOCKS - 1u) / CHUNK_BLOCKS;
+    const uint32_t fours = (blocks + 3u) / 4u, each = W > 1u ? fours : 4u;
     uint32_t row_a[FA], row_b[FB]; // rows past the end: the last one once more, its results are not stored
 #pragma unroll
     for (int i = 0; i < FA; ++i) row_a[i] = min(m0 + 16u * i + (lane & 15u), a.m - 1u);
@@ -151,57 +160,92 @@ template <int DT, int FA, int FB, uint32_t W, bool SHORT, uint32_t N> __global__
         for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     struct Chunk {
         Run a[FA], b[FB];
-        uint32_t first; // block of its rank
+        uint32_t first, rank; // block of its rank
     } c0, c1;
-    uint32_t rank = wave / chunks, chunk = wave - rank * chunks; // of the next loads
+    uint32_t rank = wave / chunks, chunk = wave - rank * chunks; // of the next loads; SHORT: the chunk is a four of blocks
     auto ask = [&](Chunk& c) {
         const uint32_t first = chunk * CHUNK_BLOCKS;
-        c.first = first;
+        c.first = first, c.rank = rank;
 #pragma unroll
-        for (int j = 0; j < FB; ++j) c.b[j] = load_run<SHORT>(a.b[rank], row_b[j], first, blocks, g);
+        for (int j = 0; j < FB; ++j) c.b[j] = load_run(a.b[rank], row_b[j], first, blocks, g);
 #pragma unroll
-        for (int i = 0; i < FA; ++i) c.a[i] = load_run<SHORT>(a.a[rank], row_a[i], first, blocks, g);
+        for (int i = 0; i < FA; ++i) c.a[i] = load_run(a.a[rank], row_a[i], first, blocks, g);
         chunk += W;
         while (chunk >= chunks) chunk -= chunks, ++rank;
     };
+    auto ask_fours = [&](Chunk& c) {
+        c.first = 4u * chunk, c.rank = rank;
+#pragma unroll
+        for (uint32_t t = 0; t < 4u; ++t) {
+            if (t >= each || rank >= a.k) break;
+#pragma unroll
+            for (int j = 0; j < FB; ++j) load_four(c.b[j], t, a.b[rank], row_b[j], 4u * chunk, blocks, g);
+#pragma unroll
+            for (int i = 0; i < FA; ++i) load_four(c.a[i], t, a.a[rank], row_a[i], 4u * chunk, blocks, g);
+            if (++chunk == fours) chunk = 0u, ++rank;
+        }
+        if (W > 1u) rank += W - 1u;
+    };
+    auto multiply_one = [&](Chunk& c, uint32_t t) {
+#pragma unroll
+        for (int i = 0; i < FA; ++i)
+#pragma unroll
+            for (int j = 0; j < FB; ++j)
+                acc[i][j] = mfma(c.b[j].block[t], c.a[i].block[t], acc[i][j], c.b[j].scales[t] >> shift, c.a[i].scales[t] >> shift);
+    };
     auto multiply = [&](Chunk& c) {
+        if (SHORT) {
+#pragma unroll
+            for (uint32_t t = 0; t < 4u; ++t) {
+                if (t >= each || c.rank >= a.k) break;
+#pragma unroll
+                for (int i = 0; i < FA; ++i) settle_four(c.a[i], t, c.first, blocks, a.cols, g);
+#pragma unroll
+                for (int j = 0; j < FB; ++j) settle_four(c.b[j], t, c.first, blocks, a.cols, g);
+                multiply_one(c, t);
+                c.first += 4u;
+                if (c.first >= blocks) c.first = 0u, ++c.rank;
+            }
+            return;
+        }
         if (c.first + CHUNK_BLOCKS >= blocks) {
 #pragma unroll
-            for (int i = 0; i < FA; ++i) settle_run<SHORT>(c.a[i], c.first, blocks, a.cols, g);
+            for (int i = 0; i < FA; ++i) settle_run(c.a[i], c.first, blocks, a.cols, g);
 #pragma unroll
-            for (int j = 0; j < FB; ++j) settle_run<SHORT>(c.b[j], c.first, blocks, a.cols, g);
+            for (int j = 0; j < FB; ++j) settle_run(c.b[j], c.first, blocks, a.cols, g);
         }
 #pragma unroll
-        for (uint32_t t = 0; t < 4u; ++t)
-#pragma unroll
-            for (int i = 0; i < FA; ++i)
-#pragma unroll
-                for (int j = 0; j < FB; ++j)
-                    acc[i][j] = mfma(c.b[j].block[t], c.a[i].block[t], acc[i][j], c.b[j].scales[t] >> shift, c.a[i].scales[t] >> shift);
+        for (uint32_t t = 0; t < 4u; ++t) multiply_one(c, t);
+    };
+    auto next = [&](Chunk& c) {
+        if (SHORT) ask_fours(c);
+        else ask(c);
     };
     if (rank < a.k) {
-        ask(c0);
+        next(c0);
         for (;;) {
             const bool more1 = rank < a.k;
-            if (more1) ask(c1);
+            if (more1) next(c1);
             multiply(c0);
             if (!more1) break;
             const bool more0 = rank < a.k;
-            if (more0) ask(c0);
+            if (more0) next(c0);
             multiply(c1);
             if (!more0) break;
         }
     }
+    if (W > 1u) {
 #pragma unroll
-    for (int i = 0; i < FA; ++i)
+        for (int i = 0; i < FA; ++i)
 #pragma unroll
-        for (int j = 0; j < FB; ++j) part[wave][i * FB + j][lane] = acc[i][j];
-    __syncthreads();
+            for (int j = 0; j < FB; ++j) part[wave][i * FB + j][lane] = acc[i][j];
+        __syncthreads();
+    }
     // a lane holds four neighbours of a row of dst
 #pragma unroll
     for (uint32_t f = 0; f < FA * FB; ++f)
         if (f % W == wave) {
-            f32x4 v = part[0][f][lane];
+            f32x4 v = W > 1u ? part[0][f][lane] : acc[f / FB][f % FB];
 #pragma unroll
             for (uint32_t w = 1; w < W; ++w) {
                 const f32x4 x = part[w][f][lane];
@@ -628,6 +672,9 @@ template <int DT, bool SHORT, uint32_t N> int launch(hipStream_t st, const HgMxP
     switch (a->form) {
         case HG_PRODUCT_DIRECT_16: hipLaunchKernelGGL((k_mx_product_direct<DT, 1, 1, 8, SHORT, N>), g, dim3(512), 0, st, p); break;
         case HG_PRODUCT_DIRECT_32: hipLaunchKernelGGL((k_mx_product_direct<DT, 2, 2, 8, SHORT, N>), g, dim3(512), 0, st, p); break;
+        case HG_PRODUCT_WAVE_32: // of short rows alone
+            if (SHORT) hipLaunchKernelGGL((k_mx_product_direct<DT, 2, 2, 1, true, N>), g, dim3(64), 0, st, p);
+            break;
         case HG_PRODUCT_MID_64:
             if (a->cols % HCOMM_GFX_MX_BLOCK) hipLaunchKernelGGL((k_mx_product_mid<DT, 1, true, N>), g, dim3(256), 0, st, p);
             else hipLaunchKernelGGL((k_mx_product_mid<DT, 1, false, N>), g, dim3(256), 0, st, p);

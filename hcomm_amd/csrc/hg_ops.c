@@ -219,11 +219,10 @@ int32_t HcommGfxMxReduceKOnThread(
 
 /* ---- product --------------------------------------------------------------------------------------------------------- */
 
-/* what the forms through LDS ask for: a whole stage of columns (8 blocks; with fewer than 16 the direct forms are ahead anyway), and ranks
- * whose matrices have the same strides */
+/* what the forms through LDS ask for: a whole stage of columns (8 blocks), and ranks whose matrices have the same strides */
 static int product_tiles(const HgMxProduct* a)
 {
-    if (mx_blocks(a->cols) < 16u) return 0;
+    if (mx_blocks(a->cols) < 8u) return 0;
     for (uint32_t j = 1; j < a->k; ++j)
         if (a->a[j].packed_stride != a->a[0].packed_stride || a->a[j].scale_stride != a->a[0].scale_stride ||
             a->b[j].packed_stride != a->b[0].packed_stride || a->b[j].scale_stride != a->b[0].scale_stride)
@@ -237,23 +236,33 @@ static uint64_t product_wgs(const HgMxProduct* a, uint32_t edge) { return (uint6
  * The largest tiles of which there are enough for the CUs.  Measured, us for an inner length of 8,192 and n = 8,192 (edge 16 / 32 /
  * 64 / 128 / 256): m = 16: 12.3 / 11.3 / 12.4 / 23 / 47, m = 64: 33 / 21 / 13 / 23 / 47, m = 256: 121 / 76 / 25.5 / 25.1 / 50,
  * m = 512: 240 / 151 / 48 / 30 / 50, m = 1,024: 477 / 299 / 92 / 59 / 54, m = 4,096: 1,894 / 1,186 / 389 / 212 / 140; 200 x 200 x 512:
- * 2.7 / 3.1 / 3.5 / 4.8 / 10.4, 300 x 300 x 4,096: 7.1 / 6.8 / 7.3 / 14 / 32.
+ * 2.7 / 3.1 / 3.5 / 4.8 / 10.4, 300 x 300 x 4,096: 7.1 / 6.8 / 7.3 / 14 / 32, 512 x 512 x 2,048: 7.4 / 5.0 / 5.4 / 8.5 / 18,
+ * 33 x 8,000 x 2,048: 10.5 / 8.7 / 5.8 / 8.7 / 17, 300 x 1,200 x 4,096 with edge 32 / 64: 13.2 / 8.7.  Edge 32 has one workgroup to a CU: up to
+ * 256 tiles of it run at once.
+ * Rows of fewer than 16 blocks: a wavefront for every 32 x 32 results instead of eight that share so little, from about as many
+ * tiles on as a wavefront takes fours of blocks (8 wavefronts / 1 / edge 64 / 128): 1,024 x 1,024 results of one rank's 32 columns
+ * 6.7 / 3.4, of four ranks' 165 8.3 / 5.6, of 16 ranks' 30 9.6 / 8.3; 512 x 512 of 8 ranks' 32 3.3 / 4.8; 4,096 x 8,192 of one rank's 32
+ * 153 / 28; 410 x 3,924 of one rank's 250 12.5 / 5.8 / 7.2 / 6.7, of four ranks' 250 18.7 / 12.8 / 11.7 / 9.3.
  */
 static int product_form(HgMxProduct* a)
 {
+    const uint64_t blocks = mx_blocks(a->cols), fours = a->k * ((blocks + 3u) / 4u), of_32 = product_wgs(a, 32u);
+    const int tiles = product_tiles(a);
     uint32_t edge = 16u;
     a->form = HG_PRODUCT_DIRECT_16;
-    const int tiles = product_tiles(a);
     if (tiles && product_wgs(a, 256u) >= 128u) {
         edge = 256u;
         a->form = HG_PRODUCT_TILE;
+    } else if (blocks < 16u && (!tiles || fours <= 2u) && of_32 >= (fours < 13u ? 192u + 64u * fours : 1024u)) {
+        edge = 32u;
+        a->form = HG_PRODUCT_WAVE_32;
     } else if (tiles && product_wgs(a, 128u) >= 128u) {
         edge = 128u;
         a->form = HG_PRODUCT_MID_128;
-    } else if (tiles && a->m > 32u && a->n > 32u && product_wgs(a, 64u) >= 64u) {
+    } else if (tiles && a->m > 32u && a->n > 32u && of_32 > 256u) {
         edge = 64u;
         a->form = HG_PRODUCT_MID_64;
-    } else if (a->m > 16u && a->n > 16u && product_wgs(a, 32u) >= 64u) {
+    } else if (a->m > 16u && a->n > 16u && of_32 >= 64u) {
         edge = 32u;
         a->form = HG_PRODUCT_DIRECT_32;
     }

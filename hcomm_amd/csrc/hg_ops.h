@@ -54,7 +54,8 @@ typedef struct {
     int dtype;
 } HgMxReduce;
 
-enum { HG_PRODUCT_DIRECT_16 = 0, HG_PRODUCT_DIRECT_32, HG_PRODUCT_MID_64, HG_PRODUCT_MID_128, HG_PRODUCT_TILE }; /* edge of a workgroup's results: 16, 32, 64, 128, 256 */
+/* edge of a workgroup's results: 16, 32, 32 (one wavefront), 64, 128, 256 */
+enum { HG_PRODUCT_DIRECT_16 = 0, HG_PRODUCT_DIRECT_32, HG_PRODUCT_WAVE_32, HG_PRODUCT_MID_64, HG_PRODUCT_MID_128, HG_PRODUCT_TILE };
 
 typedef struct {
     HgMxView a[HCOMM_GFX_MAX_RANKS];

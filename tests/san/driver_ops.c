@@ -30,7 +30,7 @@ int hg_launch_mx_reduce(void* s, const void* a) { (void)s; ++met[1]; mx_grid_ok(
 int hg_launch_mx_product(void* s, const void* args)
 {
     const HgMxProduct* p = (const HgMxProduct*)args;
-    const uint64_t edge = p->form == HG_PRODUCT_DIRECT_16 ? 16 : p->form == HG_PRODUCT_DIRECT_32 ? 32 : p->form == HG_PRODUCT_MID_64 ? 64 : p->form == HG_PRODUCT_MID_128 ? 128 : 256;
+    const uint64_t edge = p->form == HG_PRODUCT_DIRECT_16 ? 16 : p->form == HG_PRODUCT_DIRECT_32 || p->form == HG_PRODUCT_WAVE_32 ? 32 : p->form == HG_PRODUCT_MID_64 ? 64 : p->form == HG_PRODUCT_MID_128 ? 128 : 256;
     (void)s; ++met[2];
     grid(p->wgs, edge <= 32 ? 512 : 256);
     expect(p->wgs == (p->m + edge - 1) / edge * ((p->n + edge - 1) / edge), "tiles");

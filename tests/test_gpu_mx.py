@@ -357,3 +357,18 @@ def test_rows_around_what_a_workgroup_holds(gpu_thread, rows, cols):
     twice = 2 * out.values()
     assert np.array_equal(dst.double(), twice) and dst.guards_hold()
     assert np.array_equal(again.values(), ref.mx_values(*ref.mx_encode(twice), cols)) and again.guards_hold()
+
+
+SHORT = [(600, 700, 32, 1), (600, 700, 33, 3), (600, 700, 200, 9), (520, 1030, 224, 32), (1100, 600, 100, 17), (2050, 2050, 97, 2), (900, 1100, 128, 4),
+         (1500, 1600, 250, 2), (600, 700, 300, 5), (1500, 1600, 470, 2), (1400, 4100, 256, 1), (2050, 2300, 300, 3)]
+
+
+@pytest.mark.parametrize("m,n,cols,k", SHORT)
+def test_product_of_short_rows(gpu_thread, m, n, cols, k):
+    """Many results of one to fifteen blocks a rank."""
+    product_case(gpu_thread, m, n, cols, k, "bf16", np.random.default_rng(m + n + cols), pad=2, shift=3, tail=0xE, stride=1)
+
+
+@pytest.mark.parametrize("m,n,cols", [(600, 800, 40), (600, 800, 220), (700, 800, 250), (1500, 1600, 400), (1400, 4100, 300)])
+def test_product_of_short_rows_with_nan(gpu_thread, m, n, cols):
+    test_product_of_a_block_that_is_nan(gpu_thread, m, n, cols)

@@ -244,6 +244,6 @@ def test_launches_of_more_lanes_than_a_grid_counts(rec):
     assert norm(32 * ((1 << 24) - 1)) == R.SUCCESS and norm(32 * ((1 << 24) - 1) + 1) == R.E_NOT_SUPPORT and norm(1 << 31) == R.E_NOT_SUPPORT
     one = lambda m, n: h.HcommGfxMxProductKOnThread(rec, big(A), n, DT.BFP16, h.mx_views([(big(B), 16, big(C_), 1)]),  # noqa: E731
                                                     h.mx_views([(big(D), 16, big(E), 1)]), 1, m, n, 32)
-    assert one(1, 16 * ((1 << 23) - 1)) == R.SUCCESS and one(1, 16 * ((1 << 23) - 1) + 1) == R.E_NOT_SUPPORT
+    assert one(1, 32 * ((1 << 23) - 1)) == R.SUCCESS and one(1, 32 * ((1 << 23) - 1) + 1) == R.E_NOT_SUPPORT
     assert one(1 << 16, (1 << 17) - 32) == R.SUCCESS and one(1 << 16, 1 << 17) == R.E_NOT_SUPPORT
     assert [r.kind for r in h.launch_log(rec)] == [Kernel.MX_REDUCE] * 2 + [Kernel.NORM] + [Kernel.MX_PRODUCT] * 2
