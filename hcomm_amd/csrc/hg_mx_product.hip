@@ -9,8 +9,7 @@ namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef u32x2 __attribute__((aligned(2))) u32x2_at2;
+typedef u32x2_raw u32x2;
 
 #define MX_FP4 4 /* element format operand of the matrix instruction */
 #define CHUNK_BLOCKS 16u

@@ -33,7 +33,7 @@ __device__ __forceinline__ float wave_sum(float v)
     return (a + b) + (c + d);
 }
 
-// What a workgroup has: one row, several of whole wavefronts (1 or 2 each), or several of 8, 16 or 32 lanes.
+// What a workgroup has: one row, several of whole wavefronts (1 or 2 each), or several of 1 to 32 lanes.
 enum { ONE_ROW, WAVES, LANES };
 
 // N sums over the `span` lanes that share a row, the same in all of them.  Across wavefronts, at most 16: lane w of every 16 fetches wavefront w's sum from `box`, which holds N floats for each wavefront of
@@ -43,9 +43,9 @@ template <uint32_t N, int SHARE> __device__ __forceinline__ void row_sum(float (
     if (SHARE == LANES) {
 #pragma unroll
         for (uint32_t i = 0; i < N; ++i) {
-            v[i] = plus_dpp<0xB1>(v[i]);
-            v[i] = plus_dpp<0x4E>(v[i]);
-            v[i] = plus_dpp<0x141>(v[i]);
+            if (span >= 2u) v[i] = plus_dpp<0xB1>(v[i]);
+            if (span >= 4u) v[i] = plus_dpp<0x4E>(v[i]);
+            if (span >= 8u) v[i] = plus_dpp<0x141>(v[i]);
             if (span >= 16u) v[i] = plus_dpp<0x140>(v[i]);
             if (span >= 32u) v[i] += __shfl_xor(v[i], 16);
         }
@@ -199,7 +199,7 @@ template <int DT, int PT, uint32_t V, int SHARE, bool TAIL, bool NT, uint32_t N>
 
 // A run of rows to a workgroup: the parameters' gradients stay in registers over the run, and the row after the one at work
 // is on its way while the sums of this one cross the lanes.
-// SUB: rows of 8, 16 or 32 lanes, several to a wavefront, each taking every so many units of the run's rows (a unit: the rows
+// SUB: rows of 1 to 32 lanes, several to a wavefront, each taking every so many units of the run's rows (a unit: the rows
 // of one row of the gate where its gradient is written at once, else one row); their sums are joined at the run's end.
 // LEAN: rows too long for that many registers are read once more where they are needed again, out of the L2.
 //
@@ -294,13 +294,15 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool T
     };
     if (V > 1u) keep(POST, d_post), keep(PRE, d_pre), keep(GATE, d_gate);
     const float each = 1.0f / (float)cols;
+    bool fresh = false; // a gate that is asked for and not settled
     uint32_t gate_row = 0u, gate_end = 0u; // the row of the gate, and the row at which its next one begins
     auto take_gate = [&](uint32_t r) {
         gate_row = r / (uint32_t)a.d.rowsPerGate;
         gate_end = (gate_row + 1u) * (uint32_t)a.d.rowsPerGate;
         if (!LEAN) {
 #pragma unroll
-            for (uint32_t v = 0; v < HELD; ++v) gate[v] = param((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, v);
+            for (uint32_t v = 0; v < HELD; ++v) gate[v] = ask8<PT, TAIL, false>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols, tiny);
+            fresh = true;
         }
     };
     if (has_gate && row < end) take_gate(row);
@@ -337,6 +339,11 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool T
         const float r1 = inverse_rms(q[0], cols, a.d.eps), r2 = has_pre ? inverse_rms(q[1], cols, a.d.eps) : 0.0f;
         const float c2 = r2 * (q[2] * each); // mean of dz preWeight y / rms(y): r2 alone never underflows, its powers do
         float p[1] = {0.0f};
+        if (!LEAN && fresh) {
+#pragma unroll
+            for (uint32_t v = 0; v < HELD; ++v) settle8<PT, TAIL>(gate[v], (v * span + t) * 8u, cols, tiny);
+            fresh = false;
+        }
         // adds to the parameters' gradients and to p; o: g D postWeight, or g D
         auto group = [&](uint32_t v, float (&to_post)[8], float (&to_pre)[8], float (&to_gate)[8], float (&o)[8]) {
             apart();

@@ -314,11 +314,11 @@ int32_t HcommGfxMxProductKOnThread(
 
 /* ---- norms behind a fold ------------------------------------------------------------------------------------------------ */
 
-/* Lanes to a row of `cols` with `vecs` groups of eight elements each: 8, 16 or 32 of a wavefront, or whole wavefronts. */
+/* Lanes to a row of `cols` with `vecs` groups of eight elements each: 1 to 32 of a wavefront, or whole wavefronts. */
 static uint32_t row_span(uint64_t cols, uint32_t vecs)
 {
     const uint32_t lanes = (uint32_t)((cols + 8u * vecs - 1u) / (8u * vecs));
-    for (uint32_t s = 8; s <= 32u; s *= 2u)
+    for (uint32_t s = 1; s <= 32u; s *= 2u)
         if (lanes <= s) return s;
     return (lanes + 63u) / 64u * 64u;
 }

@@ -77,7 +77,7 @@ int hg_launch_mx_product(void* stream, const void* args);  /* HgMxProduct */
 typedef struct {
     HcommGfxReduceNormDesc d; /* .srcs is not followed on the device: */
     const void* src[HCOMM_GFX_MAX_RANKS];
-    uint32_t span;        /* lanes that share a row: 8, 16, 32 or whole wavefronts */
+    uint32_t span;        /* lanes that share a row: 1 to 32, a power of two, or whole wavefronts */
     uint32_t vecs;        /* groups of eight elements a lane holds */
     uint32_t rows_per_wg;
     uint32_t wgs;

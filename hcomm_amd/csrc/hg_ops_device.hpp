@@ -15,8 +15,25 @@ template <int DT> struct Raw8 {
 
 typedef u32x4 __attribute__((aligned(2))) u32x4_at2;
 typedef u32x4 __attribute__((aligned(4))) u32x4_at4;
-template <int DT> struct GroupVec { typedef u32x4_at2 type; };
-template <> struct GroupVec<DT_F32> { typedef u32x4_at4 type; };
+typedef uint32_t u32x2_raw __attribute__((ext_vector_type(2)));
+typedef u32x2_raw __attribute__((aligned(2))) u32x2_at2;
+typedef u32x2_raw __attribute__((aligned(4))) u32x2_at4;
+typedef uint32_t __attribute__((aligned(2))) u32_at2;
+// eight elements in one or two accesses; four, two and one of them
+template <int DT> struct GroupVec {
+    typedef u32x4_at2 type;
+    typedef u32x2_at2 half;
+    typedef u32_at2 quarter;
+    typedef uint16_t eighth;
+    static __device__ __forceinline__ uint32_t pair(const uint32_t* w) { return w[0]; }
+};
+template <> struct GroupVec<DT_F32> {
+    typedef u32x4_at4 type;
+    typedef u32x4_at4 half;
+    typedef u32x2_at4 quarter;
+    typedef uint32_t eighth;
+    static __device__ __forceinline__ u32x2_raw pair(const uint32_t* w) { return u32x2_raw{w[0], w[1]}; }
+};
 
 // Elements [at, at + 8) of a row of which `cols` are left; those past its end are 0.  TAIL: a row may end inside a group of
 // eight; without it a group is there or not.  NT: a cache hint for what is read (written) once and by no launch that follows
@@ -114,17 +131,29 @@ template <int DT, bool TAIL = true, bool NT = false> __device__ __forceinline__ 
             else ((wv*)p)[i] = v;
         }
     } else if (TAIL && at < cols) {
-        Raw8<DT> v = r;
-#pragma unroll 1
-        for (uint32_t e = 0, n = (uint32_t)(cols - at); e < n; ++e) {
-            st_elem<ES>(p + e * ES, ES == 4u ? v.w[0] : v.w[0] & 0xffffu);
-            // the next element takes the first one's place
+        // four, two and one elements as the count asks for them, the rest moved up behind each
+        typedef __attribute__((address_space(1))) typename GroupVec<DT>::half wh;
+        typedef __attribute__((address_space(1))) typename GroupVec<DT>::quarter wq;
+        typedef __attribute__((address_space(1))) typename GroupVec<DT>::eighth we;
+        const uint32_t n = (uint32_t)(cols - at);
+        constexpr uint32_t H = Raw8<DT>::words / 2u, Q = H / 2u;
+        uint32_t w[H];
 #pragma unroll
-            for (uint32_t i = 0; i < Raw8<DT>::words; ++i) {
-                const uint32_t above = i + 1u < Raw8<DT>::words ? v.w[i + 1u < Raw8<DT>::words ? i + 1u : i] : 0u;
-                v.w[i] = ES == 4u ? above : (v.w[i] >> 16) | (above << 16);
-            }
+        for (uint32_t i = 0; i < H; ++i) w[i] = r.w[i];
+        if (n & 4u) {
+            typename GroupVec<DT>::half v;
+#pragma unroll
+            for (uint32_t i = 0; i < H; ++i) v[i] = w[i], w[i] = r.w[H + i];
+            *(wh*)p = v;
+            p += 4u * ES;
         }
+        if (n & 2u) {
+            *(wq*)p = GroupVec<DT>::pair(w);
+            p += 2u * ES;
+#pragma unroll
+            for (uint32_t i = 0; i < Q; ++i) w[i] = w[Q + i];
+        }
+        if (n & 1u) *(we*)p = (typename GroupVec<DT>::eighth)w[0];
     }
 }
 

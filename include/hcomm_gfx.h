@@ -1040,8 +1040,8 @@ uint64_t HcommGfxSetPieceBytes(uint64_t bytes);
  * Dense matrices are row-major, `Stride` is the distance of two rows in ELEMENTS and at least the row's length; any
  * element-aligned address and any stride are taken.  Nothing outside the rows x cols elements is read or written.
  * Dense types: FP16, BFP16, FP32.  Outputs overlap no input and no other output unless a call says so.
- * A call whose launch would need 2^32 lanes or more is beyond the library's limit: a lane takes up to eight elements of a row, a row of
- * a norm eight lanes or more, a result of a product two at most.
+ * A call whose launch would need 2^32 lanes or more is beyond the library's limit: a lane takes up to eight elements of a row, a
+ * result of a product two lanes at most.
  * The work runs on the device of the thread's stream, whatever the caller's current device.
  * ------------------------------------------------------------------------------------------- */
 

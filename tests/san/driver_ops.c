@@ -42,7 +42,7 @@ int hg_launch_norm(void* s, const void* args)
     (void)s; ++met[3];
     grid(a->wgs, a->span * a->rows_per_wg);
     expect(a->span * a->rows_per_wg <= 1024 && (uint64_t)a->span * a->vecs * 8 >= a->d.cols && (uint64_t)a->wgs * a->rows_per_wg >= a->d.rows, "norm");
-    expect(a->span >= 64 ? a->span % 64 == 0 && (a->rows_per_wg == 1 || a->span <= 128) : a->span == 8 || a->span == 16 || a->span == 32, "span");
+    expect(a->span >= 64 ? a->span % 64 == 0 && (a->rows_per_wg == 1 || a->span <= 128) : a->span > 0 && a->span <= 32 && (a->span & (a->span - 1)) == 0, "span");
     return 0;
 }
 int hg_launch_norm_grad(void* s, const void* args)
@@ -51,11 +51,11 @@ int hg_launch_norm_grad(void* s, const void* args)
     const uint64_t lanes = a->span < 64 ? 64 : a->span, rows = a->d.rows;
     (void)s; ++met[4];
     grid(a->chunks, lanes);
-    expect(lanes <= 1024 && (uint64_t)a->span * a->vecs * 8 >= a->d.cols && a->pitch >= a->d.cols && a->pitch % 64 == 0 && a->pitch <= a->span * a->vecs * 8, "lanes");
+    expect(lanes <= 1024 && (uint64_t)a->span * a->vecs * 8 >= a->d.cols && a->pitch >= a->d.cols && a->pitch % 64 == 0 && (a->span < 64 || a->pitch <= a->span * a->vecs * 8), "lanes");
     expect(a->chunks * a->sums * a->pitch * 4 <= a->d.workspaceBytes, "workspace");
     if (a->by_gate) expect(a->chunks_per_gate * a->chunk_rows >= a->d.rowsPerGate && a->chunks == a->chunks_per_gate * a->gates && a->gates * a->d.rowsPerGate >= rows, "runs of a gate");
     else expect(a->chunks * a->chunk_rows >= rows && a->unit > 0 && (!a->d.dGate || (a->chunk_rows % a->d.rowsPerGate == 0 && a->unit == a->d.rowsPerGate)), "runs");
-    expect(a->chunk_rows < (1ull << 32) && (uint64_t)a->unit * 8 + rows < (1ull << 32), "32 bits");
+    expect(a->chunk_rows < (1ull << 32) && (uint64_t)a->unit * 64 + rows < (1ull << 32), "32 bits");
     return 0;
 }
 int hg_launch_norm_sums(void* s, const void* args)

@@ -346,9 +346,9 @@ def test_ends_of_rows(gpu_thread, t, p):
 
 
 @pytest.mark.parametrize("rows,per", [(6200, 2), (6149, 3), (700, 2), (1030, 257), (530, 0), (300, 1000), (9, 1), (1, 1)])
-@pytest.mark.parametrize("cols,t,p", [(64, "bf16", "fp32"), (65, "fp32", "fp32"), (128, "fp16", "fp16"), (203, "bf16", "bf16"), (256, "fp32", "fp32"), (257, "bf16", "fp32")])
+@pytest.mark.parametrize("cols,t,p", [(3, "fp16", "fp32"), (8, "fp32", "fp32"), (9, "bf16", "bf16"), (16, "fp16", "fp16"), (31, "bf16", "fp32"), (33, "fp32", "fp32"), (64, "bf16", "fp32"), (65, "fp32", "fp32"), (128, "fp16", "fp16"), (203, "bf16", "bf16"), (256, "fp32", "fp32"), (257, "bf16", "fp32")])
 def test_rows_that_share_a_wavefront(gpu_thread, rows, per, cols, t, p):
-    """8, 16 and 32 lanes to a row and the first length of a wavefront of its own; gates inside a set of lanes' rows and across sets."""
+    """1 to 32 lanes to a row and the first length of a wavefront of its own; gates inside a set of lanes' rows and across sets."""
     Case(rows, cols, t, k=2, per=per, p=p, pad=5 * (cols % 2)).run(gpu_thread)
 
 
