@@ -138,6 +138,7 @@ template <uint32_t N> struct ProductArgs {
 // a fixed order.
 // SHORT: ranks of fewer than 16 blocks.  A chunk holds fours of blocks there, EACH of them: those of one rank, so that the
 // ranks spread over the wavefronts, or with a single wavefront the next four of all ranks' fours.
+// One row of 8 ranks' 1,024 columns times 8,192 rows: 7.4 us for 35.7 MB, bound by the loads' latency and memory.
 template <int DT, int FA, int FB, uint32_t W, bool SHORT, uint32_t N> __global__ __launch_bounds__(64 * W) void k_mx_product_direct(const ProductArgs<N> a)
 {
     __shared__ f32x4 part[W > 1u ? W : 1u][W > 1u ? FA * FB : 1][W > 1u ? 64 : 1];
@@ -266,6 +267,8 @@ template <int DT, int FA, int FB, uint32_t W, bool SHORT, uint32_t N> __global__
 // the lanes that need them, each would touch 32 lines for a quarter of the lanes' worth of new bytes.
 // The wavefronts meet once a stage, before its last quarter is multiplied: by then everything of the stage is in
 // registers, its buffer takes the stage after the next, and the fragments of the next one arrive behind that quarter.
+// 4,096 x 8,192 results of 8 x 1,024 columns: 138 us, 4.0 PFLOP/s.  The matrix instructions alone would take 90 (random operands
+// hold the clock down: 6.1 PFLOP/s), all of it without the copies 120; what is left is the copies' latency at 64 KiB a stage.
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint64_t u64_at1 __attribute__((aligned(1)));
