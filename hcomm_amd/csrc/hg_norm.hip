@@ -67,7 +67,14 @@ template <uint32_t N, int SHARE> __device__ __forceinline__ void row_sum(float (
     for (uint32_t i = 0; i < N; ++i) v[i] = sum16(w < waves ? box[(first + w) * N + i] : 0.0f);
 }
 
-__device__ __forceinline__ float inverse_rms(float squares, uint64_t cols, float eps) { return 1.0f / sqrtf(squares / (float)cols + eps); }
+// 1 / rms of a row from its sum of squares, `each` = 1 / its length.  The instruction is good to one unit in the last place, of
+// normal numbers.
+__device__ __forceinline__ float inverse_rms(float squares, float each, float eps)
+{
+    const float m = fmaf(squares, each, eps);
+    const bool small = m < 0x1p-100f;
+    return __builtin_amdgcn_rsqf(small ? m * 0x1p100f : m) * (small ? 0x1p50f : 1.0f);
+}
 
 #define MAX_WAVES 16u
 
@@ -93,6 +100,7 @@ template <int DT, int PT, uint32_t V, int SHARE, bool TAIL, bool NT, uint32_t N>
     const uint64_t row = ONE ? blockIdx.x : (uint64_t)blockIdx.x * a.rows_per_wg + local;
     const uint64_t cols = ONE || row < a.d.rows ? a.d.cols : 0u; // a row that is not there has no columns
     const bool tiny = a.d.cols < 8u;
+    const float each = 1.0f / (float)a.d.cols;
     float f[V][8];
     Raw8<DT> x[AHEAD][V], res[V];
     Raw8<PT> post[V], pre[V], gate[V];
@@ -155,7 +163,7 @@ template <int DT, int PT, uint32_t V, int SHARE, bool TAIL, bool NT, uint32_t N>
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e) s[0] = fmaf(f[v][e], f[v][e], s[0]);
         row_sum<1, SHARE>(s, box[0], span);
-        const float r = inverse_rms(s[0], a.d.cols, a.d.eps);
+        const float r = inverse_rms(s[0], each, a.d.eps);
 #pragma unroll
         for (uint32_t v = 0; v < V; ++v) {
             float w[8];
@@ -185,7 +193,7 @@ template <int DT, int PT, uint32_t V, int SHARE, bool TAIL, bool NT, uint32_t N>
     }
     if (a.d.preWeight) {
         row_sum<1, SHARE>(s, box[1], span);
-        const float r = inverse_rms(s[0], a.d.cols, a.d.eps);
+        const float r = inverse_rms(s[0], each, a.d.eps);
 #pragma unroll
         for (uint32_t v = 0; v < V; ++v) {
             float w[8];
@@ -203,19 +211,22 @@ template <int DT, int PT, uint32_t V, int SHARE, bool TAIL, bool NT, uint32_t N>
 // is on its way while the sums of this one cross the lanes.
 // SUB: rows of 1 to 32 lanes, several to a wavefront, each taking every so many units of the run's rows (a unit: the rows
 // of one row of the gate where its gradient is written at once, else one row); their sums are joined at the run's end.
-// LEAN: rows too long for that many registers are read once more where they are needed again, out of the L2.
+// LEAN: rows so long that neither the next one nor the parameters have registers beside them: those are asked for again.
+// What is not there is taken as what leaves the formulas as they are (a gate of 1, a dz of 0), not by branches around them.
 //
 // Which of them, for 33.5M elements in bf16, us:
-//   SUB up to 256 columns: 99 at 64 columns, 419 with a wavefront to each row (56 of its lanes idle);
-//   V = 1 up to 4,096: 88 to 95, 4.5 TB/s of 5.1 that a copy reaches;
-//   V = 2 up to 8,192, 8 wavefronts of 256 registers, the second group's sums in LDS: 88 to 112 (fp32 195; 258 with these sums
+//   SUB up to 256 columns: 96 at 64 columns, 419 with a wavefront to each row (56 of its lanes idle);
+//   V = 1 up to 4,096: 82 to 95, 4.9 to 4.2 TB/s of 5.1 that a copy reaches;
+//   V = 2 up to 8,192, 8 wavefronts of 256 registers, the second group's sums in LDS: 88 to 93 (fp32 190; 258 with these sums
 //   in registers that spill); LEAN with V = 1 and 16 wavefronts: 200;
-//   LEAN with V = 2 above: 228 to 255, 815 and more with everything held and spilled.  A row's loads are waited for three
-//   times there, with one workgroup to a CU: bound by their latency.
+//   LEAN with V = 2 above: 167 to 170 (fp32 270 to 285); 815 and more with everything held and spilled, 228 to 255 (fp32 335) with
+//   rows read again for each of their uses.  Bound by the latency of a row's loads, with one workgroup to a CU.
 template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool TAIL, bool NT> __global__ __launch_bounds__(MOST) void k_norm_grad(const HgNormGrad a)
 {
     __shared__ float box_a[MAX_WAVES * 3], box_b[MAX_WAVES];
     constexpr uint32_t ES = ElemSize<DT>::v, PS = ElemSize<PT>::v;
+    constexpr int SHARE = SUB ? LANES : ONE_ROW;
+    constexpr int HT = V == 1u ? DT_F32 : PT; // parameters are held as this
     constexpr bool PASS = NT && !LEAN;
     const uint32_t span = a.span;
     uint32_t t = SUB ? threadIdx.x & (span - 1u) : threadIdx.x;
@@ -237,28 +248,42 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool T
     uint32_t unit_end = SUB ? row + unit : 0u;
     auto after = [&](uint32_t r) { return SUB && r + 1u == unit_end ? r + 1u + (sets - 1u) * unit : r + 1u; };
     struct Row {
-        Raw8<DT> s, y, dy, dz;
+        Raw8<DT> s, y, dy, dz; // without a norm in front of the next block y and dz stay 0
     };
-    constexpr uint32_t HELD = LEAN ? 1u : V; // groups whose rows and parameters stay in registers
-    auto ask_one = [&](const void* m, uint64_t stride, uint32_t r, uint32_t v) {
-        return ask8<DT, TAIL, PASS>((const uint8_t*)m + r * stride * ES, (v * span + t) * 8u, cols, tiny);
+    constexpr uint32_t HELD = LEAN ? 1u : V; // groups whose parameters are held
+    auto ask_one = [&](Raw8<DT>& x, const void* m, uint64_t stride, uint32_t r, uint32_t v) {
+        x = ask8<DT, TAIL, PASS>((const uint8_t*)m + r * stride * ES, (v * span + t) * 8u, cols, tiny);
     };
-    auto ask = [&](Row& x, uint32_t r, uint32_t v, bool with_dy) {
-        x.s = ask_one(a.d.sum, a.d.sumStride, r, v);
-        if (has_pre) x.y = ask_one(a.d.y, a.d.yStride, r, v), x.dz = ask_one(a.d.dz, a.d.dzStride, r, v);
-        if (with_dy) x.dy = ask_one(a.d.dy, a.d.dyStride, r, v);
+    auto ask = [&](Row& x, uint32_t r, uint32_t v) {
+        ask_one(x.s, a.d.sum, a.d.sumStride, r, v);
+        if (has_pre) ask_one(x.y, a.d.y, a.d.yStride, r, v), ask_one(x.dz, a.d.dz, a.d.dzStride, r, v);
+        else if (LEAN) x.y = x.dz = zeros8<DT>(); // not held from row to row
+        ask_one(x.dy, a.d.dy, a.d.dyStride, r, v);
+    };
+    auto ask_row = [&](Row (&x)[V], uint32_t r) {
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v) ask(x[v], r, v);
     };
     auto settle = [&](Raw8<DT>& x, uint32_t v) { settle8<DT, TAIL>(x, (v * span + t) * 8u, cols, tiny); };
-    auto settle_row = [&](Row& x, uint32_t v, bool with_dy) {
+    auto settle_row = [&](Row& x, uint32_t v) {
         settle(x.s, v);
         if (has_pre) settle(x.y, v), settle(x.dz, v);
-        if (with_dy) settle(x.dy, v);
+        settle(x.dy, v);
     };
-    auto param = [&](const void* m, uint32_t v) {
-        Raw8<PT> p = ask8<PT, TAIL, false>(m, (v * span + t) * 8u, cols, tiny);
+    // A parameter's group in fp32; one that is not there: what leaves the formulas as they are without it.
+    auto param = [&](const void* m, uint32_t v, float missing, float (&w)[8]) {
+        const float each_is[8] = {missing, missing, missing, missing, missing, missing, missing, missing};
+        Raw8<PT> p = narrow8<PT>(each_is);
+        if (m) ask8_into<PT, TAIL, false>(p, m, (v * span + t) * 8u, cols, tiny);
         settle8<PT, TAIL>(p, (v * span + t) * 8u, cols, tiny);
-        return p;
+        widen8<PT>(p, w);
     };
+    auto hold = [&](const void* m, uint32_t v, float missing) {
+        float w[8];
+        param(m, v, missing, w);
+        return narrow8<HT>(w); // exact: fp32, or the type it came in
+    };
+    auto gate_at = [&](uint32_t r) { return has_gate ? (const uint8_t*)a.d.gate + r * a.d.gateStride * PS : (const uint8_t*)nullptr; };
     // What a lane asks for behind this is not asked for before it: LEAN has room for little at a time.
     auto apart = [] {
         if (LEAN) {
@@ -266,20 +291,32 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool T
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    Row next[HELD];
-    auto ask_next = [&](uint32_t r) {
+    Row next[V];
 #pragma unroll
-        for (uint32_t v = 0; v < HELD; ++v) ask(next[v], r, v, true);
+    for (uint32_t v = 0; v < V; ++v) next[v].y = next[v].dz = zeros8<DT>();
+    if (!LEAN && row < end) ask_row(next, row);
+    uint32_t gate_row = 0u, gate_end = 0u; // the row of the gate, and the row at which its next one begins
+    Raw8<HT> post[HELD], pre[HELD], gate[HELD];
+    Raw8<PT> asked[HT == PT ? 1u : HELD]; // a row of the gate that is asked for and not settled, where `fresh`; else it goes to `gate` at once
+    bool fresh = false;
+    auto take_gate = [&](uint32_t r) {
+        gate_row = r / (uint32_t)a.d.rowsPerGate;
+        gate_end = (gate_row + 1u) * (uint32_t)a.d.rowsPerGate;
+        if (!LEAN) {
+#pragma unroll
+            for (uint32_t v = 0; v < HELD; ++v) {
+                const uint32_t at = (v * span + t) * 8u;
+                if constexpr (HT == PT) gate[v] = ask8<PT, TAIL, false>(gate_at(gate_row), at, cols, tiny);
+                else asked[v] = ask8<PT, TAIL, false>(gate_at(gate_row), at, cols, tiny);
+            }
+            fresh = true;
+        }
     };
-    if (!LEAN && row < end) ask_next(row);
-    Raw8<PT> post[HELD], pre[HELD], gate[HELD];
     if (!LEAN) {
 #pragma unroll
-        for (uint32_t v = 0; v < HELD; ++v) {
-            if (has_pre) pre[v] = param(a.d.preWeight, v);
-            if (has_post) post[v] = param(a.d.postWeight, v);
-        }
+        for (uint32_t v = 0; v < HELD; ++v) pre[v] = hold(a.d.preWeight, v, 0.0f), post[v] = hold(a.d.postWeight, v, 1.0f), gate[v] = hold(nullptr, v, 1.0f);
     }
+    if (has_gate && row < end) take_gate(row);
     float d_post[8], d_pre[8], d_gate[8];
 #pragma unroll
     for (uint32_t e = 0; e < 8u; ++e) d_post[e] = d_pre[e] = d_gate[e] = 0.0f;
@@ -296,75 +333,70 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool T
     };
     if (V > 1u) keep(POST, d_post), keep(PRE, d_pre), keep(GATE, d_gate);
     const float each = 1.0f / (float)cols;
-    bool fresh = false; // a gate that is asked for and not settled
-    uint32_t gate_row = 0u, gate_end = 0u; // the row of the gate, and the row at which its next one begins
-    auto take_gate = [&](uint32_t r) {
-        gate_row = r / (uint32_t)a.d.rowsPerGate;
-        gate_end = (gate_row + 1u) * (uint32_t)a.d.rowsPerGate;
-        if (!LEAN) {
-#pragma unroll
-            for (uint32_t v = 0; v < HELD; ++v) gate[v] = ask8<PT, TAIL, false>((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, (v * span + t) * 8u, cols, tiny);
-            fresh = true;
-        }
-    };
-    if (has_gate && row < end) take_gate(row);
     while (row < end) {
         const uint32_t following = after(row);
         if (LEAN) asm volatile("" : "+v"(t)); // no addresses held from row to row
-        Row x[HELD];
+        Row x[V];
         if (!LEAN) {
 #pragma unroll
-            for (uint32_t v = 0; v < HELD; ++v) x[v] = next[v];
-            if (following < end) ask_next(following);
-#pragma unroll
-            for (uint32_t v = 0; v < HELD; ++v) settle_row(x[v], v, true);
+            for (uint32_t v = 0; v < V; ++v) x[v] = next[v];
+            if (following < end) ask_row(next, following);
+        } else {
+            ask_row(x, row);
         }
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v) settle_row(x[v], v);
         float q[3] = {0.0f, 0.0f, 0.0f}; // sum^2, y^2, dz preWeight y
 #pragma unroll
         for (uint32_t v = 0; v < V; ++v) {
-            Row& h = x[LEAN ? 0u : v];
-            if (LEAN) ask(h, row, v, false), settle_row(h, v, false);
-            float s[8];
+            Row& h = x[v];
+            float s[8], y[8], z[8], w[8];
             widen8<DT>(h.s, s);
+            widen8<DT>(h.y, y);
+            widen8<DT>(h.dz, z);
+            if (LEAN) param(a.d.preWeight, v, 0.0f, w);
+            else widen8<HT>(pre[LEAN ? 0u : v], w);
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e) q[0] = fmaf(s[e], s[e], q[0]);
-            if (has_pre) {
-                float y[8], z[8], w[8];
-                widen8<DT>(h.y, y);
-                widen8<DT>(h.dz, z);
-                widen8<PT>(LEAN ? param(a.d.preWeight, v) : pre[LEAN ? 0u : v], w);
-#pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e) q[1] = fmaf(y[e], y[e], q[1]), q[2] = fmaf(z[e] * w[e], y[e], q[2]);
+            for (uint32_t e = 0; e < 8u; ++e) {
+                q[0] = fmaf(s[e], s[e], q[0]);
+                q[1] = fmaf(y[e], y[e], q[1]);
+                q[2] = fmaf(z[e] * w[e], y[e], q[2]);
             }
         }
-        row_sum<3, SUB ? LANES : ONE_ROW>(q, box_a, span);
-        const float r1 = inverse_rms(q[0], cols, a.d.eps), r2 = has_pre ? inverse_rms(q[1], cols, a.d.eps) : 0.0f;
-        const float c2 = r2 * (q[2] * each); // mean of dz preWeight y / rms(y): r2 alone never underflows, its powers do
+        row_sum<3, SHARE>(q, box_a, span);
+        const float r1 = has_post ? inverse_rms(q[0], each, a.d.eps) : 1.0f, r2 = has_pre ? inverse_rms(q[1], each, a.d.eps) : 0.0f;
+        const float c2 = r2 * (r2 * (q[2] * each)); // mean of dz preWeight y / rms(y), by 1 / rms(y): r2 y never underflows with y
         float p[1] = {0.0f};
         if (!LEAN && fresh) {
 #pragma unroll
-            for (uint32_t v = 0; v < HELD; ++v) settle8<PT, TAIL>(gate[v], (v * span + t) * 8u, cols, tiny);
+            for (uint32_t v = 0; v < HELD; ++v) {
+                const uint32_t at = (v * span + t) * 8u;
+                if constexpr (HT == PT) settle8<PT, TAIL>(gate[v], at, cols, tiny);
+                else {
+                    float w[8];
+                    settle8<PT, TAIL>(asked[v], at, cols, tiny);
+                    widen8<PT>(asked[v], w);
+                    gate[v] = narrow8<HT>(w);
+                }
+            }
             fresh = false;
         }
-        // adds to the parameters' gradients and to p; o: g D postWeight, or g D
+        // adds to the parameters' gradients and to p; n: s / rms(s) or s, o: g D postWeight
         auto group = [&](uint32_t v, float (&to_post)[8], float (&to_pre)[8], float (&to_gate)[8], float (&o)[8]) {
             apart();
-            Row& h = x[LEAN ? 0u : v];
-            if (LEAN) ask(h, row, v, true), settle_row(h, v, true);
-            float s[8], d[8];
+            Row& h = x[v];
+            float s[8], d[8], y[8], z[8], w[8], g[8];
             widen8<DT>(h.s, s);
             widen8<DT>(h.dy, d);
-            if (has_pre) {
-                float y[8], z[8], w[8];
-                widen8<DT>(h.y, y);
-                widen8<DT>(h.dz, z);
-                widen8<PT>(LEAN ? param(a.d.preWeight, v) : pre[LEAN ? 0u : v], w);
+            widen8<DT>(h.y, y);
+            widen8<DT>(h.dz, z);
+            if (LEAN) param(a.d.preWeight, v, 0.0f, w);
+            else widen8<HT>(pre[LEAN ? 0u : v], w);
 #pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e) {
-                    const float n = y[e] * r2;
-                    to_pre[e] = fmaf(z[e], n, to_pre[e]);
-                    d[e] = fmaf(r2, fmaf(z[e], w[e], -c2 * n), d[e]);
-                }
+            for (uint32_t e = 0; e < 8u; ++e) {
+                const float n = y[e] * r2;
+                to_pre[e] = fmaf(z[e], n, to_pre[e]);
+                d[e] = fmaf(-c2, n, fmaf(r2, z[e] * w[e], d[e]));
             }
             if (a.d.dResidual) {
                 float res[8];
@@ -372,22 +404,16 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool T
                 for (uint32_t e = 0; e < 8u; ++e) res[e] = a.d.residualScale * d[e];
                 store8<DT, TAIL, NT>((uint8_t*)a.d.dResidual + row * a.d.dResidualStride * ES, (v * span + t) * 8u, cols, narrow8<DT>(res));
             }
-            float w[8], g[8];
-            if (has_post) widen8<PT>(LEAN ? param(a.d.postWeight, v) : post[LEAN ? 0u : v], w);
-            if (has_gate) widen8<PT>(LEAN ? param((const uint8_t*)a.d.gate + gate_row * a.d.gateStride * PS, v) : gate[LEAN ? 0u : v], g);
+            if (LEAN) param(a.d.postWeight, v, 1.0f, w), param(gate_at(gate_row), v, 1.0f, g);
+            else widen8<HT>(post[LEAN ? 0u : v], w), widen8<HT>(gate[LEAN ? 0u : v], g);
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e) {
-                const float n = has_post ? s[e] * r1 : s[e];
-                if (has_gate) {
-                    to_gate[e] = fmaf(d[e], has_post ? n * w[e] : n, to_gate[e]);
-                    d[e] *= g[e];
-                }
-                if (has_post) {
-                    to_post[e] = fmaf(d[e], n, to_post[e]);
-                    d[e] *= w[e];
-                    p[0] = fmaf(d[e], s[e], p[0]);
-                }
-                o[e] = d[e];
+                const float n = s[e] * r1;
+                to_gate[e] = fmaf(d[e], n * w[e], to_gate[e]);
+                d[e] *= g[e];
+                to_post[e] = fmaf(d[e], n, to_post[e]);
+                o[e] = d[e] * w[e];
+                p[0] = fmaf(o[e], s[e], p[0]);
             }
         };
         float first[8];
@@ -400,7 +426,7 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool T
         }
         float c1 = 0.0f;
         if (has_post) {
-            row_sum<1, SUB ? LANES : ONE_ROW>(p, box_b, span);
+            row_sum<1, SHARE>(p, box_b, span);
             c1 = r1 * (p[0] * each);
         } else if (span > 64u) {
             __syncthreads(); // box_a is free for the next row
@@ -408,10 +434,8 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool T
         auto finish = [&](uint32_t v, float (&o)[8]) {
             apart();
             if (has_post) {
-                Row& h = x[LEAN ? 0u : v];
-                if (LEAN) h.s = ask_one(a.d.sum, a.d.sumStride, row, v), settle(h.s, v);
                 float s[8];
-                widen8<DT>(h.s, s);
+                widen8<DT>(x[v].s, s);
 #pragma unroll
                 for (uint32_t e = 0; e < 8u; ++e) o[e] = r1 * fmaf(-c1, s[e] * r1, o[e]);
             }

@@ -39,14 +39,14 @@ template <> struct GroupVec<DT_F32> {
 // eight; without it a group is there or not.  NT: a cache hint for what is read (written) once and by no launch that follows
 // soon.  A group that the row's end cuts is read as the row's last eight elements, which settle8, called where the group is
 // used, moves to where they belong: no load waits for another.  `short_row`: the whole row has fewer than eight (uniform).
-template <int DT, bool TAIL, bool NT> __device__ __forceinline__ Raw8<DT> ask8(const void* row, uint32_t at, uint64_t cols, bool short_row)
+// ask8_into: where a row ends before the group, what was there stays (a buffer that is used again needs its zeros once).
+template <int DT, bool TAIL, bool NT> __device__ __forceinline__ void ask8_into(Raw8<DT>& r, const void* row, uint32_t at, uint64_t cols, bool short_row)
 {
     constexpr uint32_t ES = ElemSize<DT>::v, W = Raw8<DT>::words;
     typedef const __attribute__((address_space(1))) typename GroupVec<DT>::type cv;
-    Raw8<DT> r;
-#pragma unroll
-    for (uint32_t i = 0; i < W; ++i) r.w[i] = 0u;
     if (TAIL && short_row) {
+#pragma unroll
+        for (uint32_t i = 0; i < W; ++i) r.w[i] = 0u;
         // from the last element on, each moves those behind it up by one place
 #pragma unroll 1
         for (uint32_t e = at == 0u ? (uint32_t)cols : 0u; e-- != 0u;) {
@@ -57,7 +57,7 @@ template <int DT, bool TAIL, bool NT> __device__ __forceinline__ Raw8<DT> ask8(c
                 r.w[i] = ES == 4u ? (i ? below : x) : (r.w[i] << 16) | (i ? below >> 16 : x);
             }
         }
-        return r;
+        return;
     }
     if (at < cols) {
         const int32_t back = TAIL && at + 8u > cols ? (int32_t)(at + 8u - (uint32_t)cols) : 0; // may reach in front of `row`, not of the whole row
@@ -68,6 +68,18 @@ template <int DT, bool TAIL, bool NT> __device__ __forceinline__ Raw8<DT> ask8(c
             r.w[4 * i] = v.x, r.w[4 * i + 1] = v.y, r.w[4 * i + 2] = v.z, r.w[4 * i + 3] = v.w;
         }
     }
+}
+template <int DT> __device__ __forceinline__ Raw8<DT> zeros8()
+{
+    Raw8<DT> r;
+#pragma unroll
+    for (uint32_t i = 0; i < Raw8<DT>::words; ++i) r.w[i] = 0u;
+    return r;
+}
+template <int DT, bool TAIL, bool NT> __device__ __forceinline__ Raw8<DT> ask8(const void* row, uint32_t at, uint64_t cols, bool short_row)
+{
+    Raw8<DT> r = zeros8<DT>();
+    ask8_into<DT, TAIL, NT>(r, row, at, cols, short_row);
     return r;
 }
 

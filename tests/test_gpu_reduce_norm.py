@@ -1,8 +1,8 @@
 """The norms, gate and residual behind a fold, and their gradient, against their formulas in 64 bits.
 
 Bounds count roundings of fp32 (u = 2^-24).  A sum over a row of at most 16,384 elements goes through at most 16 additions in a
-lane, 6 between lanes and 16 between wavefronts, so a sum of squares is off by at most 40 u relative and 1 / rms by half
-of that and its square root and division: RHO = 24 u.  The output's own rounding is added by close()."""
+lane, 6 between lanes and 16 between wavefronts, so a sum of squares is off by at most 40 u relative, the mean by 2 u more and
+1 / rms by half of that and an instruction good to one unit in the last place (2 u): 23 u, RHO = 24 u.  The output's own rounding is added by close()."""
 import numpy as np
 import pytest
 import torch
@@ -379,3 +379,22 @@ def test_gradients_over_their_inputs(gpu_thread, cols, t):
         h.check(h.HcommGfxThreadSynchronize(gpu_thread))
         for n, got in zip(results, (ds, dres, "dpost", "dpre", "dgate")):
             assert torch.equal(getattr(b, got).view, want[n]), (ds, dres, n)
+
+
+@pytest.mark.parametrize("power", [0, -60, 50])
+def test_small_and_large_rows_without_eps(gpu_thread, power):
+    """1 / rms scales with the row: means of squares of 2^-120 and 2^100 and eps = 0 leave z as it is for rows around 1."""
+    rows, cols = 3, 200
+    rng = np.random.default_rng(11)
+    x = rng.standard_normal((rows, cols)).astype(np.float32)
+    src, y, z = Dense(rows, cols, "fp32", cols, 0, x.astype(np.float64) * 2.0 ** power), Dense(rows, cols, "fp32"), Dense(rows, cols, "fp32")
+    w = Dense(1, cols, "fp32", cols, 0, 1 + 0.2 * rng.standard_normal((1, cols)))
+    d = h.ReduceNormDesc(srcs=[src.ptr], srcStride=cols, rows=rows, cols=cols, dataType=h.HcommDataType.FP32, paramType=h.HcommDataType.FP32,
+                         residualScale=1.0, eps=0.0, y=y.ptr, yStride=cols, z=z.ptr, zStride=cols, preWeight=w.ptr)
+    torch.cuda.synchronize()
+    h.check(h.HcommGfxReduceNormOnThread(gpu_thread, d))
+    h.check(h.HcommGfxThreadSynchronize(gpu_thread))
+    v = x.astype(np.float64)
+    want = v / np.sqrt((v * v).mean(1, keepdims=True)) * w.double()
+    close(z.double(), want, "fp32", np.abs(want) * (RHO + 2 * U), "z")
+    assert np.array_equal(y.double(), v * 2.0 ** power)
