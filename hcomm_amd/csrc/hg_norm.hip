@@ -467,15 +467,18 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool T
     }
     // this run's sums; rows that shared a wavefront's lanes are joined first
     float* mine = (float*)a.d.workspace + (uint64_t)blockIdx.x * a.sums * a.pitch;
-    auto leave = [&](int at, int which, float (&d)[8]) {
-        if (at < 0) return;
+    auto join = [&](float (&d)[8]) {
         if (SUB) {
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e)
                 for (uint32_t far = span; far < 64u; far *= 2u) d[e] += __shfl_xor(d[e], (int)far);
         }
+        return !SUB || threadIdx.x < span; // who leaves them
+    };
+    auto leave = [&](int at, int which, float (&d)[8]) {
+        if (at < 0) return;
         // the workspace's rows hold whole groups
-        if (!SUB || threadIdx.x < span) store8<DT_F32, false>(mine + (uint64_t)at * a.pitch, t * 8u, a.pitch, narrow8<DT_F32>(d));
+        if (join(d)) store8<DT_F32, false>(mine + (uint64_t)at * a.pitch, t * 8u, a.pitch, narrow8<DT_F32>(d));
         if (V > 1u) {
             float o[8];
             kept(which, o);
@@ -485,6 +488,15 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool T
     leave(a.at_post, POST, d_post);
     leave(a.at_pre, PRE, d_pre);
     leave(a.at_gate, GATE, d_gate);
+    if (a.by_gate && a.at_gate < 0) { // the run has all rows of its row of the gate
+        uint8_t* to = (uint8_t*)a.d.dGate + blockIdx.x * a.d.dGateStride * PS;
+        if (join(d_gate)) store8<PT, TAIL>(to, t * 8u, cols, narrow8<PT>(d_gate));
+        if (V > 1u) {
+            float o[8];
+            kept(GATE, o);
+            store8<PT, TAIL>(to, (span + t) * 8u, cols, narrow8<PT>(o));
+        }
+    }
 }
 
 // The runs' sums joined, in a fixed order (4 us: the latency of a launch and of a chain of loads): a workgroup takes 64 columns of one result, four neighbours to a lane, and 64

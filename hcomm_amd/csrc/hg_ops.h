@@ -87,8 +87,8 @@ typedef struct {
 /*
  * The gradient walks the rows in `chunks` runs of `chunk_rows` rows, one workgroup a run, and joins the runs' sums in a
  * second launch.  by_gate: a run never crosses from one row of the gate to the next (`chunks_per_gate` runs to each), so
- * that the gate's gradient is joined from runs too; otherwise every run holds whole gate rows and writes their
- * gradients itself.
+ * that the gate's gradient is joined from runs too, where there is more than one to a row of it; otherwise every run holds
+ * whole gate rows and writes their gradients itself.
  */
 typedef struct {
     HcommGfxReduceNormGradDesc d;

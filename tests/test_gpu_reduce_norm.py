@@ -398,3 +398,10 @@ def test_small_and_large_rows_without_eps(gpu_thread, power):
     want = v / np.sqrt((v * v).mean(1, keepdims=True)) * w.double()
     close(z.double(), want, "fp32", np.abs(want) * (RHO + 2 * U), "z")
     assert np.array_equal(y.double(), v * 2.0 ** power)
+
+
+@pytest.mark.parametrize("rows,per", [(536, 1), (300, 2), (1999, 3), (255, 9), (1300, 20), (5, 4)])
+@pytest.mark.parametrize("cols,t,p", [(20, "fp32", "fp32"), (132, "fp16", "fp16"), (626, "bf16", "fp32"), (5001, "bf16", "bf16"), (9000, "fp32", "fp32")])
+def test_a_row_of_the_gate_in_one_run(gpu_thread, rows, per, cols, t, p):
+    """Fewer gate rows than runs, each with so few rows that one run has them all."""
+    Case(rows, cols, t, k=1, per=per, p=p, pad=cols % 3).run(gpu_thread)
