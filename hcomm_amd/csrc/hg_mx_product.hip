@@ -425,7 +425,8 @@ template <int DT, uint32_t F> __device__ __forceinline__ void store_results(cons
                 for (uint32_t e = 0; e < 4u; ++e) r.w[4u * h + e] = v[e];
             }
             const uint32_t m = m0 + i0 * 32u + row;
-            if (m < rows) store8<DT>((uint8_t*)dst + m * dst_stride * ES, n0 + col, cols, r);
+            // from the wavefront's first column on: a row may be longer than 2^32 bytes
+            if (m < rows && n0 < cols) store8<DT>((uint8_t*)dst + (m * dst_stride + n0) * ES, col, cols - n0, r);
         }
         __builtin_amdgcn_wave_barrier();
     }

@@ -40,6 +40,7 @@ template <> struct GroupVec<DT_F32> {
 // soon.  A group that the row's end cuts is read as the row's last eight elements, which settle8, called where the group is
 // used, moves to where they belong: no load waits for another.  `short_row`: the whole row has fewer than eight (uniform).
 // ask8_into: where a row ends before the group, what was there stays (a buffer that is used again needs its zeros once).
+// Here and in store8 `at` counts from `row` in 32 bits of bytes: in a row that may be longer, `row` is a place near the group.
 template <int DT, bool TAIL, bool NT> __device__ __forceinline__ void ask8_into(Raw8<DT>& r, const void* row, uint32_t at, uint64_t cols, bool short_row)
 {
     constexpr uint32_t ES = ElemSize<DT>::v, W = Raw8<DT>::words;
