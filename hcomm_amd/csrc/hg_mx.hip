@@ -134,13 +134,15 @@ template <int DT, bool ONE, uint32_t U> __global__ __launch_bounds__(256) void k
 
 constexpr uint32_t FOLD_BATCH = 8;
 
-// fp64 to fp32, rounded to odd: what a further rounding to fewer bits makes of it is what it would make of the fp64 value
+// fp64 to fp32, rounded to odd: what a further rounding to fewer bits makes of it is what it would make of the fp64 value.
+// A finite value past fp32's range becomes fp32's largest number, whose last bit is odd: infinite in a narrower dense type, and
+// in a block elements under the largest scale that fp32 numbers have.
 __device__ __forceinline__ float to_odd(double v)
 {
     float f = (float)v;
     const double back = (double)f;
     uint32_t u = f32_bits(f);
-    if (back != v && (u & 0x7f800000u) != 0x7f800000u && !(u & 1u)) u += (__builtin_fabs(v) > __builtin_fabs(back)) ? 1u : 0xffffffffu;
+    if (back != v && (u & 0x7fffffffu) <= 0x7f800000u && !(u & 1u)) u += (__builtin_fabs(v) > __builtin_fabs(back)) ? 1u : 0xffffffffu;
     return bits_f32(u);
 }
 

@@ -1065,8 +1065,9 @@ typedef struct {
 
 /*
  * out = src in the format above.  A block's scale is 2^(E - 2), E the exponent of its largest magnitude (never below
- * 2^-127); elements go to the nearest value, at the middle to the even code, above 6 x scale to 6 x scale; signs are
- * kept, zeros' too.  A block that holds an infinity or a NaN becomes s = 255 with elements 0.  cols up to 2^34.
+ * 2^-127 and never above 2^125, as E is 127 for fp32's largest numbers); elements go to the nearest value, at the middle
+ * to the even code, above 6 x scale to 6 x scale; signs are kept, zeros' too.  A block that holds an infinity or a NaN
+ * becomes s = 255 with elements 0.  cols up to 2^34.
  * rows == 0 or cols == 0 succeed without doing anything.  (Its gradient is the identity.)
  */
 int32_t HcommGfxMxQuantizeOnThread(
@@ -1076,6 +1077,7 @@ int32_t HcommGfxMxQuantizeOnThread(
 /*
  * The fold of k ranks' quantised contributions: v = addend + srcs[0] + .. + srcs[k-1], every element of it, then
  * dst = v rounded once to dstType and / or again = v quantised as above (from v, not from dst).  1 <= k <= HCOMM_GFX_MAX_RANKS.
+ * A finite v of 2^128 and more is infinite in dst; in again its block has the scale 2^125 and it is an element of 6 x 2^125.
  * Every contribution is taken as its fp32 value (2^128 and above: infinite) and the sum is that of fp64, so it is exact,
  * and does not depend on the ranks' order, where its terms span no more than 53 bits.  addend (dstType, or NULL: the own
  * contribution in full precision) may be dst itself with the same stride.  One of dst and again may be NULL.
