@@ -1,0 +1,23 @@
+"""Which form every product of the GPU tests takes: a rule that moves may not leave a form without its tests (no GPU)."""
+import pytest
+
+import test_gpu_mx as mx
+from product_forms import DIRECT_16, DIRECT_32, MID_128, MID_64, SIZES, TILE, WAVE_32, form_of
+
+
+@pytest.mark.parametrize("form", sorted(SIZES))
+def test_sizes_by_form(form):
+    for size in SIZES[form]:
+        assert form_of(*size) == form, size
+
+
+def test_sizes_of_the_other_product_tests():
+    assert [form_of(*s) for s in mx.PRODUCTS] == [DIRECT_16] * 13 + [DIRECT_32] * 2 + [MID_64] * 2
+    assert [form_of(*s) for s in mx.SHORT] == [WAVE_32, WAVE_32, DIRECT_32, DIRECT_32, DIRECT_32, WAVE_32, WAVE_32, MID_128, MID_64, MID_128, WAVE_32, MID_128]
+    assert form_of(1, (1 << 30) + 5003, 256, 1) == TILE
+
+
+def test_rows_of_few_blocks_take_no_form_of_whole_stages():
+    for cols in (1, 32, 100, 224):
+        assert form_of(2900, 2900, cols, 1) == WAVE_32
+    assert form_of(2900, 2900, 225, 1) == TILE
