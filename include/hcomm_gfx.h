@@ -1146,8 +1146,9 @@ int32_t HcommGfxReduceNormOnThread(ThreadHandle thread, const HcommGfxReduceNorm
  *     dSum      = the gradient of h with respect to s, applied to g * D: every partial's gradient is this one
  *     dPostWeight = g * D * s / rms(s), dPreWeight = dz * y / rms(y), summed over the rows
  * A parameter's gradient may be NULL where it is not wanted and has to be NULL where the parameter is; it has
- * paramType, and is 0 for rows == 0.  Sums over rows are fp32 in a fixed order: the same call gives the same bits.  preWeight and dz are both given
- * or both NULL.  dSum may be sum or dy, dResidual may be y or dy, with the same stride each.
+ * paramType.  For rows == 0 the weights' gradients are 0; the gate has ceil(rows / rowsPerGate) rows, none then, and dGate
+ * is left as it was.  Sums over rows are fp32 in a fixed order: the same call gives the same bits.  preWeight and dz are
+ * both given or both NULL.  dSum may be sum or dy, dResidual may be y or dy, with the same stride each.
  * workspace: HcommGfxReduceNormGradWorkspaceBytes(desc) bytes on a 16-byte boundary that no call in flight on another
  * stream uses (NULL where that is 0); the contents do not matter before and after.
  */
