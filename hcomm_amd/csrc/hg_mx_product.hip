@@ -676,7 +676,8 @@ template <int DT, bool SHORT, uint32_t N> int launch(hipStream_t st, const HgMxP
         case HG_PRODUCT_DIRECT_16: hipLaunchKernelGGL((k_mx_product_direct<DT, 1, 1, 8, SHORT, N>), g, dim3(512), 0, st, p); break;
         case HG_PRODUCT_DIRECT_32: hipLaunchKernelGGL((k_mx_product_direct<DT, 2, 2, 8, SHORT, N>), g, dim3(512), 0, st, p); break;
         case HG_PRODUCT_WAVE_32: // of short rows alone
-            if (SHORT) hipLaunchKernelGGL((k_mx_product_direct<DT, 2, 2, 1, true, N>), g, dim3(64), 0, st, p);
+            if (!SHORT) return HCCL_E_INTERNAL;
+            hipLaunchKernelGGL((k_mx_product_direct<DT, 2, 2, 1, true, N>), g, dim3(64), 0, st, p);
             break;
         case HG_PRODUCT_MID_64:
             if (a->cols % HCOMM_GFX_MX_BLOCK) hipLaunchKernelGGL((k_mx_product_mid<DT, 1, true, N>), g, dim3(256), 0, st, p);
