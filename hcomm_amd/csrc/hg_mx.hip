@@ -3,10 +3,10 @@
 // A block is 32 elements of a row under one power-of-two scale, 16 bytes of elements and one of scale.  Both kernels
 // give a lane eight elements - one dword of packed elements - and a block four neighbouring lanes, which find the
 // block's largest magnitude among themselves (two lane exchanges inside the quad, no LDS).  Both are bound by memory once
-// there is enough of it: 67.1M bf16 elements are quantised in 28 us (170 MB, 6.1 TB/s) and turned back in 25; the fold of seven
-// ranks' 14.3M elements into fp32 takes 21 us (110 MB, 5.2 TB/s), that of 8.4M onto an addend, dense and quantised again, 16 us
-// (69 MB, 4.2 TB/s: a conversion for every pair of elements and rank, and fp64 sums, show).  8 x 16,384 elements: 3.8 us, the
-// latency of a launch, two loads and a store.
+// there is enough of it (medians of the kernels' durations): 67.1M bf16 elements are quantised in 29.4 us (170 MB, 5.8 TB/s) and
+// turned back in 25.1; the fold of seven ranks' 14.3M elements into fp32 takes 22.4 us (110 MB, 4.9 TB/s), that of 8.4M onto an
+// addend, dense and quantised again, 18.0 us (69 MB, 3.8 TB/s: a conversion for every pair of elements and rank, and fp64 sums,
+// show).  8 x 16,384 elements: 4.5 us, the latency of a launch, two loads and a store.
 #include "hg_ops_device.hpp"
 
 namespace {

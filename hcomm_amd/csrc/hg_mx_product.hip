@@ -138,7 +138,8 @@ template <uint32_t N> struct ProductArgs {
 // a fixed order.
 // SHORT: ranks of fewer than 16 blocks.  A chunk holds fours of blocks there, EACH of them: those of one rank, so that the
 // ranks spread over the wavefronts, or with a single wavefront the next four of all ranks' fours.
-// One row of 8 ranks' 1,024 columns times 8,192 rows: 7.4 us for 35.7 MB, bound by the loads' latency and memory.
+// One row of 8 ranks' 1,024 columns times 8,192 rows: 8.9 us for 35.7 MB (8.5 in a row of such calls), bound by the loads' latency
+// and memory.
 template <int DT, int FA, int FB, uint32_t W, bool SHORT, uint32_t N> __global__ __launch_bounds__(64 * W) void k_mx_product_direct(const ProductArgs<N> a)
 {
     __shared__ f32x4 part[W > 1u ? W : 1u][W > 1u ? FA * FB : 1][W > 1u ? 64 : 1];
@@ -267,8 +268,9 @@ template <int DT, int FA, int FB, uint32_t W, bool SHORT, uint32_t N> __global__
 // the lanes that need them, each would touch 32 lines for a quarter of the lanes' worth of new bytes.
 // The wavefronts meet once a stage, before its last quarter is multiplied: by then everything of the stage is in
 // registers, its buffer takes the stage after the next, and the fragments of the next one arrive behind that quarter.
-// 4,096 x 8,192 results of 8 x 1,024 columns: 138 us, 4.0 PFLOP/s.  The matrix instructions alone would take 90 (random operands
-// hold the clock down: 6.1 PFLOP/s), all of it without the copies 120; what is left is the copies' latency at 64 KiB a stage.
+// 4,096 x 8,192 results of 8 x 1,024 columns: 139 to 142 us, 3.9 PFLOP/s.  The matrix instructions alone, on random operands
+// (which hold the clock down) in a loop, reach 6.0 PFLOP/s: 91 us.  The matrix units are busy 51 % of the time; what is left is the
+// wait for the copies of 64 KiB a stage, once a stage.
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint64_t u64_at1 __attribute__((aligned(1)));
@@ -309,13 +311,15 @@ __device__ __forceinline__ Side place_side(const HgMxView& v, uint32_t row0, uin
 
 // The stage that begins at block `first` on its way to LDS.  Past the rows' last block that block is copied once more;
 // its scale is 0 (fetch_scales), and with 2^-127 on both sides the products are far below what fp32 holds.
-__device__ __forceinline__ void copy_stage(lds_byte* to, const Side& s, const HgMxView& v, uint32_t row0, uint32_t wave, uint32_t lane, uint32_t first, uint32_t blocks)
+__device__ __forceinline__ void copy_stage(lds_byte* to, const Side& s, const HgMxView& v, uint32_t row0, uint32_t wave, uint32_t lane,
+                                           uint32_t first, uint32_t blocks)
 {
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(v.packed + (uint64_t)row0 * v.packed_stride, 0, (int)s.bytes, HG_BUFFER_WORD3);
     const uint32_t at = s.lane_at + min(first + ((lane & 7u) ^ (lane >> 3)), blocks - 1u) * HCOMM_GFX_MX_BLOCK_BYTES;
 #pragma unroll
     for (uint32_t i = 0; i < 8u; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + (wave * 8u + i) * 1024u), 16, (int)(at + s.rows_at[i]), 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + (wave * 8u + i) * 1024u), 16,
+                                                 (int)(at + s.rows_at[i]), 0, 0, 0);
 }
 
 // the eight scales of this lane's row; the host takes this form from STAGE_BLOCKS blocks on
@@ -360,11 +364,13 @@ __device__ __forceinline__ void read_scales(Scales& s, lds_u64* sa, lds_u64* sb,
 }
 
 // T: the instruction of the stage; I0 .. I1: which fragments of a
-template <uint32_t T, uint32_t I0, uint32_t I1> __device__ __forceinline__ void multiply(f32x16 (&acc)[4][4], const Fragments& f, const Scales& s, uint32_t shift)
+template <uint32_t T, uint32_t I0, uint32_t I1>
+__device__ __forceinline__ void multiply(f32x16 (&acc)[4][4], const Fragments& f, const Scales& s, uint32_t shift)
 {
     uint32_t xa[4], xb[4];
 #pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i) xa[i] = (uint32_t)(s.a[i] >> (32u * (T / 2u))) >> shift, xb[i] = (uint32_t)(s.b[i] >> (32u * (T / 2u))) >> shift;
+    for (uint32_t i = 0; i < 4u; ++i)
+        xa[i] = (uint32_t)(s.a[i] >> (32u * (T / 2u))) >> shift, xb[i] = (uint32_t)(s.b[i] >> (32u * (T / 2u))) >> shift;
 #pragma unroll
     for (uint32_t i = I0; i < I1; ++i)
 #pragma unroll
@@ -387,14 +393,16 @@ template <int N> __device__ __forceinline__ void behind_each(bool reads, bool lo
 // The results of a wavefront, 32 F x 32 F of them from (m0, n0) on, to dst.  Four neighbours of a row lie in a lane; by way of
 // LDS (32 KiB of the wavefront's own) they become runs of a row that a store instruction writes in one piece.  All copies have
 // arrived and all wavefronts are done with what they read when this begins.
-template <int DT, uint32_t F> __device__ __forceinline__ void store_results(const f32x16 (&acc)[F][F], lds_byte* mine, uint32_t lane, void* dst, uint64_t dst_stride, uint32_t m0, uint32_t n0, uint32_t rows, uint32_t cols)
+template <int DT, uint32_t F>
+__device__ __forceinline__ void store_results(const f32x16 (&acc)[F][F], lds_byte* mine, uint32_t lane, void* dst, uint64_t dst_stride,
+                                              uint32_t m0, uint32_t n0, uint32_t rows, uint32_t cols)
 {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     constexpr uint32_t ES = ElemSize<DT>::v, EDGE = 32u * F, PASS = EDGE * EDGE * ES > 32768u ? F / 2u : F; // fragments of rows at a time
-    constexpr uint32_t ROW = EDGE * ES, SWAP = (ROW / 16u < 32u ? ROW / 16u : 32u) - 1u;                     // bytes of a row; its chunks of 16 change places by row
-    constexpr uint32_t LANES = EDGE / 8u;                                                                    // that read a row
+    constexpr uint32_t ROW = EDGE * ES, SWAP = (ROW / 16u < 32u ? ROW / 16u : 32u) - 1u; // bytes of a row; its chunks of 16 change places by row
+    constexpr uint32_t LANES = EDGE / 8u;                                                // that read a row
 #pragma unroll
     for (uint32_t i0 = 0; i0 < F; i0 += PASS) {
 #pragma unroll
@@ -534,7 +542,8 @@ template <int DT, bool TAIL, uint32_t N> __global__ __launch_bounds__(256) void 
         STAGE(a0, b0, a1, b1, 1)
         STAGE(a1, b1, a0, b0, 0)
     }
-    store_results<DT, 4>(acc, (lds_byte*)(wave == 0u ? a0 : wave == 1u ? b0 : wave == 2u ? a1 : b1), lane, a.dst, a.dst_stride, m0 + wm * 128u, n0 + wn * 128u, a.m, a.n);
+    lds_byte* mine = (lds_byte*)(wave == 0u ? a0 : wave == 1u ? b0 : wave == 2u ? a1 : b1);
+    store_results<DT, 4>(acc, mine, lane, a.dst, a.dst_stride, m0 + wm * 128u, n0 + wn * 128u, a.m, a.n);
 }
 
 // ---- fewer rows: smaller tiles, more stages under way -------------------------------------------------------------------
@@ -573,8 +582,8 @@ template <int DT, uint32_t F, bool TAIL, uint32_t N> __global__ __launch_bounds_
         uint32_t back, first; // how many scales the fetch went back; the stage's first block
     } q0, q1, q2, q3;
     auto copy = [&](lds_byte* to, const HgMxView& v, uint32_t row0, uint32_t last, uint32_t stride, uint32_t first) {
-        const __amdgpu_buffer_rsrc_t r =
-            __builtin_amdgcn_make_buffer_rsrc(v.packed + (uint64_t)row0 * v.packed_stride, 0, (int)(last * stride + blocks * HCOMM_GFX_MX_BLOCK_BYTES), HG_BUFFER_WORD3);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            v.packed + (uint64_t)row0 * v.packed_stride, 0, (int)(last * stride + blocks * HCOMM_GFX_MX_BLOCK_BYTES), HG_BUFFER_WORD3);
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i) {
             const uint32_t row = copy_row + i * 4u * F, block = min(first + ((place & ~7u) | ((place ^ row) & 7u)), blocks - 1u);
@@ -582,7 +591,8 @@ template <int DT, uint32_t F, bool TAIL, uint32_t N> __global__ __launch_bounds_
                                                      (int)(row * stride + block * HCOMM_GFX_MX_BLOCK_BYTES), 0, 0, 0);
         }
     };
-    uint32_t rank = 0, first = 0; // of the next stage to ask for; behind the last one that stage again and again, so that what is under way can be counted
+    // of the next stage to ask for; behind the last one that stage again and again, so that what is under way can be counted
+    uint32_t rank = 0, first = 0;
     auto ask = [&](lds_byte* to, Stage& q) {
         const HgMxView &va = a.a[rank], &vb = a.b[rank];
         copy(to, va, m0, last_a, stride_a, first);
@@ -600,7 +610,8 @@ template <int DT, uint32_t F, bool TAIL, uint32_t N> __global__ __launch_bounds_
     uint32_t done = 0;
     auto meet = [&](lds_byte* in, uint32_t set, const Stage& q) {
         asm volatile("s_waitcnt vmcnt(18)" ::: "memory");
-        if (TAIL && lane < 16u * F) { // elements of the last block past cols do not count: they become 0 in the rows of a that this wavefront has copied
+        if (TAIL && lane < 16u * F) {
+            // elements of the last block past cols do not count: they become 0 in the rows of a that this wavefront has copied
             const uint32_t last = blocks - 1u - q.first, row = wave * 16u * F + lane; // last: the block in its stage, if it is there
             const uint32_t n = last < LONG ? a.cols - (blocks - 1u) * HCOMM_GFX_MX_BLOCK : HCOMM_GFX_MX_BLOCK, at = last < LONG ? last : 0u;
             lds_vec* p = (lds_vec*)(in + row * ROW + ((at & ~7u) | ((at ^ row) & 7u)) * HCOMM_GFX_MX_BLOCK_BYTES);
@@ -663,7 +674,8 @@ template <int DT, uint32_t F, bool TAIL, uint32_t N> __global__ __launch_bounds_
         multiply((lds_byte*)s3, 3);
         if (done == total) break;
     }
-    store_results<DT, F>(acc, (lds_byte*)(wave == 0u ? s0 : wave == 1u ? s1 : wave == 2u ? s2 : s3), lane, a.dst, a.dst_stride, m0 + wm * 32u * F, n0 + wn * 32u * F, a.m, a.n);
+    lds_byte* mine = (lds_byte*)(wave == 0u ? s0 : wave == 1u ? s1 : wave == 2u ? s2 : s3);
+    store_results<DT, F>(acc, mine, lane, a.dst, a.dst_stride, m0 + wm * 32u * F, n0 + wn * 32u * F, a.m, a.n);
 }
 
 template <int DT, bool SHORT, uint32_t N> int launch(hipStream_t st, const HgMxProduct* a)

@@ -2,10 +2,10 @@
 //
 // One pass over memory: the wavefronts that share a row keep it in registers (eight elements a lane and group, 64 lanes a
 // wavefront), so k partials and the residual are read once, the sums over the row cross the lanes twice and everything
-// in between never leaves the registers.  Bound by memory from a few hundred rows on (8,192 x 4,096 bf16 of eight ranks: 137 us
-// for 805 MB, 5.9 TB/s; its gradient: 80 us and 4 for the join, 403 MB, 4.8 TB/s); a single row is bound by the latency of its load,
-// two reductions and store (5.4 us at 8,192 columns of eight ranks).  Rows that do not begin on cache lines take up to half
-// as long again: every access of a wavefront touches a line more, and neighbouring rows share theirs.
+// in between never leaves the registers.  Bound by memory from a few hundred rows on (medians of the kernels' durations, 8,192 x
+// 4,096 bf16 of eight ranks: 138 us for 805 MB, 5.8 TB/s; its gradient: 79 us and 4.6 for the join, 403 MB, 4.8 TB/s); a single row
+// is bound by the latency of its load, two reductions and store (5.3 us at 8,192 columns of eight ranks).  Rows that do not begin
+// on cache lines take up to half as long again: every access of a wavefront touches a line more, and neighbouring rows share theirs.
 #include "hg_ops_device.hpp"
 
 namespace {
@@ -38,8 +38,9 @@ __device__ __forceinline__ float wave_sum(float v)
 // What a workgroup has: one row, several of whole wavefronts (1 or 2 each), or several of 1 to 32 lanes.
 enum { ONE_ROW, WAVES, LANES };
 
-// N sums over the `span` lanes that share a row, the same in all of them.  Across wavefronts, at most 16: lane w of every 16 fetches wavefront w's sum from `box`, which holds N floats for each wavefront of
-// the workgroup and is not written again before every wavefront has passed another barrier.
+// N sums over the `span` lanes that share a row, the same in all of them.  Across wavefronts, at most 16: lane w of every 16
+// fetches wavefront w's sum from `box`, which holds N floats for each wavefront of the workgroup and is not written again before
+// every wavefront has passed another barrier.
 template <uint32_t N, int SHARE> __device__ __forceinline__ void row_sum(float (&v)[N], float* box, uint32_t span)
 {
     if (SHARE == LANES) {
@@ -89,8 +90,11 @@ template <uint32_t N> struct NormArgs {
 
 // DT: type of the matrices, PT: of the parameters, V: groups of eight elements a lane holds, SHARE: a workgroup has one row
 // (where it begins is a scalar then), several of whole wavefronts, or several of fewer lanes, TAIL: rows end inside a group,
-// NT: larger than the L2s, so that what is read once and what is written passes by them (8,192 x 4,096 of eight ranks 153 -> 138 us; rows off 16-byte boundaries share lines, which
-// has to be fetched again then), N: most ranks
+// NT: what is read once and what is written passes by the L2s, N: most ranks.
+// NT is taken for rows of whole groups that move more than the L2s hold.  8,192 x 4,096 of eight ranks without / with it, us:
+// 154 / 139, as a view with a row every 4,099 elements, whose rows share lines, 184 / 174, 4,096 x 8,200: 207 / 203.  More than eight
+// ranks take it at any size (with it alone compiled): 16 ranks' 8,192 x 4,096 252 / 216, 1,024 rows 37.5 / 34.5, 64 rows 9.8 / 11,
+// a row of 8,192 7.9 / 7.9.  Rows that end inside a group do without: neighbours share lines that would be fetched again.
 template <int DT, int PT, uint32_t V, int SHARE, bool TAIL, bool NT, uint32_t N> __global__ __launch_bounds__(1024) void k_norm(const NormArgs<N> a)
 {
     __shared__ float box[2][MAX_WAVES];
@@ -221,7 +225,8 @@ template <int DT, int PT, uint32_t V, int SHARE, bool TAIL, bool NT, uint32_t N>
 //   in registers that spill); LEAN with V = 1 and 16 wavefronts: 200;
 //   LEAN with V = 2 above: 167 to 170 (fp32 270 to 285); 815 and more with everything held and spilled, 228 to 255 (fp32 335) with
 //   rows read again for each of their uses.  Bound by the latency of a row's loads, with one workgroup to a CU.
-template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool TAIL, bool NT> __global__ __launch_bounds__(MOST) void k_norm_grad(const HgNormGrad a)
+template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool TAIL, bool NT>
+__global__ __launch_bounds__(MOST) void k_norm_grad(const HgNormGrad a)
 {
     __shared__ float box_a[MAX_WAVES * 3], box_b[MAX_WAVES];
     constexpr uint32_t ES = ElemSize<DT>::v, PS = ElemSize<PT>::v;
@@ -297,7 +302,8 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool T
     if (!LEAN && row < end) ask_row(next, row);
     uint32_t gate_row = 0u, gate_end = 0u; // the row of the gate, and the row at which its next one begins
     Raw8<HT> post[HELD], pre[HELD], gate[HELD];
-    Raw8<PT> asked[HT == PT ? 1u : HELD]; // a row of the gate that is asked for and not settled, where `fresh`; else it goes to `gate` at once
+    // a row of the gate that is asked for and not settled, where `fresh`; else it goes to `gate` at once
+    Raw8<PT> asked[HT == PT ? 1u : HELD];
     bool fresh = false;
     auto take_gate = [&](uint32_t r) {
         gate_row = r / (uint32_t)a.d.rowsPerGate;
@@ -314,7 +320,8 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool T
     };
     if (!LEAN) {
 #pragma unroll
-        for (uint32_t v = 0; v < HELD; ++v) pre[v] = hold(a.d.preWeight, v, 0.0f), post[v] = hold(a.d.postWeight, v, 1.0f), gate[v] = hold(nullptr, v, 1.0f);
+        for (uint32_t v = 0; v < HELD; ++v)
+            pre[v] = hold(a.d.preWeight, v, 0.0f), post[v] = hold(a.d.postWeight, v, 1.0f), gate[v] = hold(nullptr, v, 1.0f);
     }
     if (has_gate && row < end) take_gate(row);
     float d_post[8], d_pre[8], d_gate[8];
@@ -499,8 +506,8 @@ template <int DT, int PT, uint32_t V, uint32_t MOST, bool SUB, bool LEAN, bool T
     }
 }
 
-// The runs' sums joined, in a fixed order (4 us: the latency of a launch and of a chain of loads): a workgroup takes 64 columns of one result, four neighbours to a lane, and 64
-// of its lanes share a column's runs.
+// The runs' sums joined, in a fixed order (4.6 to 4.9 us: the latency of a launch and of a chain of loads): a workgroup takes 64
+// columns of one result, four neighbours to a lane, and 64 of its lanes share a column's runs.
 #define SUM_COLS 64u
 
 template <int PT> __global__ __launch_bounds__(1024) void k_norm_sums(const HgNormGrad a)
@@ -560,7 +567,8 @@ template <int DT, int PT, uint32_t V, int SHARE, bool TAIL, bool NT, uint32_t N>
 template <int DT, int PT, uint32_t V, int SHARE> int launch_norm_v(hipStream_t st, const HgNorm* a)
 {
     if (a->d.cols % 8u)
-        return a->d.k <= 8u ? launch_norm_n<DT, PT, V, SHARE, true, false, 8>(st, a) : launch_norm_n<DT, PT, V, SHARE, true, false, HCOMM_GFX_MAX_RANKS>(st, a);
+        return a->d.k <= 8u ? launch_norm_n<DT, PT, V, SHARE, true, false, 8>(st, a)
+                            : launch_norm_n<DT, PT, V, SHARE, true, false, HCOMM_GFX_MAX_RANKS>(st, a);
     if (a->d.k > 8u) return launch_norm_n<DT, PT, V, SHARE, false, true, HCOMM_GFX_MAX_RANKS>(st, a);
     return a->stream ? launch_norm_n<DT, PT, V, SHARE, false, true, 8>(st, a) : launch_norm_n<DT, PT, V, SHARE, false, false, 8>(st, a);
 }
@@ -627,7 +635,8 @@ int hg_launch_norm_sums(void* stream, const void* args)
     const HgNormGrad* a = (const HgNormGrad*)args;
     OnDeviceOf device((hipStream_t)stream);
     if (device.err != hipSuccess) return HCCL_E_RUNTIME;
-    const dim3 g((uint32_t)((a->d.cols + SUM_COLS - 1u) / SUM_COLS), (uint32_t)((a->at_post >= 0) + (a->at_pre >= 0) + (a->at_gate >= 0 ? a->gates : 0u))), b(1024);
+    const uint64_t results = (a->at_post >= 0) + (a->at_pre >= 0) + (a->at_gate >= 0 ? a->gates : 0u);
+    const dim3 g((uint32_t)((a->d.cols + SUM_COLS - 1u) / SUM_COLS), (uint32_t)results), b(1024);
     switch (a->d.paramType) {
         case HCOMM_DATA_TYPE_FP16: hipLaunchKernelGGL((k_norm_sums<DT_F16>), g, b, 0, (hipStream_t)stream, *a); break;
         case HCOMM_DATA_TYPE_BFP16: hipLaunchKernelGGL((k_norm_sums<DT_BF16>), g, b, 0, (hipStream_t)stream, *a); break;

@@ -237,8 +237,11 @@ static uint64_t product_wgs(const HgMxProduct* a, uint32_t edge) { return (uint6
  * 64 / 128 / 256): m = 16: 12.3 / 11.3 / 12.4 / 23 / 47, m = 64: 33 / 21 / 13 / 23 / 47, m = 256: 121 / 76 / 25.5 / 25.1 / 50,
  * m = 512: 240 / 151 / 48 / 30 / 50, m = 1,024: 477 / 299 / 92 / 59 / 54, m = 4,096: 1,894 / 1,186 / 389 / 212 / 140; 200 x 200 x 512:
  * 2.7 / 3.1 / 3.5 / 4.8 / 10.4, 300 x 300 x 4,096: 7.1 / 6.8 / 7.3 / 14 / 32, 512 x 512 x 2,048: 7.4 / 5.0 / 5.4 / 8.5 / 18,
- * 33 x 8,000 x 2,048: 10.5 / 8.7 / 5.8 / 8.7 / 17, 300 x 1,200 x 4,096 with edge 32 / 64: 13.2 / 8.7.  Edge 32 has one workgroup to a CU: up to
- * 256 tiles of it run at once.
+ * 33 x 8,000 x 2,048: 10.5 / 8.7 / 5.8 / 8.7 / 17, 300 x 1,200 x 4,096 with edge 32 / 64: 13.2 / 8.7.  Edge 32 has one workgroup to a
+ * CU: up to 256 tiles of it run at once.
+ * The rule counts tiles, not how full they are: more than 16,256 rows of b make enough tiles for edge 128, more than 32,512 for
+ * 256, whatever m is.  Few rows of a lose by it (8 ranks' 1,024 columns, m = 1: n = 16,256 15.5 us, 16,384 24.3; n = 32,512 32.9, 32,768
+ * 56.9; m = 64: 16.6 / 25.3, 35.0 / 59.6); the smaller edges have not been measured there.
  * Rows of fewer than 16 blocks: a wavefront for every 32 x 32 results instead of eight that share so little, from about as many
  * tiles on as a wavefront takes fours of blocks (8 wavefronts / 1 / edge 64 / 128): 1,024 x 1,024 results of one rank's 32 columns
  * 6.7 / 3.4, of four ranks' 165 8.3 / 5.6, of 16 ranks' 30 9.6 / 8.3; 512 x 512 of 8 ranks' 32 3.3 / 4.8; 4,096 x 8,192 of one rank's 32
@@ -284,7 +287,8 @@ int32_t HcommGfxMxProductKOnThread(
     if (!es || cols == 0) return HCCL_E_PARA;
     HgMxProduct p;
     memset(&p, 0, sizeof(p));
-    int rc = m > HG_LIMIT_ROWS - 512u || n > HG_LIMIT_ROWS - 512u || mx_blocks(cols) * HCOMM_GFX_MX_BLOCK_BYTES >= HG_MX_PRODUCT_STRIDE ? HCCL_E_NOT_SUPPORT : HCCL_SUCCESS;
+    const int large = m > HG_LIMIT_ROWS - 512u || n > HG_LIMIT_ROWS - 512u || mx_blocks(cols) * HCOMM_GFX_MX_BLOCK_BYTES >= HG_MX_PRODUCT_STRIDE;
+    int rc = large ? HCCL_E_NOT_SUPPORT : HCCL_SUCCESS;
     if (rc == HCCL_SUCCESS) {
         Range r[1 + 4 * HCOMM_GFX_MAX_RANKS];
         memset(r, 0, sizeof(r));
@@ -392,6 +396,8 @@ int32_t HcommGfxReduceNormOnThread(ThreadHandle thread, const HcommGfxReduceNorm
  * Runs of rows: as many as run at once, with up to 8 wavefronts to each of the CUs (their registers allow no more).  Enough to
  * keep every CU loading, few enough that the runs' sums stay a small part of the traffic; a few more than that would have the
  * card wait for a second turn (5,461 x 6,144 bf16: 341 runs of 6 wavefronts 129 us).
+ * With the gate's gradient a run ends with a row of the gate, so that numbers of gate rows just above half or all of these runs
+ * leave CUs without one: gates of 128 rows x 4,096 take 1.21 us each where there are 192 or 256, 1.55 where 129, 1.49 where 257.
  */
 #define HG_NORM_GRAD_CUS 256u
 #define HG_NORM_GRAD_WAVES 8u

@@ -1033,15 +1033,17 @@ uint64_t HcommGfxSetPieceBytes(uint64_t bytes);
  * 5. Operators around a fold (no reference counterpart)
  *
  * Every call is asynchronous on the thread's stream, allocates nothing, keeps nothing after it returns and may be
- * captured into a graph.  Checks come in this order: pointers (HCCL_E_PTR, an invalid thread last), then sizes, types,
- * alignment and overlaps (HCCL_E_PARA), a limit of this library (HCCL_E_NOT_SUPPORT), a call between
- * HcommBatchModeStart and HcommBatchModeEnd (HCCL_E_NOT_SUPPORT), a thread that holds recorded operations of another
- * host thread's batch (HCCL_E_UNAVAIL).  After a refusal nothing was queued.
+ * captured into a graph.  Refusals: HCCL_E_PTR for pointers and an invalid thread, HCCL_E_PARA for sizes, types, alignment
+ * and overlaps, HCCL_E_NOT_SUPPORT for a limit of this library and for a call between HcommBatchModeStart and
+ * HcommBatchModeEnd, HCCL_E_UNAVAIL for a thread that holds recorded operations of another host thread's batch; they are
+ * looked for about in this order (a number of ranks before the pointers that it counts, a workspace behind the sizes that
+ * it follows from, sizes past a limit before their overlaps).  After a refusal nothing was queued.
  * Dense matrices are row-major, `Stride` is the distance of two rows in ELEMENTS and at least the row's length; any
  * element-aligned address and any stride are taken.  Nothing outside the rows x cols elements is read or written.
  * Dense types: FP16, BFP16, FP32.  Outputs overlap no input and no other output unless a call says so.
- * A call whose launch would need 2^32 lanes or more is beyond the library's limit: a lane takes up to eight elements of a row, a
- * result of a product two lanes at most.
+ * A call whose launch would need 2^32 lanes or more is beyond the library's limit: a lane takes up to eight elements of a
+ * row, a result of a product two lanes at most.  So are 2^31 rows of the norms, m or n above 2^31 - 513 and inner lengths
+ * above 2^24 - 32 of a product.
  * The work runs on the device of the thread's stream, whatever the caller's current device.
  * ------------------------------------------------------------------------------------------- */
 
